@@ -220,14 +220,15 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------------------------
 # the package's calls
 # ---------------------------------------------------------------------------------------------
-_rt = None
+_rt = _scratch = None
 
 
 def _package():
-    global _rt
+    global _rt, _scratch
     vm = importlib.import_module("pjrt-ocl_b200")
     if _rt is None:
         _rt = vm.Runtime.Create(torch.cuda.current_device())
+        _scratch = vm.Scratch.Create(_rt)
     return vm, _rt
 
 
@@ -262,7 +263,7 @@ def _own(s):
         return s["out"]
     if op == "rotate_back":
         s["rope"].ApplyBackward(c["rows"], s["p"][0], r[0], r[1], r[2], r[3], r[4], r[5], q_weight=s["p"][1], k_weight=s["p"][2],
-                                dq_weight=s["p"][3], dk_weight=s["p"][4], stream=stream)
+                                dq_weight=s["p"][3], dk_weight=s["p"][4], scratch=_scratch, stream=stream)
         return s["out"]
     if op == "write":
         s["cache"].Write(s["batch"], r[0], r[1], stream=stream)
@@ -270,7 +271,7 @@ def _own(s):
     if op == "read":
         s["cache"].Read(s["batch"], r[0], r[1], stream=stream)
         return [t[:s["total"]] for t in s["out"]]
-    s["cache"].Attend(s["batch"], r[0], r[1], lse=s["out"][1].data_ptr(), scale=c["dim"] ** -0.5, causal=True, window=c["window"], stream=stream)
+    s["cache"].Attend(s["batch"], r[0], r[1], _scratch, lse=s["out"][1].data_ptr(), scale=c["dim"] ** -0.5, causal=True, window=c["window"], stream=stream)
     return [t[:s["total"]] for t in s["out"]]
 
 
