@@ -59,7 +59,8 @@ typedef struct {
 /* Device-side outcome of the last execute of a loaded program. */
 typedef struct {
   uint32_t code;          /* 0 ok, 1 barrier wait ran out, 2 control stack overflow,
-                             3 unsupported tile op reached, 4 tensor-core wait ran out */
+                             3 unsupported tile op reached, 4 tensor-core wait ran out,
+                             5 and 6 see b2_cache_status */
   uint32_t lane;          /* lane that recorded it */
   uint32_t where;         /* barrier index / entry index */
   uint32_t detail;        /* tile op or extra information */
@@ -204,6 +205,126 @@ size_t b2_loaded_lane_times(b2_loaded *lp, uint64_t *out, size_t cap);
 b2_status b2_sum_f32_static(int device_ordinal, const void *dev_in, uint64_t n_elems, void *dev_out,
                             void *cuda_stream, char *err, size_t err_cap);
 uint64_t b2_sum_f32_static_max_elems(void);
+
+/* ---- operators beside the programs (no counterpart in the reference) --------
+ * What stands between a decoder block's products when the cache is shared by sequences of different lengths: rotary
+ * positions with the norms of queries and keys, a paged cache, and the attention of new rows over it. They take
+ * device buffers of the caller's and enqueue on `cuda_stream` (NULL = the default stream of the runtime's device)
+ * without waiting; they allocate nothing and may be captured into a graph once the handles are made. The device that
+ * is current when a call is made stays current; buffers are the runtime's device's.
+ * A call may be made from any thread; two calls at once are independent of each other, but for what is said below
+ * about b2_scratch and about rows that both write. */
+
+/* Types of rows and pages: the VMProgram enum's values, and 8-bit floats (4 exponent, 3 mantissa bits; no infinity). */
+enum { B2_F32 = 0, B2_F16 = 6, B2_BF16 = 7, B2_E4M3 = 8 };
+
+/* rows x heads x head_dim in device memory, the last axis without gaps; strides in elements. Any alignment the type
+ * has is taken; 16-byte aligned rows and heads are fastest. */
+typedef struct {
+  void *data;
+  int64_t row_stride, head_stride;
+} b2_rows;
+
+/* Scratch for the calls that need any: partial results, and counters that every call leaves at zero. The calls that
+ * share one run one after another (one stream, or streams ordered by events; graphs that hold such calls, too).
+ * A loaded program's rule for its launches, for the same reason. */
+typedef struct b2_scratch b2_scratch;
+b2_status b2_scratch_create(b2_runtime *rt, b2_scratch **out, char *err, size_t err_cap);
+void b2_scratch_destroy(b2_scratch *scratch);
+
+/* -- rotary positions, with the norms of queries and keys in the same pass --
+ * A head's row x (head_dim values) becomes, with `norm`, y = x * w / sqrt(mean(x^2) + eps), else y = x. Its first
+ * rot_dim values are turned by pairs: (a, b) = (y[i], y[i + rot_dim/2]), or (y[2i], y[2i+1]) when `interleaved`,
+ * by the angle position * frequencies[i]: a' = m (a cos - b sin), b' = m (a sin + b cos), m = magnitude. The rest
+ * passes. In f32, the angle in 64 bits (any int32 position is exact to the last f32 bit of its sine), one rounding. */
+typedef struct b2_rope b2_rope;
+typedef struct {
+  uint32_t head_dim, rot_dim;      /* even; head_dim <= 256, rot_dim <= head_dim, 0 = the norms alone */
+  uint32_t q_heads, k_heads;       /* either may be 0: its rows are not touched then */
+  uint32_t dtype;                  /* rows: B2_F32, B2_F16, B2_BF16 */
+  uint32_t weight_dtype;           /* B2_F32, or `dtype` */
+  uint32_t interleaved, norm;
+  float eps;
+  double magnitude;
+  const double *frequencies;       /* host, rot_dim / 2 values, radians for each position; copied */
+} b2_rope_desc;
+/* Frequencies base^(-2i/rot_dim), and their forms for contexts longer than the one trained on (`factor` times):
+ * LINEAR divides them by factor; STRETCH takes base * factor^(rot_dim/(rot_dim-2)); PARTS leaves those that make
+ * `fast` turns or more over original_length, divides those that make `slow` or fewer, and blends between. */
+enum { B2_ROPE_PLAIN = 0, B2_ROPE_LINEAR = 1, B2_ROPE_STRETCH = 2, B2_ROPE_PARTS = 3 };
+b2_status b2_rope_frequencies(uint32_t rot_dim, double base, int scaling, double factor, double original_length,
+                              double slow, double fast, double *out, size_t out_cap, char *err, size_t err_cap);
+b2_status b2_rope_create(b2_runtime *rt, const b2_rope_desc *desc, b2_rope **out, char *err, size_t err_cap);
+void b2_rope_destroy(b2_rope *rope);
+/* positions: device, n_rows int32. Weights: device, head_dim values each; NULL = ones. The results may be written over
+ * the inputs (same data and strides). */
+b2_status b2_rope_apply(const b2_rope *rope, uint32_t n_rows, const void *positions, const b2_rows *q, const b2_rows *k,
+                        const void *q_weight, const void *k_weight, const b2_rows *q_out, const b2_rows *k_out,
+                        void *cuda_stream, char *err, size_t err_cap);
+/* Gradients of b2_rope_apply: q and k are the inputs it had (with norm; else unused and may be NULL), dq_out and dk_out
+ * the gradients of its results, dq and dk those of q and k (they may be written over dq_out and dk_out, or over q and
+ * k). dq_weight / dk_weight: device, head_dim f32 each, written (not added to); either may be NULL. Sums over rows and
+ * heads are in f32 in an order that does not change from call to call. `scratch` is needed for weight gradients only. */
+b2_status b2_rope_apply_backward(const b2_rope *rope, b2_scratch *scratch, uint32_t n_rows, const void *positions,
+                                 const b2_rows *q, const b2_rows *k, const void *q_weight, const void *k_weight,
+                                 const b2_rows *dq_out, const b2_rows *dk_out, const b2_rows *dq, const b2_rows *dk,
+                                 void *dq_weight, void *dk_weight, void *cuda_stream, char *err, size_t err_cap);
+
+/* -- a paged cache of keys and values --
+ * A view of pages that the caller owns: page p, slot s, head h of K starts at k_pages[p * page_stride + s *
+ * slot_stride + h * head_stride] (V alike), head_dim values without a gap; base addresses and strides multiples of 16
+ * bytes. e4m3 pages come with an f32 scale for each (page, slot, head): the values are code * scale. */
+typedef struct b2_cache b2_cache;
+typedef struct {
+  uint32_t dtype;                  /* of the pages: B2_F16, B2_BF16, B2_E4M3 */
+  uint32_t row_dtype;              /* of the rows that go in and out: B2_F16, B2_BF16, B2_F32; 16-bit pages: the same, or B2_F32 */
+  uint32_t heads, q_heads;         /* q_heads: a multiple of heads; query head h reads cache head h / (q_heads / heads) */
+  uint32_t head_dim;               /* a multiple of 16, at most 128 */
+  uint32_t page_size, n_pages;     /* any page_size >= 1 */
+  void *k_pages, *v_pages;
+  int64_t page_stride, slot_stride, head_stride;                       /* elements */
+  float *k_scales, *v_scales;                                          /* e4m3 only */
+  int64_t scale_page_stride, scale_slot_stride, scale_head_stride;     /* elements */
+} b2_cache_desc;
+/* A batch of sequences, on the device but for its bounds. Sequence b has rows row_start[b] .. row_start[b+1] - 1 of the
+ * row tensors, which are its last positions: it is `length[b]` positions long with them, and row i of its n is at
+ * position length[b] - n + i (a row whose position is negative is not written to the cache, and gives zeros). Position
+ * p is slot p % page_size of page pages[b * pages_stride + p / page_size]. Rows from row_start[n_seqs] on (a padded
+ * batch) are left as they are. */
+typedef struct {
+  uint32_t n_seqs;
+  uint32_t n_rows;                 /* rows that the row tensors have: at least row_start[n_seqs] */
+  uint32_t max_rows;               /* the most rows a sequence of the batch has; 0 = not known */
+  uint32_t max_pages;              /* entries of a sequence's page list */
+  int64_t pages_stride;
+  const void *row_start;           /* int32[n_seqs + 1], starting at 0 */
+  const void *length;              /* int32[n_seqs] */
+  const void *pages;               /* int32 */
+} b2_batch;
+b2_status b2_cache_create(b2_runtime *rt, const b2_cache_desc *desc, b2_cache **out, char *err, size_t err_cap);
+void b2_cache_destroy(b2_cache *cache);
+/* The batch's rows of K and V into the pages. e4m3: scale = max|x| / 448 of the row, code = x / scale to the nearest
+ * (ties to even); a row of zeros has scale 0; one that holds a NaN or an infinity reads back as NaN throughout.
+ * Two rows of one call that name the same slot leave a mixture there. */
+b2_status b2_cache_write(b2_cache *cache, const b2_batch *batch, const b2_rows *k, const b2_rows *v, void *cuda_stream,
+                         char *err, size_t err_cap);
+/* The batch's positions out of the pages into rows (all of a sequence: as many rows as positions). */
+b2_status b2_cache_read(b2_cache *cache, const b2_batch *batch, const b2_rows *k, const b2_rows *v, void *cuda_stream,
+                        char *err, size_t err_cap);
+/* out = softmax(scale q k^T) v for the batch's rows over the cache, in one pass. causal: a row sees the keys up to its
+ * own position, of these the last `window` (0 = all); else every position of its sequence (window must be 0). Values
+ * that a row does not see never reach it, whatever they are. A row that sees nothing gives zeros. lse (may be NULL):
+ * f32 [n_rows][q_heads], the logarithm of the softmax's sum (-inf for a row that sees nothing). Rows are B2_F16 or
+ * B2_BF16. scale > 0. */
+b2_status b2_cache_attend(b2_cache *cache, b2_scratch *scratch, const b2_batch *batch, const b2_rows *q, float scale,
+                          int causal, uint32_t window, const b2_rows *out, void *lse, void *cuda_stream, char *err,
+                          size_t err_cap);
+/* Waits for the device and reports the first fault that this cache's calls met since the last report: code 5 = a page
+ * number outside the cache (`lane` = sequence, `where` = entry of its list, `detail` = the number), 6 = a batch that
+ * does not fit its bounds (`lane` = sequence, `detail` = the value: row_start, length or more rows than max_rows).
+ * Nothing outside the buffers is touched then: such keys count as absent, such rows are left out. 4 = a wait on the
+ * tensor cores ran out. Not during stream capture. */
+b2_status b2_cache_status(b2_cache *cache, b2_exec_status *out, char *err, size_t err_cap);
 
 #ifdef __cplusplus
 }

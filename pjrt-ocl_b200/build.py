@@ -13,7 +13,10 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
-SOURCES = ["runtime.cc", "loader.cc", "replan.cc", "vmprog.cc", "static_sum.cu"]
+# the operators beside the programs, and the headers that only they include
+OPERATORS = ["operators.cc", "operators_check.cc", "rope.cu", "paged_cache.cu", "attend_step.cu", "attend_chunk.cu"]
+OPERATOR_HEADERS = ("operators.h", "operators_dev.cuh", "attend_common.cuh")
+SOURCES = ["runtime.cc", "loader.cc", "replan.cc", "vmprog.cc", "static_sum.cu", *OPERATORS]
 KERNEL = "vm_kernel.cu"      # compiled once per entry of csrc/variants.h,
 PLAN_KERNEL = "plan_kernel.cu"   # except the entries named plan*, which are this one's
 OUT = os.path.join(HERE, "libb2vm.so")
@@ -76,9 +79,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
     plan_only = ("plan_format.h", "replan.h", "ops_fuse.cuh", "ops_rowpipe.cuh", "ops_pairs.cuh", "ops_flatpipe.cuh", "ops_gemm.cuh", "ops_sgemm.cuh", "ops_skinny.cuh")
 
     def deps(u):
-        if u[0].endswith(KERNEL):       # the wire builds do not include the planned ops
-            return [u[0], *(h for h in heads if os.path.basename(h) not in plan_only)]
-        return [u[0], *heads]
+        name = os.path.basename(u[0])
+        if name in OPERATORS:
+            return [u[0], *(h for h in heads if os.path.basename(h) in (*OPERATOR_HEADERS, "ptx.cuh", "tc_common.cuh", "dev_common.cuh", "b2vm.h"))]
+        mine = [h for h in heads if os.path.basename(h) not in OPERATOR_HEADERS]
+        if name in (KERNEL, PLAN_KERNEL):     # no kernel of the programs knows the C ABI; the wire builds do not include the planned ops
+            mine = [h for h in mine if os.path.basename(h) not in (("b2vm.h",) if name == PLAN_KERNEL else ("b2vm.h", *plan_only))]
+        return [u[0], *mine]
     jobs = [u for u in units if force or _newer(u[1], deps(u))]
     if jobs:
         with concurrent.futures.ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 1)) as ex:

@@ -1,0 +1,329 @@
+// Rotary positions with the norms of queries and keys in the same pass, and its backward pass.
+//
+// A row x of hd values (one token, one head):  r = 1 / sqrt(mean x^2 + eps),  y = x r w;  pairs (a, b) of the first rot values
+// turn by t = position f_i:  (a', b') = m (a cos t - b sin t, a sin t + b cos t).  Backward, with g = R^T dy and h = w g:
+//   dx = r h - x r^3 / hd sum(h x),   dw = sum over rows and heads of g x r.
+//
+// Bound: HBM. Every row is read once and written once (backward: x and dy read, dx written).
+// A CTA takes some tokens at a time; the angles of its tokens are worked out once, in 64-bit turns (position x turns, less
+// the nearest whole number: exact for every int32 position; sine and cosine of the rest in f32), and shared by all heads. A row
+// belongs to up to 32 threads; a thread holds V pairs of it, both halves of each, so that neither layout needs an exchange
+// between threads: the half layout is two V-wide accesses rot/2 apart, the neighbouring one two that touch. What lies behind
+// rot is treated the same with no angle. V is as wide as the addresses, strides and rot allow up to 16 bytes.
+// Gradients of the weights stay in registers, are joined in shared memory once a CTA, and a second small launch adds the CTAs'
+// sums in their order, so that a result does not change from call to call.
+#include "operators_dev.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int kRopeThreads = 256, kRopeWarps = kRopeThreads / 32;
+constexpr uint32_t kRopeTokens = 8;           // most tokens of a CTA at a time
+constexpr uint32_t kRopeBackPerSm = 2;
+
+struct RopeShape {
+  uint32_t tokens;        // of a CTA at a time
+  uint32_t lanes;         // threads to a row, a power of two
+  uint32_t units;         // V-pair units of a row
+  uint32_t rot_units;     // of these turned
+};
+
+// First elements of the two V-wide accesses of unit u.
+template <int V>
+__device__ __forceinline__ void unit_at(const RopeArgs &a, const RopeShape &s, uint32_t u, uint32_t &e0, uint32_t &e1) {
+  if (u < s.rot_units) {
+    if (a.interleaved) { e0 = 2u * V * u; e1 = e0 + V; }
+    else { e0 = V * u; e1 = e0 + a.rot / 2u; }
+  } else {
+    e0 = a.rot + V * (u - s.rot_units);
+    e1 = e0 + (a.hd - a.rot) / 2u;
+  }
+}
+// Pair i of a unit in its 2 V values: half layout (i, V + i), neighbours (2 i, 2 i + 1).
+template <int V>
+__device__ __forceinline__ void turn(float (&y)[2 * V], const float2 (&cs)[V], bool inter, float sign) {
+  if (inter) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float p = y[2 * i], q = y[2 * i + 1], sn = sign * cs[i].y;
+      y[2 * i] = p * cs[i].x - q * sn;
+      y[2 * i + 1] = p * sn + q * cs[i].x;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float p = y[i], q = y[V + i], sn = sign * cs[i].y;
+      y[i] = p * cs[i].x - q * sn;
+      y[V + i] = p * sn + q * cs[i].x;
+    }
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void load_unit(const RowsRef &r, uint32_t tok, uint32_t head, uint32_t e0, uint32_t e1, float (&x)[2 * V]) {
+  const T *p = reinterpret_cast<const T *>(r.p) + static_cast<int64_t>(tok) * r.row + static_cast<int64_t>(head) * r.head;
+  const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(p + e0), b = *reinterpret_cast<const Vec<T, V> *>(p + e1);
+#pragma unroll
+  for (int i = 0; i < V; ++i) { x[i] = ToF(a.v[i]); x[V + i] = ToF(b.v[i]); }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_unit(const RowsRef &r, uint32_t tok, uint32_t head, uint32_t e0, uint32_t e1, const float (&x)[2 * V]) {
+  T *p = reinterpret_cast<T *>(r.p) + static_cast<int64_t>(tok) * r.row + static_cast<int64_t>(head) * r.head;
+  Vec<T, V> a, b;
+#pragma unroll
+  for (int i = 0; i < V; ++i) { a.v[i] = FromF<T>(x[i]); b.v[i] = FromF<T>(x[V + i]); }
+  *reinterpret_cast<Vec<T, V> *>(p + e0) = a;
+  *reinterpret_cast<Vec<T, V> *>(p + e1) = b;
+}
+__device__ __forceinline__ float row_sum(float v, uint32_t lanes) {
+  for (uint32_t o = lanes >> 1; o > 0u; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// U: units of a row that a thread may have (rows of more than 32 units).
+template <typename T, int V, int U, bool BACK>
+__global__ void __launch_bounds__(kRopeThreads) b2_rope(const __grid_constant__ RopeArgs a, const __grid_constant__ RopeShape s) {
+  extern __shared__ __align__(16) uint8_t sm[];
+  float *w_s = reinterpret_cast<float *>(sm);                                 // [2][hd]
+  float2 *cs_s = reinterpret_cast<float2 *>(w_s + 2u * a.hd);                 // [tokens][rot / 2]
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, half = a.rot / 2u;
+  const uint32_t rows_per_warp = 32u / s.lanes, slot = lane / s.lanes, sub = lane & (s.lanes - 1u);
+  if (a.norm) {
+    for (uint32_t i = tid; i < 2u * a.hd; i += kRopeThreads) {
+      const uint32_t t = i >= a.hd ? 1u : 0u, e = i - t * a.hd;
+      const void *w = a.w[t];
+      w_s[i] = !w ? 1.0f : a.weight_f32 ? static_cast<const float *>(w)[e] : ToF(static_cast<const T *>(w)[e]);
+    }
+  }
+  uint32_t e0[U], e1[U];
+  bool has[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const uint32_t u = sub + static_cast<uint32_t>(k) * s.lanes;
+    has[k] = u < s.units;
+    unit_at<V>(a, s, has[k] ? u : 0u, e0[k], e1[k]);
+  }
+  float acc[2][U][2 * V];
+  if (BACK) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) acc[t][k][i] = 0.0f;
+  }
+  const uint32_t groups[2] = {(a.heads[0] + rows_per_warp - 1u) / rows_per_warp, (a.heads[1] + rows_per_warp - 1u) / rows_per_warp};
+  const uint32_t per_token = groups[0] + groups[1];
+  const float inv_hd = 1.0f / static_cast<float>(a.hd);
+  const bool inter = a.interleaved != 0u;
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * s.tokens; base < a.n_rows; base += static_cast<uint64_t>(gridDim.x) * s.tokens) {
+    const uint32_t tok0 = static_cast<uint32_t>(base), n_tok = min(s.tokens, a.n_rows - tok0);
+    __syncthreads();                                      // the angles before have been used
+    for (uint32_t i = tid; i < n_tok * half; i += kRopeThreads) {
+      const uint32_t tk = i / half, f = i - tk * half;
+      double t = static_cast<double>(a.pos[tok0 + tk]) * a.turns[f];
+      t -= rint(t);
+      float sn, cn;
+      sincospif(2.0f * static_cast<float>(t), &sn, &cn);
+      cs_s[i] = make_float2(cn * a.magnitude, sn * a.magnitude);
+    }
+    __syncthreads();
+    for (uint32_t task = warp; task < n_tok * per_token; task += kRopeWarps) {
+      const uint32_t tk = task / per_token, g = task - tk * per_token, t = g >= groups[0] ? 1u : 0u;
+      const uint32_t head = (g - (t ? groups[0] : 0u)) * rows_per_warp + slot, tok = tok0 + tk;
+      const bool live = head < a.heads[t];
+      float x[U][2 * V], y[U][2 * V];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (live && has[k]) {
+          if (!BACK || a.norm) load_unit<T, V>(a.x[t], tok, head, e0[k], e1[k], x[k]);
+          if (BACK) load_unit<T, V>(a.g[t], tok, head, e0[k], e1[k], y[k]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) { x[k][i] = 0.0f; y[k][i] = 0.0f; }
+        }
+      }
+      float r = 1.0f;
+      if (a.norm) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) ss += x[k][i] * x[k][i];
+        const float sum = row_sum(ss, s.lanes);
+        r = live ? 1.0f / sqrtf(sum * inv_hd + a.eps) : 0.0f;      // (no row: adds nothing to the weights' gradients)
+      }
+      if (!BACK) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (a.norm) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) { x[k][i] *= r * w_s[t * a.hd + e0[k] + i]; x[k][V + i] *= r * w_s[t * a.hd + e1[k] + i]; }
+          }
+          const uint32_t u = sub + static_cast<uint32_t>(k) * s.lanes;
+          if (u < s.rot_units) {
+            float2 cs[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) cs[i] = cs_s[tk * half + V * u + i];
+            turn<V>(x[k], cs, inter, 1.0f);
+          }
+          if (live && has[k]) store_unit<T, V>(a.y[t], tok, head, e0[k], e1[k], x[k]);
+        }
+      } else {
+        float hx = 0.0f;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const uint32_t u = sub + static_cast<uint32_t>(k) * s.lanes;
+          if (u < s.rot_units) {
+            float2 cs[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) cs[i] = cs_s[tk * half + V * u + i];
+            turn<V>(y[k], cs, inter, -1.0f);
+          }
+          if (a.norm) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float g0 = y[k][i] * x[k][i] * r, g1 = y[k][V + i] * x[k][V + i] * r;
+              if (t) { acc[1][k][i] += g0; acc[1][k][V + i] += g1; }
+              else { acc[0][k][i] += g0; acc[0][k][V + i] += g1; }
+              y[k][i] *= w_s[t * a.hd + e0[k] + i];
+              y[k][V + i] *= w_s[t * a.hd + e1[k] + i];
+              hx += y[k][i] * x[k][i] + y[k][V + i] * x[k][V + i];
+            }
+          }
+        }
+        if (a.norm) {
+          const float c = row_sum(hx, s.lanes) * inv_hd * r * r * r;
+#pragma unroll
+          for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) y[k][i] = r * y[k][i] - c * x[k][i];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+          if (live && has[k]) store_unit<T, V>(a.y[t], tok, head, e0[k], e1[k], y[k]);
+      }
+    }
+  }
+  if (!BACK || !a.partial) return;
+  // ---- gradients of the weights: lanes of the same unit, then warps, then CTAs ----
+  __syncthreads();
+  float *red = reinterpret_cast<float *>(sm);             // [warps][2][hd]
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i) {
+        float v = acc[t][k][i];
+        for (uint32_t o = s.lanes; o < 32u; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (slot == 0u && has[k]) red[(warp * 2u + t) * a.hd + (i < V ? e0[k] + i : e1[k] + i - V)] = v;
+      }
+  __syncthreads();
+  const uint32_t cols = 2u * a.hd;
+  for (uint32_t i = tid; i < cols; i += kRopeThreads) {
+    float v = 0.0f;
+#pragma unroll
+    for (int wp = 0; wp < kRopeWarps; ++wp) v += red[wp * cols + i];
+    a.partial[static_cast<size_t>(blockIdx.x) * cols + i] = v;
+  }
+}
+
+// The CTAs' sums in their order: 32 columns to a CTA, its warps an eighth of them each.
+__global__ void __launch_bounds__(kRopeThreads) b2_rope_weights(const __grid_constant__ RopeArgs a, uint32_t ctas) {
+  __shared__ float red[kRopeWarps][32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, cols = 2u * a.hd, c = blockIdx.x * 32u + lane;
+  const uint32_t per = (ctas + kRopeWarps - 1u) / kRopeWarps, b1 = min(ctas, (warp + 1u) * per);
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < cols) {
+    const float *p = a.partial + c;
+    uint32_t b = warp * per;
+    for (; b + 8u <= b1; b += 8u) {
+      float q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = p[static_cast<size_t>(b + i) * cols];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i & 3] += q[i];
+    }
+    for (; b < b1; ++b) v[0] += p[static_cast<size_t>(b) * cols];
+  }
+  red[warp][lane] = (v[0] + v[1]) + (v[2] + v[3]);
+  __syncthreads();
+  if (warp == 0u && c < cols) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kRopeWarps; ++k) sum += red[k][lane];
+    const uint32_t t = c >= a.hd ? 1u : 0u;
+    if (a.dw[t]) a.dw[t][c - t * a.hd] = sum;
+  }
+}
+
+uint32_t Pow2AtLeast(uint32_t v) {
+  uint32_t p = 1;
+  while (p < v) p *= 2;
+  return p;
+}
+
+template <typename T, int V, int U, bool BACK>
+int Launch(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
+  RopeShape s;
+  s.units = a.hd / 2u / V;
+  s.rot_units = a.rot / 2u / V;
+  s.lanes = Pow2AtLeast(s.units) < 32u ? Pow2AtLeast(s.units) : 32u;
+  // Few tokens: one to a CTA, so that all SMs have some (32 rows of a decode step: 32 CTAs). Many: as many as leave four rounds for
+  // each of the CTAs that fit, up to 8, so that the angles and the barriers around them are shared by more rows.
+  const uint32_t rounds = a.n_rows / (sms * 16u);
+  s.tokens = rounds < 1u ? 1u : rounds > kRopeTokens ? kRopeTokens : rounds;
+  uint32_t ctas = (a.n_rows + s.tokens - 1u) / s.tokens;
+  const uint32_t most = BACK ? kRopeBackPerSm * sms : sms * 8u;
+  ctas = ctas < 1u ? 1u : ctas > most ? most : ctas;
+  size_t smem = sizeof(float) * 2u * a.hd + sizeof(float2) * s.tokens * (a.rot / 2u);
+  const size_t red = sizeof(float) * 2u * a.hd * kRopeWarps;
+  if (BACK && red > smem) smem = red;
+  b2_rope<T, V, U, BACK><<<ctas, kRopeThreads, smem, stream>>>(a, s);
+  if (BACK && a.partial) b2_rope_weights<<<(2u * a.hd + 31u) / 32u, kRopeThreads, 0, stream>>>(a, ctas);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// The widest access that every address of the call allows.
+template <typename T>
+uint32_t Width(const RopeArgs &a, bool backward) {
+  uint32_t v = 16u / sizeof(T);
+  const uint32_t half = a.rot / 2u, rest = (a.hd - a.rot) / 2u;
+  while (v > 1u && (half % v || rest % v)) v /= 2u;
+  auto fit = [&](const RowsRef &r, uint32_t heads) {
+    if (!heads || !r.p) return;
+    while (v > 1u && (reinterpret_cast<uintptr_t>(r.p) % (v * sizeof(T)) || r.row % static_cast<int64_t>(v) || (heads > 1u && r.head % static_cast<int64_t>(v)))) v /= 2u;
+  };
+  for (int t = 0; t < 2; ++t) {
+    if (!backward || a.norm) fit(a.x[t], a.heads[t]);
+    fit(a.y[t], a.heads[t]);
+    if (backward) fit(a.g[t], a.heads[t]);
+  }
+  return v;
+}
+
+template <typename T, bool BACK>
+int Dispatch(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
+  const uint32_t v = Width<T>(a, BACK);
+  if constexpr (sizeof(T) == 2) {
+    if (v == 8u) return Launch<T, 8, 1, BACK>(a, sms, stream);
+  }
+  if (v >= 4u) return Launch<T, 4, 1, BACK>(a, sms, stream);
+  return Launch<T, 1, 4, BACK>(a, sms, stream);
+}
+
+}  // namespace
+
+uint32_t RopeBackwardCtas(uint32_t sms) { return kRopeBackPerSm * sms; }
+
+int LaunchRope(const RopeArgs &a, uint32_t dtype, bool backward, uint32_t sms, CUstream_st *stream) {
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (backward) {
+    if (dtype == B2_F32) return Dispatch<float, true>(a, sms, s);
+    return dtype == B2_BF16 ? Dispatch<__nv_bfloat16, true>(a, sms, s) : Dispatch<__half, true>(a, sms, s);
+  }
+  if (dtype == B2_F32) return Dispatch<float, false>(a, sms, s);
+  return dtype == B2_BF16 ? Dispatch<__nv_bfloat16, false>(a, sms, s) : Dispatch<__half, false>(a, sms, s);
+}
+
+}  // namespace b2

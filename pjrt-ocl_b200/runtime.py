@@ -98,7 +98,9 @@ EXPORTS = [
     "b2_loaded_status", "b2_loaded_launch_count", "b2_loaded_set_wait_budget_ns",
     "b2_loaded_phase_ns", "b2_loaded_stat", "b2_sum_f32_static", "b2_sum_f32_static_max_elems",
     "b2_loaded_lane_timing", "b2_loaded_lane_times", "b2_loaded_in_out_result",
-    "b2_loaded_preset_arrivals",
+    "b2_loaded_preset_arrivals", "b2_scratch_create", "b2_scratch_destroy", "b2_rope_frequencies", "b2_rope_create",
+    "b2_rope_destroy", "b2_rope_apply", "b2_rope_apply_backward", "b2_cache_create", "b2_cache_destroy", "b2_cache_write",
+    "b2_cache_read", "b2_cache_attend", "b2_cache_status",
 ]
 
 
@@ -114,6 +116,7 @@ def lib():
     L = ctypes.CDLL(path)
     vp, cp, sz = ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t
     pvp = ctypes.POINTER(ctypes.c_void_p)
+    u32, f64 = ctypes.c_uint32, ctypes.c_double
     sig = {
         "b2_runtime_create": (ctypes.c_int, [ctypes.c_int, pvp, cp, sz]),
         "b2_runtime_destroy": (None, [vp]),
@@ -150,6 +153,19 @@ def lib():
         "b2_loaded_preset_arrivals": (ctypes.c_int, [vp, ctypes.c_uint32, cp, sz]),
         "b2_sum_f32_static": (ctypes.c_int, [ctypes.c_int, vp, ctypes.c_uint64, vp, vp, cp, sz]),
         "b2_sum_f32_static_max_elems": (ctypes.c_uint64, []),
+        "b2_scratch_create": (ctypes.c_int, [vp, pvp, cp, sz]),
+        "b2_scratch_destroy": (None, [vp]),
+        "b2_rope_frequencies": (ctypes.c_int, [u32, f64, ctypes.c_int, f64, f64, f64, f64, vp, sz, cp, sz]),
+        "b2_rope_create": (ctypes.c_int, [vp, vp, pvp, cp, sz]),
+        "b2_rope_destroy": (None, [vp]),
+        "b2_rope_apply": (ctypes.c_int, [vp, u32] + [vp] * 8 + [cp, sz]),
+        "b2_rope_apply_backward": (ctypes.c_int, [vp, vp, u32] + [vp] * 12 + [cp, sz]),
+        "b2_cache_create": (ctypes.c_int, [vp, vp, pvp, cp, sz]),
+        "b2_cache_destroy": (None, [vp]),
+        "b2_cache_write": (ctypes.c_int, [vp] * 5 + [cp, sz]),
+        "b2_cache_read": (ctypes.c_int, [vp] * 5 + [cp, sz]),
+        "b2_cache_attend": (ctypes.c_int, [vp] * 4 + [ctypes.c_float, ctypes.c_int, u32] + [vp] * 3 + [cp, sz]),
+        "b2_cache_status": (ctypes.c_int, [vp, ctypes.POINTER(_ExecStatus), cp, sz]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
