@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t seq_of_row(const int32_t *row_start, uint32_
     const uint32_t k = m ? 31u - __clz(m) : 0u;           // the last of the 32 that starts at or before i
     const uint32_t end = lo + n;
     lo += k * step;
-    n = min(step, end - lo);
+    n = min(lo + step, end) - lo;
   }
   return lo;
 }

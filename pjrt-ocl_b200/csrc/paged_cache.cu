@@ -70,10 +70,10 @@ __global__ void __launch_bounds__(kMoveThreads) b2_cache_move(const __grid_const
     }
   }
   for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * s.tokens; base < b.n_rows; base += static_cast<uint64_t>(gridDim.x) * s.tokens) {
-    const uint32_t n_tok = min(s.tokens, b.n_rows - static_cast<uint32_t>(base));
+    const uint32_t tok0 = static_cast<uint32_t>(base), n_tok = min(tok0 + s.tokens, b.n_rows) - tok0;
     __syncthreads();                                      // the places before have been used
     for (uint32_t t = warp; t < n_tok; t += kMoveWarps) {
-      const int32_t i = static_cast<int32_t>(base) + static_cast<int32_t>(t);
+      const int32_t i = static_cast<int32_t>(tok0 + t);
       const uint32_t q = seq_of_row(b.row_start, b.n_seqs, i);
       if (lane == 0u) {
         const Seq sq = load_seq(b, cap, q);

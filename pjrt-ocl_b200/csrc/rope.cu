@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(kRopeThreads) b2_rope(const __grid_constant__ 
   const float inv_hd = 1.0f / static_cast<float>(a.hd);
   const bool inter = a.interleaved != 0u;
   for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * s.tokens; base < a.n_rows; base += static_cast<uint64_t>(gridDim.x) * s.tokens) {
-    const uint32_t tok0 = static_cast<uint32_t>(base), n_tok = min(s.tokens, a.n_rows - tok0);
+    // (min(s.tokens, a.n_rows - tok0) came out as s.tokens for the last, shorter run: the compiler of CUDA 12.9 with this loop around it)
+    const uint32_t tok0 = static_cast<uint32_t>(base), n_tok = min(tok0 + s.tokens, a.n_rows) - tok0;
     __syncthreads();                                      // the angles before have been used
     for (uint32_t i = tid; i < n_tok * half; i += kRopeThreads) {
       const uint32_t tk = i / half, f = i - tk * half;

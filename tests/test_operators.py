@@ -60,6 +60,8 @@ ROPE = [  # rows, q heads, k heads, dim, rot, dtype, interleaved, norm, layout, 
     (300, 7, 7, 64, 0, "bf16", False, True, "fused", "rows", "plain"),
     (2500, 4, 2, 128, 96, "bf16", True, True, "fused", "f32", "plain"),
     (9, 2, 2, 200, 8, "f16", False, True, "heads_first", "f32", "plain"),
+    (5001, 2, 1, 128, 128, "bf16", False, True, "fused", "f32", "plain"),        # (more than one token to a CTA, the last run shorter)
+    (16384 + 5, 1, 1, 64, 32, "f16", True, True, "fused", "f32", "plain"),
 ]
 
 
@@ -196,6 +198,8 @@ CACHE = [  # rows, past, dtype, row dtype, heads, dim, page, head major, pad
     ([1] * 40 + [0] * 3 + [2] * 40, [3] * 83, "e4m3", "bf16", 1, 48, 5, False, 3),
     ([2600, 1300], [5, 0], "e4m3", "bf16", 4, 128, 128, False, 9),
     ([3000], [70], "bf16", "f32", 8, 64, 32, False, 0),
+    ([5000, 3, 2308], [1, 0, 9], "e4m3", "bf16", 1, 64, 64, False, 2),
+    ([9001, 6000, 1, 4000], [0, 3, 50, 1], "f16", "f16", 2, 32, 16, False, 1),
 ]
 
 
