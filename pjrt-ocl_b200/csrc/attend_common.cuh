@@ -77,5 +77,43 @@ static __device__ __noinline__ void attend_row_alone(const AttendArgs &a, uint32
   if (lane == 0u && a.lse) a.lse[static_cast<int64_t>(s.first + i) * a.q_heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
+// The sequence b whose units hold unit `target` of all sequences' units in a row, and the number of those before b's; false where
+// there are not that many. of(b): the units of sequence b. All threads of the CTA; `sh` has room for THREADS / 32 + 2 words.
+template <uint32_t THREADS, typename F>
+__device__ __forceinline__ bool find_unit(uint32_t n_seqs, unsigned long long target, unsigned long long *sh, F of, uint32_t &seq, unsigned long long &before) {
+  constexpr uint32_t W = THREADS / 32u;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, w = tid >> 5;
+  unsigned long long run = 0;
+  bool found = false;
+  for (uint32_t i0 = 0; i0 < n_seqs && !found; i0 += THREADS) {
+    const uint32_t i = i0 + tid;
+    const unsigned long long v = i < n_seqs ? of(i) : 0ull;
+    unsigned long long x = v;
+#pragma unroll
+    for (uint32_t o = 1; o < 32u; o <<= 1) {
+      const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31u) sh[w] = x;
+    __syncthreads();
+    unsigned long long mine = run;
+    for (uint32_t k = 0; k < W; ++k) {
+      if (k < w) mine += sh[k];
+      run += sh[k];
+    }
+    if (v != 0ull && mine + x > target && mine + x - v <= target) {
+      sh[W] = i;
+      sh[W + 1u] = mine + x - v;
+    }
+    found = run > target;                                 // (the same for all threads)
+  }
+  __syncthreads();
+  if (!found) return false;
+  seq = static_cast<uint32_t>(sh[W]);
+  before = sh[W + 1u];
+  return true;
+}
+
 }  // namespace b2
 #endif

@@ -298,6 +298,12 @@ ATTEND = [  # rows, past, dtype, row dtype, heads, q heads, dim, page, causal, w
     ([1000], [3000], "bf16", "bf16", 1, 8, 128, 128, True, 0, False, 0),
     ([64] * 9, [0, 1, 63, 64, 65, 127, 128, 129, 1000], "f16", "f16", 1, 2, 96, 32, True, 0, False, 0),
     ([300], [2000], "e4m3", "bf16", 4, 4, 32, 16, True, 0, False, 0),
+    # more tiles of rows than SMs: keys are not split
+    ([600, 1, 90], [300, 777, 0], "bf16", "bf16", 16, 64, 128, 64, True, 0, False, 3),
+    ([70] * 40, list(range(0, 800, 20)), "e4m3", "bf16", 4, 16, 128, 48, True, 0, True, 0),
+    ([20] * 150, [37] * 150, "f16", "f16", 1, 2, 64, 16, True, 30, False, 0),
+    ([513] * 3, [0, 100, 1000], "e4m3", "f16", 20, 20, 64, 32, True, 0, False, 0),
+    ([40] * 30, [200] * 30, "bf16", "bf16", 5, 5, 80, 64, False, 0, False, 0),
 ]
 
 
