@@ -23,7 +23,9 @@ namespace b2 {
 namespace {
 
 constexpr uint32_t kCkRows = 128, kCkKeys = 128;          // rows of a slot, keys of a block
-constexpr uint32_t kSoftWarps = 8, kLoadWarps = 4, kCkThreads = (kSoftWarps + kLoadWarps + 1) * 32;
+constexpr uint32_t kSoftWarps = 8, kLoadWarps = 4, kCkThreads = (kSoftWarps + kLoadWarps + 4) * 32;     // (three of the last four warps only hold registers back)
+// Registers of a thread: launched with 128 each, the softmax warps take those that the others give up (2 x 184 + 88 + 56 = 4 x 128).
+constexpr int kSoftRegs = 184, kLoadRegs = 88, kIssueRegs = 56;
 constexpr uint32_t kCkCols = 512;                         // tensor memory: S0, S1 (128 columns each), O0, O1
 constexpr float kGrow = 8.0f;                             // log2 of the growth of a row maximum that forces a rescale
 constexpr float kCkPScale = 64.0f;                        // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
@@ -371,43 +373,39 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, const Til
     const int32_t j0 = t.keys.lo + static_cast<int32_t>(j * kCkKeys);
     const int32_t lo = sp.lo - j0, hi = sp.hi - j0;       // columns [lo, hi) are seen
     const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= static_cast<int32_t>(kCkKeys));
-    // 1: the maximum
+    // 1: the row's scores into registers, and their maximum
+    uint32_t x[4][32];
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tc_ld32(s_addr + 32u * c, x[c]);
+    tc_wait_ld();
     float mx = -INFINITY, v_top = 0.0f;
-#pragma unroll 1
-    for (uint32_t c0 = 0; c0 < kCkKeys; c0 += 32u) {
-      uint32_t x[32];
-      __syncwarp();
-      tc_ld32(s_addr + c0, x);
-      tc_wait_ld();
-      if (Q8) {
+    if (Q8) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 k4 = *reinterpret_cast<const float4 *>(ks + c0 + i), v4 = *reinterpret_cast<const float4 *>(vs + c0 + i);
-          const float kk[4] = {k4.x, k4.y, k4.z, k4.w}, vv[4] = {v4.x, v4.y, v4.z, v4.w};
+      for (int i = 0; i < 128; i += 4) {
+        const float4 k4 = *reinterpret_cast<const float4 *>(ks + i), v4 = *reinterpret_cast<const float4 *>(vs + i);
+        const float kk[4] = {k4.x, k4.y, k4.z, k4.w}, vv[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int32_t c = static_cast<int32_t>(c0) + i + e;
-            const bool seen = whole || (c >= lo && c < hi);
-            mx = fmaxf(mx, seen ? __uint_as_float(x[i + e]) * kk[e] : -INFINITY);
-            v_top = fmaxf(v_top, seen ? vv[e] : 0.0f);
-          }
+        for (int e = 0; e < 4; ++e) {
+          x[i >> 5][(i & 31) + e] = __float_as_uint(__uint_as_float(x[i >> 5][(i & 31) + e]) * kk[e]);
+          const bool seen = whole || (i + e >= lo && i + e < hi);
+          v_top = fmaxf(v_top, seen ? vv[e] : 0.0f);
         }
-      } else {
-        if (!whole) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int32_t c = static_cast<int32_t>(c0) + i;
-            if (c < lo || c >= hi) x[i] = 0xff800000u;
-          }
-        }
-        float m4[4] = {mx, mx, mx, mx};
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) m4[e] = max3(m4[e], __uint_as_float(x[i + e]), __uint_as_float(x[i + e + 4]));
-        }
-        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 128; ++i)
+        if (i < lo || i >= hi) x[i >> 5][i & 31] = 0xff800000u;
+    }
+    {
+      float m4[4] = {mx, mx, mx, mx};
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        m4[i & 1] = max3(m4[i & 1], __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
+        m4[2 + (i & 1)] = max3(m4[2 + (i & 1)], __uint_as_float(x[2][i]), __uint_as_float(x[3][i]));
+      }
+      mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
     }
     mx *= sl2;
     bool grow = mx > m_used + kGrow;
@@ -428,14 +426,14 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, const Til
     }
     if (j > b0 && __any_sync(0xffffffffu, grow)) {        // (these scores came after the products before them: O is at rest)
 #pragma unroll 1
-      for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
-        uint32_t x[32];
+      for (uint32_t c0 = 0; c0 < HD; c0 += 16u) {
+        uint32_t y[16];
         __syncwarp();
-        tc_ld32(o_addr + c0, x);
+        tc_ld16(o_addr + c0, y);
         tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
-        tc_st32(o_addr + c0, x);
+        for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+        tc_st16(o_addr + c0, y);
       }
       tc_wait_st();
     }
@@ -443,39 +441,25 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, const Til
     const float neg = m_used == -INFINITY ? 0.0f : -m_used;
     const unsigned long long sl2_2 = pack_f32x2(sl2, sl2), neg_2 = pack_f32x2(neg, neg);
     unsigned long long sum[2] = {0ull, 0ull};
-#pragma unroll 1
-    for (uint32_t c0 = 0; c0 < kCkKeys; c0 += 32u) {
-      uint32_t x[32], pk[16];
-      __syncwarp();
-      tc_ld32(s_addr + c0, x);
-      tc_wait_ld();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float x0 = __uint_as_float(x[2 * i]), x1 = __uint_as_float(x[2 * i + 1]);
-        float v0 = 1.0f, v1 = 1.0f;
-        if (Q8) {
-          const float2 k2 = *reinterpret_cast<const float2 *>(ks + c0 + 2 * i), v2 = *reinterpret_cast<const float2 *>(vs + c0 + 2 * i);
-          x0 *= k2.x; x1 *= k2.y;
-          v0 = v2.x * v_mul; v1 = v2.y * v_mul;
-        }
-        if (!whole) {
-          const int32_t c = static_cast<int32_t>(c0) + 2 * i;
-          if (c < lo || c >= hi) x0 = -INFINITY;
-          if (c + 1 < lo || c + 1 >= hi) x1 = -INFINITY;
-        }
         float e0, e1;
-        unpack_f32x2(fma_f32x2(pack_f32x2(x0, x1), sl2_2, neg_2), e0, e1);
+        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), sl2_2, neg_2), e0, e1);
         e0 = fast_ex2(e0);
         e1 = fast_ex2(e1);
         sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
         if (Q8) {
-          e0 = e0 == 0.0f ? 0.0f : e0 * v0;
-          e1 = e1 == 0.0f ? 0.0f : e1 * v1;
+          const float2 v2 = *reinterpret_cast<const float2 *>(vs + 32 * c + 2 * i);
+          e0 = e0 == 0.0f ? 0.0f : e0 * (v2.x * v_mul);
+          e1 = e1 == 0.0f ? 0.0f : e1 * (v2.y * v_mul);
         }
         pk[i] = BF && !Q8 ? cvt_bf16x2(e1, e0) : cvt_f16x2(e1, e0);
       }
       __syncwarp();
-      tc_st16(s_addr + c0 / 2u, pk);
+      tc_st16(s_addr + 16u * c, pk);
     }
     tc_wait_st();
     tc_fence_before_sync();
@@ -599,9 +583,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) b2_attend_chunk(const __grid_co
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (w < kSoftWarps) chunk_rows<BF, Q8, HD>(a, t, wk, b0, b1, sm, S);
-  else if (w < kSoftWarps + kLoadWarps) chunk_load<BF, Q8, HD>(a, t, wk.head, b0, b1, sm, S);
-  else chunk_products<Q8 || !BF, HD>(b1 - b0, t.rows > kCkRows ? 2u : 1u, sm, S);
+  if (w < kSoftWarps) {
+    more_registers<kSoftRegs>();
+    chunk_rows<BF, Q8, HD>(a, t, wk, b0, b1, sm, S);
+  } else if (w < kSoftWarps + kLoadWarps) {
+    fewer_registers<kLoadRegs>();
+    chunk_load<BF, Q8, HD>(a, t, wk.head, b0, b1, sm, S);
+  } else {
+    fewer_registers<kIssueRegs>();
+    if (w == kSoftWarps + kLoadWarps) chunk_products<Q8 || !BF, HD>(b1 - b0, t.rows > kCkRows ? 2u : 1u, sm, S);
+  }
   __syncwarp();
   tc_fence_before_sync();
   __syncthreads();

@@ -6,6 +6,10 @@
 
 namespace b2 {
 
+// A warpgroup's registers, by the thread: all four warps of it execute these.
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // Two e4m3 values as two f16 (exact).
 __device__ __forceinline__ uint32_t cvt_e4m3x2_f16x2(uint32_t lo16) {
   uint32_t r;
