@@ -416,7 +416,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, const Til
       m_used = mx;
     }
     if (Q8) {
-      const float ref = __uint_as_float(min(250u, max(4u, (__float_as_uint(v_top) >> 23) + 1u)) << 23);
+      const float ref = power_above(v_top);
       if (ref > v_ref) {
         alpha *= v_ref / ref;
         v_ref = ref;

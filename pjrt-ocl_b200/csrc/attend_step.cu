@@ -1,19 +1,22 @@
 // Attention of a few rows of each sequence over the paged cache: decode steps. rows x (query heads to a cache head) <= 16.
 //
-// One pass over the keys with the running maximum m and sum l of the softmax (base 2): for a tile of keys s = q k^T scale log2 e,
-// m' = max(m, s), p = 2^(s - m'), l = l 2^(m - m') + sum p, o = o 2^(m - m') + p v; the result is o / l.
+// One pass over the keys with a running maximum m and sum l of the softmax (base 2): for a tile of keys s = k q^T scale log2 e,
+// p = 2^(s - m), l += sum p, o += v^T p; where a row's scores outgrow m by more than 2^8, m moves and l and o are scaled by
+// 2^(m_old - m). The result is o / l.
 //
-// Bound: HBM, K and V of every visible key read once. The query heads that share a cache head are the rows of one 16-row
-// product (m16n8k16 warp-level products: at most 16 multiplications to a byte, far from any tensor rate, and their results come in
-// registers, where the softmax wants them).
-// Work: a cache head of a sequence is an item, cut into tiles of 16 or 32 keys. All tiles of the batch in a row are dealt to the CTAs in
-// equal runs (one CTA to an SM), whatever the lengths; a CTA's eight warps take its tiles in turn, each with a ring of three
-// stages of its own (K and V of a tile, 8 KB, by 16-byte asynchronous copies, page by page), so that a warp always has two tiles on
-// the way and no barrier stands between tiles. At an item's end the warps' (m, l, o) are joined through the stage each has free; an
-// item that is split between CTAs leaves partial results, and the CTA that comes last joins them in the CTAs' order.
+// Bound: HBM, K and V of every visible key read once.
+// Work: a cache head of a sequence is an item, cut into tiles of 16 or 32 keys. The tiles of the whole batch in a row, with some for
+// what an item costs beside its tiles, are dealt to the CTAs in equal runs (one CTA to an SM), whatever the lengths. A CTA's warps take
+// its tiles in turn, each through two stages of its own (K and V of a tile, 8 KB, by 16-byte asynchronous copies, page by page): no barrier
+// stands between tiles. At an item's end the warps' (m, l, o) are joined through the stage each has free; an item that is split between
+// CTAs leaves partial results, and the CTA that comes last joins them in the CTAs' order.
+// Products: warp-level, 16 x 8 x 16, with the keys (then the values' head_dim) as the 16 rows and the rows of q that share a cache head as the 8
+// columns, so that a decode step of up to 8 heads to a cache head wastes nothing (as the 16 rows they would be half padding at best: twice the
+// products, scores and registers; 32 x 8 bits x 128: 1240 instructions a tile, 283 us for 64 sequences of 200 to 16000 tokens). Scores become the
+// second product's operand by a transposition of 8 x 8 fragments.
 // 8-bit pages: codes are exact in f16, so the products are f16 x f16 whatever the rows' type. q of type bf16 is scaled by a power of
 // two for each row so that its largest value is near 2^14 (f16 then holds what bf16 held to 2^-38 of that); a key's scale goes onto its
-// scores, a value's onto p, relative to a power of two not below any scale so far (p v's factor stays in f16's normal range).
+// scores, a value's onto p, relative to a power of two not below any scale that the row has seen (p v's factor stays in f16's normal range).
 // bf16 pages: p is split into two bf16 values (p and what rounding left), since the second product costs nothing here; the result is
 // then only rounded once, as it is stored.
 #include "attend_common.cuh"
@@ -21,8 +24,10 @@
 namespace b2 {
 namespace {
 
-constexpr uint32_t kStepWarps = 8, kStepThreads = kStepWarps * 32, kStages = 3;
-constexpr float kPScale = 16384.0f;      // 8-bit pages: p = 1 on the largest scale, in f16
+constexpr uint32_t kStepWarps = 12, kStepThreads = kStepWarps * 32, kStages = 2;
+constexpr float kPScale = 64.0f;         // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
+constexpr float kGrow = 8.0f;            // log2 of the growth of a row maximum that moves it
+constexpr uint32_t kItemTiles = 8;       // what an item costs beside its tiles, in tiles
 
 template <bool Q8, int HD>
 struct StepShape {
@@ -31,22 +36,32 @@ struct StepShape {
   static constexpr int kBytes = KT * CH * 16;                 // K (or V) of a tile
   static constexpr int kScales = Q8 ? 2 * KT * 4 : 0;
   static constexpr int kStage = 2 * kBytes + kScales;
-  static constexpr int kSmem = static_cast<int>(kStepWarps * kStages) * kStage;
-  static_assert(2 * kBytes >= 16 * HD * 4, "a stage holds a warp's result");
+  static constexpr int kRing = static_cast<int>(kStepWarps * kStages) * kStage;
+  static constexpr int kQ = 16 * HD * 2;                      // q of an item
+  static constexpr int kSmem = kRing + 2 * kQ;
 };
 // Chunk of a row in shared memory: eight rows of the same chunk lie in different banks.
 template <int CH>
 __device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t c) {
   return (row * CH + (CH >= 8 ? (c ^ (row & 7u)) : (c ^ ((row >> 1) & 3u)))) * 16u;
 }
+// The transposed 8 x 8 fragment of 16-bit values.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float lds_f32(uint32_t at) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
 
 struct StepShared {
   float m[kStepWarps][16], l[kStepWarps][16];
-  unsigned long long sum[kStepWarps], scan[kStepWarps];
-  unsigned long long total;
-  uint32_t found_seq;
-  unsigned long long found_base;
-  uint32_t last, redo[2];           // by turns: an item's rows to be worked out again
+  unsigned long long sum[2][kStepWarps], find[kStepWarps + 2];
+  uint32_t at[kStepWarps];         // the stage each warp left its result in
+  uint32_t last, redo[2];          // redo by turns: an item's rows to be worked out again
 };
 
 // An item: cache head h of sequence b, `nt` tiles of keys from `lo`.
@@ -61,95 +76,99 @@ struct Walk {
     keys = s.n > 0 ? SeenByRows(s, 0, s.n, a.causal, a.window) : Span{0, 0};
     nt = s.n > 0 ? max(1u, (static_cast<uint32_t>(keys.hi - keys.lo) + KT - 1u) / KT) : 0u;
   }
-  __device__ __forceinline__ void next(const AttendArgs &a, uint64_t cap) {
-    if (++h < a.c.heads) return;
+  // false behind the last item
+  __device__ __forceinline__ bool next(const AttendArgs &a, uint64_t cap) {
+    if (++h < a.c.heads) return true;
     h = 0;
     do {
-      ++b;
-      if (b >= a.b.n_seqs) { nt = 0xffffffffu; return; }      // (nobody walks beyond the last item)
+      if (++b >= a.b.n_seqs) return false;
       load(a, cap);
     } while (nt == 0u);
+    return true;
   }
 };
 
-template <bool BF, bool Q8, int HD>
+// NR: groups of 8 rows.
+template <bool BF, bool Q8, int HD, int NR>
 __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_constant__ AttendArgs a) {
   using Sh = StepShape<Q8, HD>;
-  constexpr int KT = Sh::KT, CH = Sh::CH, NT = KT / 8;
+  constexpr int KT = Sh::KT, CH = Sh::CH, MT = KT / 16;
+  constexpr uint32_t kPitch = NR == 1 ? HD + 4 : HD;          // of a result's rows in a stage
+  static_assert(2 * Sh::kBytes >= 8 * NR * static_cast<int>(kPitch) * 4, "a stage holds a warp's result");
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ StepShared S;
   const uint32_t tid = threadIdx.x, w = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u, quad = lane >> 2, t4 = lane & 3u;
   const uint64_t cap = capacity_of(a.c, a.b);
-  // ---- how many tiles there are, and where this CTA's run of them begins ----
-  auto tiles_of = [&](uint32_t i) -> unsigned long long {
+  // ---- how much work there is, and where this CTA's run of it begins ----
+  auto units_of = [&](uint32_t i, uint32_t &items) -> unsigned long long {
     Walk<KT> x;
     x.b = i; x.h = 0;
     x.load(a, cap);
     if (x.s.bad && blockIdx.x == 0u) cache_fault(a.c.status, kStBadBatch, i, static_cast<uint32_t>(x.s.bad), static_cast<uint32_t>(x.s.value));
-    return static_cast<unsigned long long>(x.nt) * a.c.heads;
+    items = x.nt ? a.c.heads : 0u;
+    return x.nt ? static_cast<unsigned long long>(x.nt + kItemTiles) * a.c.heads : 0ull;
   };
-  unsigned long long mine = 0;
-  for (uint32_t i = tid; i < a.b.n_seqs; i += kStepThreads) mine += tiles_of(i);
-  const unsigned long long sum = warp_reduce(mine, [](unsigned long long x, unsigned long long y) { return x + y; });
-  if (lane == 0u) S.sum[w] = sum;
+  unsigned long long mine = 0, many = 0, first_units = 0;
+  for (uint32_t i = tid; i < a.b.n_seqs; i += kStepThreads) {
+    uint32_t items;
+    const unsigned long long u = units_of(i, items);
+    if (i == tid) first_units = u;
+    mine += u;
+    many += items;
+  }
+  auto add = [](unsigned long long x, unsigned long long y) { return x + y; };
+  mine = warp_reduce(mine, add);
+  many = warp_reduce(many, add);
+  if (lane == 0u) { S.sum[0][w] = mine; S.sum[1][w] = many; }
   if (tid == 0u) S.redo[0] = 0u;
   __syncthreads();
-  unsigned long long U = 0;
+  unsigned long long U = 0, items = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < kStepWarps; ++i) U += S.sum[i];
+  for (uint32_t i = 0; i < kStepWarps; ++i) { U += S.sum[0][i]; items += S.sum[1][i]; }
   if (U == 0ull) return;
-  // every CTA that takes part has a tile for each of its warps, where there are as many
-  unsigned long long G = U / kStepWarps;
+  // As many CTAs as give each warp a tile; but items of up to four tiles for each of a CTA's warps are not split for that (300 keys, 8 heads:
+  // joining two or three CTAs' results takes longer than another round of tiles).
+  const unsigned long long tiles = U - items * kItemTiles;
+  unsigned long long G = tiles / kStepWarps;
+  if (G > items && tiles <= items * 4ull * kStepWarps) G = items;
   G = G < 1ull ? 1ull : G > gridDim.x ? gridDim.x : G;
   if (blockIdx.x >= G) return;
   const unsigned long long u0 = U * blockIdx.x / G, u1 = U * (blockIdx.x + 1ull) / G;
-  {
-    unsigned long long run = 0;
-    for (uint32_t i0 = 0; i0 < a.b.n_seqs; i0 += kStepThreads) {
-      const uint32_t i = i0 + tid;
-      const unsigned long long v = i < a.b.n_seqs ? (a.b.n_seqs <= kStepThreads ? mine : tiles_of(i)) : 0ull;
-      unsigned long long x = v;
-#pragma unroll
-      for (uint32_t o = 1; o < 32u; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      __syncthreads();
-      if (lane == 31u) S.scan[w] = x;
-      __syncthreads();
-      unsigned long long before = run;
-      for (uint32_t k = 0; k < kStepWarps; ++k) {
-        if (k < w) before += S.scan[k];
-        run += S.scan[k];
-      }
-      if (before + x > u0 && before + x - v <= u0) {
-        S.found_seq = i;
-        S.found_base = before + x - v;
-      }
-      if (run > u0) break;                                // (the same for all threads)
-    }
-    __syncthreads();
-  }
   Walk<KT> cw;                                            // the item being worked on
-  cw.b = S.found_seq;
+  unsigned long long x0;                                  // its place: kItemTiles units, then its tiles
+  uint32_t ignored;
+  if (!find_unit<kStepThreads>(a.b.n_seqs, u0, S.find, [&](uint32_t i) { return a.b.n_seqs <= kStepThreads ? first_units : units_of(i, ignored); }, cw.b, x0)) return;
   cw.load(a, cap);
-  cw.h = static_cast<uint32_t>((u0 - S.found_base) / cw.nt);
-  uint32_t t_begin = static_cast<uint32_t>((u0 - S.found_base) - static_cast<unsigned long long>(cw.h) * cw.nt);
+  const uint32_t per = cw.nt + kItemTiles;
+  cw.h = static_cast<uint32_t>((u0 - x0) / per);
+  x0 += static_cast<unsigned long long>(cw.h) * per;
+  // tiles [t_begin, t_end) of the item are this CTA's
+  auto tile_at = [](unsigned long long u, unsigned long long x, uint32_t nt) -> uint32_t {
+    return u <= x + kItemTiles ? 0u : static_cast<uint32_t>(min(static_cast<unsigned long long>(nt), u - x - kItemTiles));
+  };
+  uint32_t t_begin = tile_at(u0, x0, cw.nt), t_end = tile_at(u1, x0, cw.nt);
+  if (t_begin >= t_end) return;                           // (a run that is shorter than what an item costs beside its tiles)
 
-  // ---- the warp's copies: its tiles are w, w + 8, .. of the CTA's ----
+  // ---- the warp's copies: its tiles are w, w + 12, .. of the CTA's ----
   uint8_t *const ring = sm + w * (kStages * Sh::kStage);
   const uint32_t ring_s = smem_addr(ring);
   Walk<KT> pw = cw;                                       // the item of the next tile to fetch
-  unsigned long long pt = static_cast<unsigned long long>(t_begin) + w;     // its tile in that item
-  unsigned long long p_left = u1 - u0 > w ? (u1 - u0 - w + kStepWarps - 1ull) / kStepWarps : 0ull;    // tiles still to fetch
+  uint32_t p_tile = t_begin + w, p_end = t_end;           // its tile there, and the end of the CTA's tiles there
+  unsigned long long px = x0;
+  bool p_more = true;
   uint32_t issued = 0;
   int32_t page = -1;                                      // page number of the lane's key in that tile
   uint32_t key_slot = 0, key_entry = 0;
   bool key_live = false;
   auto look_ahead = [&]() {                               // the next tile's place, and its keys' pages on the way
-    if (p_left == 0ull) return;
-    while (pt >= pw.nt) { pt -= pw.nt; pw.next(a, cap); }
-    const int32_t j = pw.keys.lo + static_cast<int32_t>(pt) * KT + static_cast<int32_t>(lane);
+    while (p_more && p_tile >= p_end) {
+      p_tile -= p_end;
+      px += pw.nt + kItemTiles;
+      p_more = px + kItemTiles < u1 && pw.next(a, cap);
+      p_end = p_more ? tile_at(u1, px, pw.nt) : 0u;
+    }
+    if (!p_more) return;
+    const int32_t j = pw.keys.lo + static_cast<int32_t>(p_tile) * KT + static_cast<int32_t>(lane);
     key_live = lane < KT && j < pw.keys.hi;
     if (key_live) {
       key_entry = a.c.by_page.quot(static_cast<uint32_t>(j));
@@ -158,28 +177,44 @@ __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_c
     }
   };
   auto issue = [&]() {
-    if (p_left != 0ull) {
+    if (p_more) {
       const uint32_t st = ring_s + (issued % kStages) * Sh::kStage;
-      int64_t off = 0;
       bool live = key_live;
       if (live && static_cast<uint32_t>(page) >= a.c.n_pages) {
         cache_fault(a.c.status, kStBadPage, pw.b, key_entry, static_cast<uint32_t>(page));
         live = false;
       }
-      if (live) off = page * a.c.page_bytes + key_slot * a.c.slot_bytes + pw.h * a.c.head_bytes;
       const uint32_t mask = __ballot_sync(0xffffffffu, live);
-      constexpr int kRowsAtOnce = 32 / CH;
+      constexpr int kAtOnce = 32 / CH;
       const uint32_t sub = lane % CH, r0 = lane / CH;
       const bool in_hd = sub * 16u < a.c.hd * (Q8 ? 1u : 2u);
+      const int64_t head_at = pw.h * a.c.head_bytes + sub * 16u;
+      const uint32_t entry0 = __shfl_sync(0xffffffffu, key_entry, 0);
+      constexpr uint32_t kAll = KT == 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u;
+      if (mask == kAll && __all_sync(0xffffffffu, lane >= KT || key_entry == entry0)) {     // a whole tile in one page
+        int64_t o = __shfl_sync(0xffffffffu, page, 0) * a.c.page_bytes + (__shfl_sync(0xffffffffu, key_slot, 0) + r0) * a.c.slot_bytes + head_at;
+        if (!in_hd) o = 0;
+        const int64_t step = in_hd ? kAtOnce * a.c.slot_bytes : 0;
+        const uint32_t bytes = in_hd ? 16u : 0u;
+        const uint8_t *kp = a.c.k + o, *vp = a.c.v + o;
 #pragma unroll
-      for (int i = 0; i < KT / kRowsAtOnce; ++i) {
-        const uint32_t r = i * kRowsAtOnce + r0;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r);
-        const uint32_t bytes = ((mask >> r) & 1u) && in_hd ? 16u : 0u;         // else zeros
-        const int64_t at = bytes ? o + sub * 16u : 0;
-        const uint32_t dst = st + chunk_at<CH>(r, sub);
-        cp_async_16_zfill(dst, a.c.k + at, bytes);
-        cp_async_16_zfill(dst + Sh::kBytes, a.c.v + at, bytes);
+        for (int i = 0; i < KT / kAtOnce; ++i, kp += step, vp += step) {
+          const uint32_t dst = st + chunk_at<CH>(i * kAtOnce + r0, sub);
+          cp_async_16_zfill(dst, kp, bytes);
+          cp_async_16_zfill(dst + Sh::kBytes, vp, bytes);
+        }
+      } else {
+        const int64_t off = live ? page * a.c.page_bytes + key_slot * a.c.slot_bytes : 0;
+#pragma unroll
+        for (int i = 0; i < KT / kAtOnce; ++i) {
+          const uint32_t r = i * kAtOnce + r0;
+          const int64_t o = __shfl_sync(0xffffffffu, off, r);
+          const uint32_t bytes = ((mask >> r) & 1u) && in_hd ? 16u : 0u;       // else zeros
+          const int64_t at = bytes ? o + head_at : 0;
+          const uint32_t dst = st + chunk_at<CH>(r, sub);
+          cp_async_16_zfill(dst, a.c.k + at, bytes);
+          cp_async_16_zfill(dst + Sh::kBytes, a.c.v + at, bytes);
+        }
       }
       if (Q8) {
         const int64_t so = live ? page * a.c.s_page + key_slot * a.c.s_slot + pw.h * a.c.s_head : 0;
@@ -187,203 +222,275 @@ __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_c
         cp_async_4_zfill(dst, a.c.ks + so, live ? 4u : 0u);
         cp_async_4_zfill(dst + KT * 4u, a.c.vs + so, live ? 4u : 0u);
       }
-      --p_left;
-      pt += kStepWarps;
+      p_tile += kStepWarps;
     }
     cp_async_commit();
     ++issued;
     look_ahead();
   };
-  look_ahead();
-  issue();
-  issue();
-
-  uint32_t taken = 0, turn = 0;                           // tiles that the warp has worked on; items so far
-  unsigned long long u = u0;
-  unsigned long long wu = u0 + w;                         // the warp's next tile among all
-  while (u < u1) {
-    const uint32_t t_end = static_cast<uint32_t>(min(static_cast<unsigned long long>(cw.nt), t_begin + (u1 - u)));
-    const unsigned long long u_end = u + (t_end - t_begin);
-    const uint32_t rows = static_cast<uint32_t>(cw.s.n) * a.group;
-    // this thread's rows of the products: quad and quad + 8
-    Span sp[2];
-    float sl2[2] = {a.scale_log2, a.scale_log2};
-    uint32_t qf[HD / 16][4];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[HD / 8][4];
-    const bool any = wu < u_end;
-    if (any) {
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) { o[i][0] = 0.0f; o[i][1] = 0.0f; o[i][2] = 0.0f; o[i][3] = 0.0f; }
-      float top[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t r = quad + 8u * half, tok = r / a.group;
-        const bool live = r < rows;
-        sp[half] = live ? SeenBy(cw.s, static_cast<int32_t>(tok), a.causal, a.window) : Span{0, 0};
-        const uint8_t *p = live ? row_at(a.q, cw.s.first + static_cast<int32_t>(tok), cw.h * a.group + (r - tok * a.group)) : a.q.p;
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-          for (int b8 = 0; b8 < 2; ++b8) {
-            // 8-bit pages: a thread's values of two products lie side by side (see the K operand below)
-            const uint32_t d = Q8 ? (ks >> 1) * 32u + 8u * t4 + 4u * (ks & 1) + 2u * b8 : ks * 16u + 2u * t4 + 8u * b8;
-            uint32_t v = 0u;
-            if (live && d < a.c.hd) v = *reinterpret_cast<const uint16_t *>(p + 2u * d) | (static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(p + 2u * d + 2u)) << 16);
-            qf[ks][half + 2 * b8] = v;
-            if (Q8 && BF) top[half] = fmaxf(top[half], fmaxf(fabsf(__uint_as_float(v << 16)), fabsf(__uint_as_float(v & 0xffff0000u))));
-          }
-      }
-      if (Q8 && BF) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float x = fmaxf(top[half], __shfl_xor_sync(0xffffffffu, top[half], 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          // 2^e brings the largest to [2^14, 2^15); rows of zeros, and of what is not finite, stay as they are
-          const int ex = static_cast<int>(__float_as_uint(x) >> 23);
-          const int e = ex == 0 || ex == 255 ? 0 : max(-100, min(100, 127 + 14 - ex));
-          const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          sl2[half] = a.scale_log2 * down;
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-            for (int b8 = 0; b8 < 2; ++b8) {
-              const uint32_t v = qf[ks][half + 2 * b8];
-              qf[ks][half + 2 * b8] = cvt_f16x2(__uint_as_float(v & 0xffff0000u) * up, __uint_as_float(v << 16) * up);
-            }
-        }
+  // q of an item: [16 rows][HD], rows and values that are not there as zeros
+  const uint32_t q_s = smem_addr(sm + Sh::kRing);
+  const bool q_vec = ((reinterpret_cast<uintptr_t>(a.q.p) & 15u) | ((a.q.row | a.q.head) & 7)) == 0;
+  auto fetch_q = [&](const Walk<KT> &x, uint32_t buf) {
+    constexpr uint32_t QC = HD / 8;
+    const uint32_t rows = static_cast<uint32_t>(x.s.n) * a.group;
+    for (uint32_t i = tid; i < 8u * NR * QC; i += kStepThreads) {
+      const uint32_t r = i / QC, c = i - r * QC, tok = r / a.group;
+      const bool live = r < rows && c * 8u < a.c.hd;
+      const uint8_t *p = live ? row_at(a.q, x.s.first + static_cast<int32_t>(tok), x.h * a.group + (r - tok * a.group)) + 16u * c : a.q.p;
+      const uint32_t dst = q_s + buf * Sh::kQ + chunk_at<QC>(r, c);
+      if (q_vec) {
+        cp_async_16_zfill(dst, p, live ? 16u : 0u);
+      } else {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        const uint16_t *e = reinterpret_cast<const uint16_t *>(p);
+        if (live) v = make_uint4(e[0] | (static_cast<uint32_t>(e[1]) << 16), e[2] | (static_cast<uint32_t>(e[3]) << 16), e[4] | (static_cast<uint32_t>(e[5]) << 16), e[6] | (static_cast<uint32_t>(e[7]) << 16));
+        sts_v4(dst, v);
       }
     }
-    float v_ref[2] = {0.0f, 0.0f};                        // 8-bit pages: power of two not below the scales that the row has seen, 0 = none yet
-    for (; wu < u_end; wu += kStepWarps, ++taken) {
-      cp_async_wait<1>();
-      __syncwarp();
-      issue();                                            // into the stage before last
-      const uint32_t st = ring_s + (taken % kStages) * Sh::kStage;
-      const int32_t j0 = cw.keys.lo + static_cast<int32_t>(t_begin + static_cast<uint32_t>(wu - u)) * KT;
-      float s[NT][4];
+  };
+  look_ahead();
+  fetch_q(cw, 0u);
+  cp_async_commit();
+  issue();
+  cp_async_wait<1>();
+  __syncthreads();
+
+  uint32_t taken = 0, turn = 0;                           // tiles that the warp has worked on; items so far
+  uint32_t w_tile = t_begin + w;                          // the warp's next tile, in the item
+  Walk<KT> nw = cw;                                       // the item after
+  for (;;) {
+    const unsigned long long nx = x0 + cw.nt + kItemTiles;
+    bool more = nx + kItemTiles < u1;                     // (a tile of the next item lies in the CTA's run)
+    if (more) more = nw.next(a, cap);
+    const uint32_t rows = static_cast<uint32_t>(cw.s.n) * a.group;
+    const bool any = w_tile < t_end;
+    // this thread's rows (columns of the products): 8 g + 2 t4 + e
+    Span sp[NR][2];
+    float sl2[NR][2], m[NR][2], l[NR][2], v_ref[NR][2];   // v_ref, 8-bit pages: power of two not below the scales that the row has seen, 0 = none yet
+    uint32_t qf[NR][HD / 16][2];
+    float o[NR][HD / 16][4];
+    int32_t full_lo = 0, full_hi = 0x7fffffff;            // keys that all rows see
+    if (any) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) { s[n][0] = 0.0f; s[n][1] = 0.0f; s[n][2] = 0.0f; s[n][3] = 0.0f; }
+      for (int g = 0; g < NR; ++g) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) { o[g][i][0] = 0.0f; o[g][i][1] = 0.0f; o[g][i][2] = 0.0f; o[g][i][3] = 0.0f; }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t r = 8u * g + 2u * t4 + e;
+          sp[g][e] = r < rows ? SeenBy(cw.s, static_cast<int32_t>(r / a.group), a.causal, a.window) : Span{0, 0};
+          sl2[g][e] = a.scale_log2; m[g][e] = -INFINITY; l[g][e] = 0.0f; v_ref[g][e] = 0.0f;
+        }
+        const uint32_t qb = q_s + (turn & 1u) * Sh::kQ;
+        if constexpr (!Q8) {
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ks += 2) {
+            uint32_t b[4];
+            ldmatrix_x4(b, qb + chunk_at<HD / 8>(8u * g + (lane & 7u), ks * 2 + (lane >> 3)));
+            qf[g][ks][0] = b[0]; qf[g][ks][1] = b[1]; qf[g][ks + 1][0] = b[2]; qf[g][ks + 1][1] = b[3];
+          }
+        } else {
+          float top = 0.0f;
+#pragma unroll
+          for (int seg = 0; seg < HD / 32; ++seg) {       // eight values side by side: those of product 2 seg first (as K's codes lie)
+            const uint4 v = lds_v4(qb + chunk_at<HD / 8>(8u * g + quad, seg * 4 + t4));
+            qf[g][2 * seg][0] = v.x; qf[g][2 * seg][1] = v.y; qf[g][2 * seg + 1][0] = v.z; qf[g][2 * seg + 1][1] = v.w;
+            if (BF) {
+              const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(ww[i] << 16)), fabsf(__uint_as_float(ww[i] & 0xffff0000u))));
+            }
+          }
+          if (BF) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^e brings the largest to [2^14, 2^15); rows of zeros, and of what is not finite, stay as they are
+            const int ex = static_cast<int>(__float_as_uint(top) >> 23);
+            const int e = ex == 0 || ex == 255 ? 0 : max(-100, min(100, 127 + 14 - ex));
+            const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) qf[g][ks][i] = cvt_f16x2(__uint_as_float(qf[g][ks][i] & 0xffff0000u) * up, __uint_as_float(qf[g][ks][i] << 16) * up);
+            sl2[g][0] *= __shfl_sync(0xffffffffu, down, 8u * t4);
+            sl2[g][1] *= __shfl_sync(0xffffffffu, down, 8u * t4 + 4u);
+          }
+        }
+      }
+      if (cw.s.n > 0) {
+        full_lo = SeenBy(cw.s, cw.s.n - 1, a.causal, a.window).lo;
+        full_hi = SeenBy(cw.s, 0, a.causal, a.window).hi;
+      }
+    }
+    if (more) fetch_q(nw, (turn + 1u) & 1u);              // (on the way with the next tile's copies)
+    for (; w_tile < t_end; w_tile += kStepWarps, ++taken) {
+      cp_async_wait_all();
+      __syncwarp();
+      issue();                                            // into the other stage
+      const uint32_t st = ring_s + (taken % kStages) * Sh::kStage;
+      const int32_t j0 = cw.keys.lo + static_cast<int32_t>(w_tile) * KT;
+      float s[NR][MT][4];
+#pragma unroll
+      for (int g = 0; g < NR; ++g)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) { s[g][t][0] = 0.0f; s[g][t][1] = 0.0f; s[g][t][2] = 0.0f; s[g][t][3] = 0.0f; }
       if constexpr (!Q8) {
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
-          for (int np = 0; np < NT / 2; ++np) {
-            uint32_t b[4];
-            ldmatrix_x4(b, st + chunk_at<CH>(np * 16 + (lane >> 4) * 8 + (lane & 7u), ks * 2 + ((lane >> 3) & 1u)));
-            if (BF) { mma_bf16_16816(s[2 * np], qf[ks], b[0], b[1]); mma_bf16_16816(s[2 * np + 1], qf[ks], b[2], b[3]); }
-            else { mma_f16_16816(s[2 * np], qf[ks], b[0], b[1]); mma_f16_16816(s[2 * np + 1], qf[ks], b[2], b[3]); }
+          for (int t = 0; t < MT; ++t) {
+            uint32_t x[4];
+            ldmatrix_x4(x, st + chunk_at<CH>(t * 16 + (lane & 15u), ks * 2 + (lane >> 4)));
+#pragma unroll
+            for (int g = 0; g < NR; ++g) {
+              if (BF) mma_bf16_16816(s[g][t], x, qf[g][ks][0], qf[g][ks][1]);
+              else mma_f16_16816(s[g][t], x, qf[g][ks][0], qf[g][ks][1]);
+            }
           }
       } else {
 #pragma unroll
         for (int seg = 0; seg < HD / 32; ++seg)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            // eight codes of key `quad`, those of product 2 seg first; the order along d is Q's
-            uint2 c;
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c.x), "=r"(c.y) : "r"(st + chunk_at<CH>(n * 8 + quad, seg * 2 + (t4 >> 1)) + (t4 & 1u) * 8u) : "memory");
-            mma_f16_16816(s[n], qf[2 * seg], cvt_e4m3x2_f16x2(c.x & 0xffffu), cvt_e4m3x2_f16x2(c.x >> 16));
-            mma_f16_16816(s[n], qf[2 * seg + 1], cvt_e4m3x2_f16x2(c.y & 0xffffu), cvt_e4m3x2_f16x2(c.y >> 16));
+          for (int t = 0; t < MT; ++t) {
+            // eight codes each of keys `quad` and `quad` + 8, those of product 2 seg first
+            uint2 c[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c[i].x), "=r"(c[i].y) : "r"(st + chunk_at<CH>(t * 16 + i * 8 + quad, seg * 2 + (t4 >> 1)) + (t4 & 1u) * 8u) : "memory");
+            const uint32_t x0f[4] = {cvt_e4m3x2_f16x2(c[0].x & 0xffffu), cvt_e4m3x2_f16x2(c[1].x & 0xffffu), cvt_e4m3x2_f16x2(c[0].x >> 16), cvt_e4m3x2_f16x2(c[1].x >> 16)};
+            const uint32_t x1f[4] = {cvt_e4m3x2_f16x2(c[0].y & 0xffffu), cvt_e4m3x2_f16x2(c[1].y & 0xffffu), cvt_e4m3x2_f16x2(c[0].y >> 16), cvt_e4m3x2_f16x2(c[1].y >> 16)};
+#pragma unroll
+            for (int g = 0; g < NR; ++g) {
+              mma_f16_16816(s[g][t], x0f, qf[g][2 * seg][0], qf[g][2 * seg][1]);
+              mma_f16_16816(s[g][t], x1f, qf[g][2 * seg + 1][0], qf[g][2 * seg + 1][1]);
+            }
           }
       }
-      // scores in the log2 domain, keys that the row does not see at -inf
-      float mx[2] = {-INFINITY, -INFINITY}, v_top[2] = {0.0f, 0.0f};
-      float2 vs2[NT];
+      // scores in the log2 domain, keys that the row does not see at -inf; the thread's keys: 16 t + quad, + 8
+      const bool whole = j0 >= full_lo && j0 + KT <= full_hi;
+      float vs[MT][2], top[NR][2], v_top[NR][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float2 ks2 = make_float2(1.0f, 1.0f);
+      for (int g = 0; g < NR; ++g) { top[g][0] = top[g][1] = -INFINITY; v_top[g][0] = v_top[g][1] = 0.0f; }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        float ksc[2] = {1.0f, 1.0f};
         if (Q8) {
-          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks2.x), "=f"(ks2.y) : "r"(st + 2u * Sh::kBytes + (n * 8 + 2u * t4) * 4u) : "memory");
-          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(vs2[n].x), "=f"(vs2[n].y) : "r"(st + 2u * Sh::kBytes + (KT + n * 8 + 2u * t4) * 4u) : "memory");
-        }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int32_t j = j0 + n * 8 + static_cast<int32_t>(2u * t4) + (c & 1);
-          const float x = s[n][c] * (Q8 ? sl2[c >> 1] * ((c & 1) ? ks2.y : ks2.x) : sl2[c >> 1]);
-          const bool seen = j >= sp[c >> 1].lo && j < sp[c >> 1].hi;
-          s[n][c] = seen ? x : -INFINITY;
-          if (Q8) v_top[c >> 1] = fmaxf(v_top[c >> 1], seen ? ((c & 1) ? vs2[n].y : vs2[n].x) : 0.0f);
-          // (a NaN must not be lost here: fmaxf would drop it, and the sum below finds it again)
-          mx[c >> 1] = fmaxf(mx[c >> 1], s[n][c]);
-        }
-      }
-      float corr[2];
-      bool moved = false;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
-        mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
-        const float m2 = fmaxf(m[half], mx[half]);
-        corr[half] = m[half] == m2 ? 1.0f : m[half] == -INFINITY ? 0.0f : fast_ex2(m[half] - m2);
-        moved = moved || corr[half] != 1.0f;
-        m[half] = m2;
-        l[half] *= corr[half];
-      }
-      float v_mul[2] = {1.0f, 1.0f};
-      if (Q8) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float x = fmaxf(v_top[half], __shfl_xor_sync(0xffffffffu, v_top[half], 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          const float ref = __uint_as_float(min(250u, max(4u, (__float_as_uint(x) >> 23) + 1u)) << 23);
-          if (ref > v_ref[half]) {
-            corr[half] *= v_ref[half] / ref;              // (a power of two, or 0 at first)
-            moved = true;
-            v_ref[half] = ref;
+          for (int i = 0; i < 2; ++i) {
+            ksc[i] = lds_f32(st + 2u * Sh::kBytes + (t * 16 + i * 8 + quad) * 4u);
+            vs[t][i] = lds_f32(st + 2u * Sh::kBytes + (KT + t * 16 + i * 8 + quad) * 4u);
           }
-          v_mul[half] = kPScale / v_ref[half];
-        }
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
-      }
-      const float neg[2] = {m[0] == -INFINITY ? 0.0f : -m[0], m[1] == -INFINITY ? 0.0f : -m[1]};
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float p = fast_ex2(s[n][c] + neg[c >> 1]);
-          l[c >> 1] += p;
-          s[n][c] = Q8 ? (p == 0.0f ? 0.0f : p * (((c & 1) ? vs2[n].y : vs2[n].x) * v_mul[c >> 1])) : p;
-        }
-      }
-#pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk) {
-        const float(&x)[4] = s[2 * kk];
-        const float(&y)[4] = s[2 * kk + 1];
-        uint32_t pa[4], pl[4];
-        if (BF && !Q8) {
-          pa[0] = cvt_bf16x2(x[1], x[0]); pa[1] = cvt_bf16x2(x[3], x[2]); pa[2] = cvt_bf16x2(y[1], y[0]); pa[3] = cvt_bf16x2(y[3], y[2]);
-          auto left = [](float hi, float lo, uint32_t r) { return cvt_bf16x2(hi - __uint_as_float(r & 0xffff0000u), lo - __uint_as_float(r << 16)); };
-          pl[0] = left(x[1], x[0], pa[0]); pl[1] = left(x[3], x[2], pa[1]); pl[2] = left(y[1], y[0], pa[2]); pl[3] = left(y[3], y[2], pa[3]);
-        } else {
-          pa[0] = cvt_f16x2(x[1], x[0]); pa[1] = cvt_f16x2(x[3], x[2]); pa[2] = cvt_f16x2(y[1], y[0]); pa[3] = cvt_f16x2(y[3], y[2]);
         }
 #pragma unroll
-        for (int n2 = 0; n2 < HD / 16; ++n2) {
-          uint32_t b[4];
-          if constexpr (!Q8) {
-            ldmatrix_x4_trans(b, st + Sh::kBytes + chunk_at<CH>(kk * 16 + ((lane >> 3) & 1u) * 8 + (lane & 7u), n2 * 2 + (lane >> 4)));
-            if (BF) {
-              mma_bf16_16816(o[2 * n2], pa, b[0], b[1]); mma_bf16_16816(o[2 * n2 + 1], pa, b[2], b[3]);
-              mma_bf16_16816(o[2 * n2], pl, b[0], b[1]); mma_bf16_16816(o[2 * n2 + 1], pl, b[2], b[3]);
+        for (int g = 0; g < NR; ++g)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int32_t j = j0 + t * 16 + static_cast<int32_t>(quad) + 8 * (c >> 1);
+            const int e = c & 1;
+            const bool seen = whole || (j >= sp[g][e].lo && j < sp[g][e].hi);
+            const float x = s[g][t][c] * (Q8 ? sl2[g][e] * ksc[c >> 1] : sl2[g][e]);
+            s[g][t][c] = seen ? x : -INFINITY;
+            // (a NaN is dropped here; the sum of the weights finds it)
+            top[g][e] = fmaxf(top[g][e], s[g][t][c]);
+            if (Q8) v_top[g][e] = fmaxf(v_top[g][e], seen ? vs[t][c >> 1] : 0.0f);
+          }
+      }
+      bool grow = false;
+#pragma unroll
+      for (int g = 0; g < NR; ++g)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) grow = grow || top[g][e] > m[g][e] + kGrow || (Q8 && v_top[g][e] >= v_ref[g][e] && v_top[g][e] > 0.0f);
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int g = 0; g < NR; ++g) {
+          float corr[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = top[g][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            corr[e] = 1.0f;
+            if (x > m[g][e] + kGrow) {
+              corr[e] = m[g][e] == -INFINITY ? 0.0f : fast_ex2(m[g][e] - x);
+              l[g][e] *= corr[e];
+              m[g][e] = x;
+            }
+            if (Q8) {
+              float v = v_top[g][e];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+              const float ref = power_above(v);
+              if (ref > v_ref[g][e]) {
+                corr[e] *= v_ref[g][e] / ref;             // (a power of two, or 0 at first)
+                v_ref[g][e] = ref;
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i) { o[g][i][0] *= corr[0]; o[g][i][1] *= corr[1]; o[g][i][2] *= corr[0]; o[g][i][3] *= corr[1]; }
+        }
+      }
+      uint32_t pb[NR][MT][2], pl[NR][MT][2];
+#pragma unroll
+      for (int g = 0; g < NR; ++g) {
+        float neg[2], mul[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          neg[e] = m[g][e] == -INFINITY ? 0.0f : -m[g][e];
+          // kPScale / v_ref of a power of two: by its exponent
+          mul[e] = Q8 && v_ref[g][e] > 0.0f ? __uint_as_float(__float_as_uint(kPScale) + (127u << 23) - __float_as_uint(v_ref[g][e])) : 0.0f;
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int e = c & 1;
+            const float p = fast_ex2(s[g][t][c] + neg[e]);
+            l[g][e] += p;
+            s[g][t][c] = Q8 ? (p == 0.0f ? 0.0f : p * (vs[t][c >> 1] * mul[e])) : p;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float lo = s[g][t][2 * i], hi = s[g][t][2 * i + 1];
+            if (BF && !Q8) {
+              const uint32_t r = cvt_bf16x2(hi, lo);
+              pb[g][t][i] = transposed(r);
+              pl[g][t][i] = transposed(cvt_bf16x2(hi - __uint_as_float(r & 0xffff0000u), lo - __uint_as_float(r << 16)));
             } else {
-              mma_f16_16816(o[2 * n2], pa, b[0], b[1]); mma_f16_16816(o[2 * n2 + 1], pa, b[2], b[3]);
+              pb[g][t][i] = transposed(cvt_f16x2(hi, lo));
             }
-          } else if (kk == 0) {
-            // Transposed by pairs of codes: a register holds d = 2 quad and 2 quad + 1 of two keys; split, the even and the odd values of
-            // the 16 are one column tile each. Both halves of the 32 keys come at once.
-            ldmatrix_x4_trans(b, st + Sh::kBytes + chunk_at<CH>((lane >> 3) * 8 + (lane & 7u), n2));
-            uint32_t pb[4];
-            const float(&x2)[4] = s[NT > 2 ? 2 : 0];
-            const float(&y2)[4] = s[NT > 2 ? 3 : 1];
-            pb[0] = cvt_f16x2(x2[1], x2[0]); pb[1] = cvt_f16x2(x2[3], x2[2]); pb[2] = cvt_f16x2(y2[1], y2[0]); pb[3] = cvt_f16x2(y2[3], y2[2]);
+          }
+        }
+      }
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
-              const uint32_t c0 = __byte_perm(b[2 * k2], 0u, 0x3120), c1 = __byte_perm(b[2 * k2 + 1], 0u, 0x3120);
-              mma_f16_16816(o[2 * n2], k2 ? pb : pa, cvt_e4m3x2_f16x2(c0 & 0xffffu), cvt_e4m3x2_f16x2(c1 & 0xffffu));
-              mma_f16_16816(o[2 * n2 + 1], k2 ? pb : pa, cvt_e4m3x2_f16x2(c0 >> 16), cvt_e4m3x2_f16x2(c1 >> 16));
+      for (int n = 0; n < HD / 16; ++n) {
+        if constexpr (!Q8) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            uint32_t x[4];
+            ldmatrix_x4_trans(x, st + Sh::kBytes + chunk_at<CH>(t * 16 + (lane >> 4) * 8 + (lane & 7u), n * 2 + ((lane >> 3) & 1u)));
+#pragma unroll
+            for (int g = 0; g < NR; ++g) {
+              if (BF) {
+                mma_bf16_16816(o[g][n], x, pb[g][t][0], pb[g][t][1]);
+                mma_bf16_16816(o[g][n], x, pl[g][t][0], pl[g][t][1]);
+              } else {
+                mma_f16_16816(o[g][n], x, pb[g][t][0], pb[g][t][1]);
+              }
             }
+          }
+        } else {
+          // Transposed by pairs of codes: a register holds values 2 quad and 2 quad + 1 of two keys; the even ones are rows 0 to 7 of the
+          // product, the odd ones 8 to 15. All 32 keys come at once.
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, st + Sh::kBytes + chunk_at<CH>(lane, n));
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const uint32_t c0 = __byte_perm(b[2 * t], 0u, 0x3120), c1 = __byte_perm(b[2 * t + 1], 0u, 0x3120);
+            const uint32_t x[4] = {cvt_e4m3x2_f16x2(c0 & 0xffffu), cvt_e4m3x2_f16x2(c0 >> 16), cvt_e4m3x2_f16x2(c1 & 0xffffu), cvt_e4m3x2_f16x2(c1 >> 16)};
+#pragma unroll
+            for (int g = 0; g < NR; ++g) mma_f16_16816(o[g][n], x, pb[g][t][0], pb[g][t][1]);
           }
         }
       }
@@ -393,35 +500,37 @@ __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_c
     float *slot = reinterpret_cast<float *>(ring + (issued % kStages) * Sh::kStage);
     if (any) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-        const uint32_t r = quad + 8u * half;
-        if (t4 == 0u) { S.m[w][r] = m[half]; S.l[w][r] = l[half]; }
-        const float mul = Q8 ? v_ref[half] * (1.0f / kPScale) : 1.0f;
-        if (r < rows) {
+      for (int g = 0; g < NR; ++g)
 #pragma unroll
-          for (int i = 0; i < HD / 16; ++i) {
-            const float x0 = o[2 * i][2 * half] * mul, x1 = o[2 * i][2 * half + 1] * mul, y0 = o[2 * i + 1][2 * half] * mul, y1 = o[2 * i + 1][2 * half + 1] * mul;
-            if (Q8) {
-              *reinterpret_cast<float4 *>(slot + r * HD + i * 16 + 4u * t4) = make_float4(x0, y0, x1, y1);
-            } else {
-              *reinterpret_cast<float2 *>(slot + r * HD + i * 16 + 2u * t4) = make_float2(x0, x1);
-              *reinterpret_cast<float2 *>(slot + r * HD + i * 16 + 8u + 2u * t4) = make_float2(y0, y1);
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t r = 8u * g + 2u * t4 + e;
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[g][e] += __shfl_xor_sync(0xffffffffu, l[g][e], d);
+          if (quad == 0u) { S.m[w][r] = m[g][e]; S.l[w][r] = l[g][e]; }
+          const float mul = Q8 ? v_ref[g][e] * (1.0f / kPScale) : 1.0f;
+          if (r < rows) {
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) {
+              const float lo = o[g][n][e] * mul, hi = o[g][n][2 + e] * mul;
+              if (Q8) {
+                *reinterpret_cast<float2 *>(slot + r * kPitch + n * 16 + 2u * quad) = make_float2(lo, hi);
+              } else {
+                slot[r * kPitch + n * 16 + quad] = lo;
+                slot[r * kPitch + n * 16 + 8u + quad] = hi;
+              }
             }
           }
         }
-      }
     } else if (lane < 16u) {
       S.m[w][lane] = -INFINITY;
       S.l[w][lane] = 0.0f;
     }
-    // where each warp's stage is: all warps have issued the same number or one less; the number is left beside m
-    if (lane == 0u) S.scan[w] = issued % kStages;
+    if (lane == 0u) S.at[w] = (w * kStages + issued % kStages) * Sh::kStage;
+    cp_async_commit();
+    cp_async_wait_all();                                  // the next item's q
     __syncthreads();
     if (tid == 0u) S.redo[(turn + 1u) & 1u] = 0u;         // the next item's (everybody is done with the one before)
     const bool whole = t_begin == 0u && t_end == cw.nt;
-    const unsigned long long item0 = u - t_begin, item1 = item0 + cw.nt;      // the item's tiles among all
     // partial results: [CTA][first or last item][16 rows][HD + 2]
     constexpr uint32_t kPart = 16u * (HD + 2u);
     float *part = a.part + (static_cast<size_t>(blockIdx.x) * 2u + (t_begin == 0u ? 1u : 0u)) * kPart;
@@ -452,7 +561,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_c
         // a warp without a tile of this item has left nothing in its stage; one without a key that the row sees has zeros there
         if (S.m[k][r] == -INFINITY && S.l[k][r] == 0.0f) continue;
         const float f = S.m[k][r] == mm ? 1.0f : fast_ex2(S.m[k][r] - mm);
-        const float4 y = *reinterpret_cast<const float4 *>(sm + k * (kStages * Sh::kStage) + S.scan[k] * Sh::kStage + (r * HD + d) * 4u);
+        const float4 y = *reinterpret_cast<const float4 *>(sm + S.at[k] + (r * kPitch + d) * 4u);
         ll += S.l[k][r] * f;
         x.x += y.x * f; x.y += y.y * f; x.z += y.z * f; x.w += y.w * f;
       }
@@ -465,7 +574,8 @@ __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_c
     }
     if (!whole) {
       // the item's CTAs: those whose runs hold its first and its last tile, and all between
-      const uint32_t c0 = static_cast<uint32_t>(((item0 + 1ull) * G - 1ull) / U), c1 = static_cast<uint32_t>((item1 * G - 1ull) / U);
+      const unsigned long long t0 = x0 + kItemTiles, t1 = t0 + cw.nt;
+      const uint32_t c0 = static_cast<uint32_t>(((t0 + 1ull) * G - 1ull) / U), c1 = static_cast<uint32_t>((t1 * G - 1ull) / U);
       __threadfence();
       __syncthreads();
       if (tid == 0u) {
@@ -480,8 +590,10 @@ __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_c
           const uint32_t r = i / (HD / 4), d = (i - r * (HD / 4)) * 4u;
           float mm = -INFINITY, ll = 0.0f;
           auto of = [&](uint32_t c) { return a.part + (static_cast<size_t>(c) * 2u + (c == c0 ? 1u : 0u)) * kPart; };
+#pragma unroll 4
           for (uint32_t c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(of(c) + 16u * HD + r));
           float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
           for (uint32_t c = c0; c <= c1; ++c) {
             const float *p = of(c);
             const float mc = __ldcg(p + 16u * HD + r), lc = __ldcg(p + 16u * HD + 16u + r);
@@ -500,29 +612,43 @@ __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_c
       for (uint32_t r = w; r < rows; r += kStepWarps)
         if ((redo >> r) & 1u) attend_row_alone(a, cw.b, cw.s, static_cast<int32_t>(r / a.group), cw.h * a.group + r % a.group);
     }
-    u = u_end;
-    ++turn;
+    if (!more) break;
+    w_tile -= t_end;                                      // (the warps take the CTA's tiles in turn, across items)
+    x0 = nx;
+    cw = nw;
     t_begin = 0;
-    if (u < u1) cw.next(a, cap);
+    t_end = tile_at(u1, x0, cw.nt);
+    ++turn;
   }
   cp_async_wait_all();
 }
 
-template <bool BF, bool Q8, int HD>
+template <bool BF, bool Q8, int HD, int NR>
 int Launch(const AttendArgs &a, uint32_t sms, cudaStream_t stream) {
-  b2_attend_step<BF, Q8, HD><<<sms, kStepThreads, StepShape<Q8, HD>::kSmem, stream>>>(a);
+  b2_attend_step<BF, Q8, HD, NR><<<sms, kStepThreads, StepShape<Q8, HD>::kSmem, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
-template <bool BF, bool Q8, int HD>
+template <bool BF, bool Q8, int HD, int NR>
 cudaError_t Attr() {
-  return cudaFuncSetAttribute(b2_attend_step<BF, Q8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, StepShape<Q8, HD>::kSmem);
+  return cudaFuncSetAttribute(b2_attend_step<BF, Q8, HD, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, StepShape<Q8, HD>::kSmem);
+}
+template <bool BF, bool Q8>
+cudaError_t Attrs() {
+  for (cudaError_t e : {Attr<BF, Q8, 64, 1>(), Attr<BF, Q8, 64, 2>(), Attr<BF, Q8, 128, 1>(), Attr<BF, Q8, 128, 2>()})
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
+}
+template <bool BF, bool Q8>
+int Choose(const AttendArgs &a, uint32_t sms, cudaStream_t s) {
+  const bool wide = a.b.max_rows * a.group > 8u;
+  if (a.c.hd > 64u) return wide ? Launch<BF, Q8, 128, 2>(a, sms, s) : Launch<BF, Q8, 128, 1>(a, sms, s);
+  return wide ? Launch<BF, Q8, 64, 2>(a, sms, s) : Launch<BF, Q8, 64, 1>(a, sms, s);
 }
 
 }  // namespace
 
 int PrepareAttendStep() {
-  for (cudaError_t e : {Attr<true, false, 64>(), Attr<true, false, 128>(), Attr<false, false, 64>(), Attr<false, false, 128>(), Attr<true, true, 64>(), Attr<true, true, 128>(),
-                        Attr<false, true, 64>(), Attr<false, true, 128>()})
+  for (cudaError_t e : {Attrs<true, false>(), Attrs<false, false>(), Attrs<true, true>(), Attrs<false, true>()})
     if (e != cudaSuccess) return static_cast<int>(e);
   return 0;
 }
@@ -530,13 +656,8 @@ size_t AttendStepPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * 
 
 int LaunchAttendStep(const AttendArgs &a, uint32_t sms, CUstream_st *stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const bool big = a.c.hd > 64u;
-  if (a.e4m3) {
-    if (a.bf16) return big ? Launch<true, true, 128>(a, sms, s) : Launch<true, true, 64>(a, sms, s);
-    return big ? Launch<false, true, 128>(a, sms, s) : Launch<false, true, 64>(a, sms, s);
-  }
-  if (a.bf16) return big ? Launch<true, false, 128>(a, sms, s) : Launch<true, false, 64>(a, sms, s);
-  return big ? Launch<false, false, 128>(a, sms, s) : Launch<false, false, 64>(a, sms, s);
+  if (a.e4m3) return a.bf16 ? Choose<true, true>(a, sms, s) : Choose<false, true>(a, sms, s);
+  return a.bf16 ? Choose<true, false>(a, sms, s) : Choose<false, false>(a, sms, s);
 }
 
 }  // namespace b2

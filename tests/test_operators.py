@@ -385,6 +385,23 @@ def test_what_a_row_does_not_see_does_not_reach_it(rt, scratch, dtype, rows, pas
                 assert not bool(torch.isfinite(got[sees]).any()), (c, value)
 
 
+@pytest.mark.parametrize("rows, q_heads", [(1, 4), (2, 8), (5, 2), (60, 4)])
+def test_rows_of_zeros_in_an_8_bit_cache(rt, scratch, rows, q_heads):
+    """Their scale is 0: all of the cache, its first positions, its last ones."""
+    vm = package()
+    for zeros in (slice(0, None), slice(0, 40), slice(90, None)):
+        p = Paged(rt, [rows], [100], dtype="e4m3", heads=2, q_heads=q_heads, dim=64, page=16, seed=9)
+        pos = torch.arange(100 + rows, device="cuda")[zeros]
+        for i in range(2):
+            p.pages[i].view(torch.uint8)[p.table[0, pos // 16].long(), pos % 16] = 0
+            p.scales[i][p.table[0, pos // 16].long(), pos % 16] = 0.0
+        q = normal((rows, q_heads, 64), "bf16", 8, 2.0)
+        o = torch.empty_like(q)
+        p.cache.Attend(p.batch, vm.Rows.Of(q), vm.Rows.Of(o), scratch, stream=_stream())
+        want, _, tol = p.attend(q, 0.125)
+        assert bool(((o.double() - want).abs() <= tol + half_step("bf16") * want.abs()).all())
+
+
 def test_batches_without_rows(rt, scratch):
     vm = package()
     p = Paged(rt, [0, 0], [5, 0], pad=3)
