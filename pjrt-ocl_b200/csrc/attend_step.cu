@@ -24,7 +24,7 @@
 namespace b2 {
 namespace {
 
-constexpr uint32_t kStepWarps = 12, kStepThreads = kStepWarps * 32, kStages = 2;
+constexpr uint32_t kStepWarps = 6, kStepThreads = kStepWarps * 32, kStages = 2, kStepPerSm = 2;
 constexpr float kPScale = 64.0f;         // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
 constexpr float kGrow = 8.0f;            // log2 of the growth of a row maximum that moves it
 constexpr uint32_t kItemTiles = 8;       // what an item costs beside its tiles, in tiles
@@ -90,7 +90,7 @@ struct Walk {
 
 // NR: groups of 8 rows.
 template <bool BF, bool Q8, int HD, int NR>
-__global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const __grid_constant__ AttendArgs a) {
   using Sh = StepShape<Q8, HD>;
   constexpr int KT = Sh::KT, CH = Sh::CH, MT = KT / 16;
   constexpr uint32_t kPitch = NR == 1 ? HD + 4 : HD;          // of a result's rows in a stage
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) b2_attend_step(const __grid_c
 
 template <bool BF, bool Q8, int HD, int NR>
 int Launch(const AttendArgs &a, uint32_t sms, cudaStream_t stream) {
-  b2_attend_step<BF, Q8, HD, NR><<<sms, kStepThreads, StepShape<Q8, HD>::kSmem, stream>>>(a);
+  b2_attend_step<BF, Q8, HD, NR><<<sms * kStepPerSm, kStepThreads, StepShape<Q8, HD>::kSmem, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 template <bool BF, bool Q8, int HD, int NR>
@@ -652,7 +652,7 @@ int PrepareAttendStep() {
     if (e != cudaSuccess) return static_cast<int>(e);
   return 0;
 }
-size_t AttendStepPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * 2u * 16u * (128u + 2u) * sizeof(float); }
+size_t AttendStepPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * kStepPerSm * 2u * 16u * (128u + 2u) * sizeof(float); }
 
 int LaunchAttendStep(const AttendArgs &a, uint32_t sms, CUstream_st *stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
