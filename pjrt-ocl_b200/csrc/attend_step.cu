@@ -27,7 +27,7 @@ namespace {
 constexpr uint32_t kStepWarps = 6, kStepThreads = kStepWarps * 32, kStages = 2, kStepPerSm = 2;
 constexpr float kPScale = 64.0f;         // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
 constexpr float kGrow = 8.0f;            // log2 of the growth of a row maximum that moves it
-constexpr uint32_t kItemTiles = 8;       // what an item costs beside its tiles, in tiles
+constexpr uint32_t kItemTiles = 10;      // what an item costs beside its tiles, in tiles
 
 template <bool Q8, int HD>
 struct StepShape {
@@ -61,7 +61,7 @@ struct StepShared {
   float m[kStepWarps][16], l[kStepWarps][16];
   unsigned long long sum[2][kStepWarps], find[kStepWarps + 2];
   uint32_t at[kStepWarps];         // the stage each warp left its result in
-  uint32_t last, redo[2];          // redo by turns: an item's rows to be worked out again
+  uint32_t redo[2];                // by turns: an item's rows to be worked out again
 };
 
 // An item: cache head h of sequence b, `nt` tiles of keys from `lo`.
@@ -108,23 +108,34 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
     items = x.nt ? a.c.heads : 0u;
     return x.nt ? static_cast<unsigned long long>(x.nt + kItemTiles) * a.c.heads : 0ull;
   };
-  unsigned long long mine = 0, many = 0, first_units = 0;
-  for (uint32_t i = tid; i < a.b.n_seqs; i += kStepThreads) {
-    uint32_t items;
-    const unsigned long long u = units_of(i, items);
-    if (i == tid) first_units = u;
-    mine += u;
-    many += items;
+  // Up to 128 sequences: every warp looks at all of them, four to a lane, and waits for no other. More: the CTA together.
+  const bool few = a.b.n_seqs <= 128u;
+  unsigned long long mine = 0, many = 0, u4[4] = {0, 0, 0, 0};
+  if (few) {
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; ++k) {
+      uint32_t items = 0;
+      if (lane * 4u + k < a.b.n_seqs) u4[k] = units_of(lane * 4u + k, items);
+      mine += u4[k];
+      many += items;
+    }
+  } else {
+    for (uint32_t i = tid; i < a.b.n_seqs; i += kStepThreads) {
+      uint32_t items;
+      mine += units_of(i, items);
+      many += items;
+    }
   }
   auto add = [](unsigned long long x, unsigned long long y) { return x + y; };
-  mine = warp_reduce(mine, add);
-  many = warp_reduce(many, add);
-  if (lane == 0u) { S.sum[0][w] = mine; S.sum[1][w] = many; }
+  unsigned long long U = warp_reduce(mine, add), items = warp_reduce(many, add);
   if (tid == 0u) S.redo[0] = 0u;
-  __syncthreads();
-  unsigned long long U = 0, items = 0;
+  if (!few) {
+    if (lane == 0u) { S.sum[0][w] = U; S.sum[1][w] = items; }
+    __syncthreads();
+    U = items = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < kStepWarps; ++i) { U += S.sum[0][i]; items += S.sum[1][i]; }
+    for (uint32_t i = 0; i < kStepWarps; ++i) { U += S.sum[0][i]; items += S.sum[1][i]; }
+  }
   if (U == 0ull) return;
   // As many CTAs as give each warp a tile; but items of up to four tiles for each of a CTA's warps are not split for that (300 keys, 8 heads:
   // joining two or three CTAs' results takes longer than another round of tiles).
@@ -136,8 +147,25 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
   const unsigned long long u0 = U * blockIdx.x / G, u1 = U * (blockIdx.x + 1ull) / G;
   Walk<KT> cw;                                            // the item being worked on
   unsigned long long x0;                                  // its place: kItemTiles units, then its tiles
-  uint32_t ignored;
-  if (!find_unit<kStepThreads>(a.b.n_seqs, u0, S.find, [&](uint32_t i) { return a.b.n_seqs <= kStepThreads ? first_units : units_of(i, ignored); }, cw.b, x0)) return;
+  if (few) {
+    unsigned long long x = mine;
+#pragma unroll
+    for (uint32_t o = 1; o < 32u; o <<= 1) {
+      const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const uint32_t from = __ffs(__ballot_sync(0xffffffffu, x > u0)) - 1u;     // the lane that has it
+    x -= mine;
+    uint32_t k = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 3u; ++i)
+      if (k == i && x + u4[i] <= u0) { x += u4[i]; ++k; }
+    x0 = __shfl_sync(0xffffffffu, x, from);
+    cw.b = __shfl_sync(0xffffffffu, lane * 4u + k, from);
+  } else {
+    uint32_t ignored;
+    if (!find_unit<kStepThreads>(a.b.n_seqs, u0, S.find, [&](uint32_t i) { return units_of(i, ignored); }, cw.b, x0)) return;
+  }
   cw.load(a, cap);
   const uint32_t per = cw.nt + kItemTiles;
   cw.h = static_cast<uint32_t>((u0 - x0) / per);
@@ -526,8 +554,10 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
       S.l[w][lane] = 0.0f;
     }
     if (lane == 0u) S.at[w] = (w * kStages + issued % kStages) * Sh::kStage;
-    cp_async_commit();
-    cp_async_wait_all();                                  // the next item's q
+    if (!any) {                                           // the next item's q is there (a tile's wait came after it)
+      cp_async_commit();
+      cp_async_wait_all();
+    }
     __syncthreads();
     if (tid == 0u) S.redo[(turn + 1u) & 1u] = 0u;         // the next item's (everybody is done with the one before)
     const bool whole = t_begin == 0u && t_end == cw.nt;
@@ -572,21 +602,25 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
         if (d == 0u) { part[16u * HD + r] = mm; part[16u * HD + 16u + r] = ll; }
       }
     }
-    if (!whole) {
-      // the item's CTAs: those whose runs hold its first and its last tile, and all between
+    __syncthreads();                                      // the stages may be filled again
+    bool joined = whole;
+    if (!whole && w == turn % kStepWarps) {
+      // One warp goes on with it, the others with the next item. The item's CTAs: those whose runs hold its first and its last tile, and
+      // all between.
       const unsigned long long t0 = x0 + kItemTiles, t1 = t0 + cw.nt;
       const uint32_t c0 = static_cast<uint32_t>(((t0 + 1ull) * G - 1ull) / U), c1 = static_cast<uint32_t>((t1 * G - 1ull) / U);
-      __threadfence();
-      __syncthreads();
-      if (tid == 0u) {
-        const uint32_t old = atomicAdd(a.arrived + c0, 1u);
-        S.last = old == c1 - c0 ? 1u : 0u;
-        if (S.last) a.arrived[c0] = 0u;                   // at rest again: nobody else comes
-      }
-      __syncthreads();
-      if (S.last) {
+      uint32_t last = 0u;
+      if (lane == 0u) {
         __threadfence();
-        for (uint32_t i = tid; i < rows * (HD / 4); i += kStepThreads) {
+        last = atomicAdd(a.arrived + c0, 1u) == c1 - c0 ? 1u : 0u;
+        if (last) a.arrived[c0] = 0u;                     // at rest again: nobody else comes
+        __threadfence();
+      }
+      last = __shfl_sync(0xffffffffu, last, 0);
+      __syncwarp();
+      if (last) {
+        joined = true;
+        for (uint32_t i = lane; i < rows * (HD / 4); i += 32u) {
           const uint32_t r = i / (HD / 4), d = (i - r * (HD / 4)) * 4u;
           float mm = -INFINITY, ll = 0.0f;
           auto of = [&](uint32_t c) { return a.part + (static_cast<size_t>(c) * 2u + (c == c0 ? 1u : 0u)) * kPart; };
@@ -604,12 +638,12 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
           }
           finish(r, d, x, mm, ll);
         }
+        __syncwarp();
       }
     }
-    __syncthreads();                                      // the stages may be filled again
-    const uint32_t redo = S.redo[turn & 1u];
-    if (redo && (whole || S.last)) {
-      for (uint32_t r = w; r < rows; r += kStepWarps)
+    const uint32_t redo = joined ? *reinterpret_cast<volatile uint32_t *>(&S.redo[turn & 1u]) : 0u;
+    if (redo) {
+      for (uint32_t r = whole ? w : 0u; r < rows; r += whole ? kStepWarps : 1u)
         if ((redo >> r) & 1u) attend_row_alone(a, cw.b, cw.s, static_cast<int32_t>(r / a.group), cw.h * a.group + r % a.group);
     }
     if (!more) break;
