@@ -17,8 +17,8 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2_f16x2(uint32_t lo16) {
   return r;
 }
 
-// A power of two above x >= 0, within what 2^14 over it and its own inverse allow.
-__device__ __forceinline__ float power_above(float x) { return __uint_as_float(min(250u, max(20u, (__float_as_uint(x) >> 23) + 1u)) << 23); }
+// A power of two above a scale, from 2^-80 (below which a value's last bits, then the value, are lost) to 2^104 (above which its product overflows).
+__device__ __forceinline__ float power_above(float x) { return __uint_as_float(min(231u, max(47u, (__float_as_uint(x) >> 23) + 1u)) << 23); }
 
 // A value of the rows' type (16 bits) as f32.
 __device__ __forceinline__ float row_value(const uint8_t *p, bool bf16) {

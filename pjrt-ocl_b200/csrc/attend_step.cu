@@ -24,20 +24,22 @@
 namespace b2 {
 namespace {
 
-constexpr uint32_t kStepWarps = 6, kStepThreads = kStepWarps * 32, kStages = 2, kStepPerSm = 2;
-constexpr float kPScale = 64.0f;         // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
+constexpr uint32_t kStages = 2;
+// CTAs to an SM: of three warps four, so that one's joins lie under the others' loads.
+constexpr uint32_t PerSm(int warps) { return warps == 3 ? 4u : 1u; }
+constexpr float kPHead = 6.0f;           // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
 constexpr float kGrow = 8.0f;            // log2 of the growth of a row maximum that moves it
-constexpr uint32_t kItemTiles = 10;      // what an item costs beside its tiles, in tiles
+constexpr uint32_t kItemTiles = 8;       // what an item costs beside its tiles, in tiles
 
-template <bool Q8, int HD>
+template <bool Q8, int HD, int NR, int NW>
 struct StepShape {
   static constexpr int KT = (Q8 || HD == 64) ? 32 : 16;       // keys of a tile
   static constexpr int CH = HD * (Q8 ? 1 : 2) / 16;           // 16-byte chunks of a row
   static constexpr int kBytes = KT * CH * 16;                 // K (or V) of a tile
   static constexpr int kScales = Q8 ? 2 * KT * 4 : 0;
   static constexpr int kStage = 2 * kBytes + kScales;
-  static constexpr int kRing = static_cast<int>(kStepWarps * kStages) * kStage;
-  static constexpr int kQ = 16 * HD * 2;                      // q of an item
+  static constexpr int kRing = NW * static_cast<int>(kStages) * kStage;
+  static constexpr int kQ = 8 * NR * HD * 2;                    // q of an item
   static constexpr int kSmem = kRing + 2 * kQ;
 };
 // Chunk of a row in shared memory: eight rows of the same chunk lie in different banks.
@@ -57,11 +59,13 @@ __device__ __forceinline__ float lds_f32(uint32_t at) {
   return x;
 }
 
+template <int NW>
 struct StepShared {
+  static constexpr uint32_t kStepWarps = NW;
   float m[kStepWarps][16], l[kStepWarps][16];
   unsigned long long sum[2][kStepWarps], find[kStepWarps + 2];
   uint32_t at[kStepWarps];         // the stage each warp left its result in
-  uint32_t redo[2];                // by turns: an item's rows to be worked out again
+  uint32_t last, redo[2];          // redo by turns: an item's rows to be worked out again
 };
 
 // An item: cache head h of sequence b, `nt` tiles of keys from `lo`.
@@ -88,15 +92,16 @@ struct Walk {
   }
 };
 
-// NR: groups of 8 rows.
-template <bool BF, bool Q8, int HD, int NR>
-__global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const __grid_constant__ AttendArgs a) {
-  using Sh = StepShape<Q8, HD>;
+// NR: groups of 8 rows. NW: warps of a CTA.
+template <bool BF, bool Q8, int HD, int NR, int NW>
+__global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __grid_constant__ AttendArgs a) {
+  using Sh = StepShape<Q8, HD, NR, NW>;
+  constexpr uint32_t kStepWarps = NW, kStepThreads = NW * 32;
   constexpr int KT = Sh::KT, CH = Sh::CH, MT = KT / 16;
   constexpr uint32_t kPitch = NR == 1 ? HD + 4 : HD;          // of a result's rows in a stage
   static_assert(2 * Sh::kBytes >= 8 * NR * static_cast<int>(kPitch) * 4, "a stage holds a warp's result");
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ StepShared S;
+  __shared__ StepShared<NW> S;
   const uint32_t tid = threadIdx.x, w = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u, quad = lane >> 2, t4 = lane & 3u;
   const uint64_t cap = capacity_of(a.c, a.b);
   // ---- how much work there is, and where this CTA's run of it begins ----
@@ -295,7 +300,8 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
     const bool any = w_tile < t_end;
     // this thread's rows (columns of the products): 8 g + 2 t4 + e
     Span sp[NR][2];
-    float sl2[NR][2], m[NR][2], l[NR][2], v_ref[NR][2];   // v_ref, 8-bit pages: power of two not below the scales that the row has seen, 0 = none yet
+    // the maximum in use; the exponent that weights are relative to; 8-bit pages: a power of two above the scales that the row has seen
+    float sl2[NR][2], m[NR][2], ref[NR][2], l[NR][2], v_ref[NR][2];
     uint32_t qf[NR][HD / 16][2];
     float o[NR][HD / 16][4];
     int32_t full_lo = 0, full_hi = 0x7fffffff;            // keys that all rows see
@@ -308,7 +314,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
         for (int e = 0; e < 2; ++e) {
           const uint32_t r = 8u * g + 2u * t4 + e;
           sp[g][e] = r < rows ? SeenBy(cw.s, static_cast<int32_t>(r / a.group), a.causal, a.window) : Span{0, 0};
-          sl2[g][e] = a.scale_log2; m[g][e] = -INFINITY; l[g][e] = 0.0f; v_ref[g][e] = 0.0f;
+          sl2[g][e] = a.scale_log2; m[g][e] = ref[g][e] = -INFINITY; l[g][e] = 0.0f; v_ref[g][e] = power_above(0.0f);
         }
         const uint32_t qb = q_s + (turn & 1u) * Sh::kQ;
         if constexpr (!Q8) {
@@ -395,40 +401,56 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
             }
           }
       }
-      // scores in the log2 domain, keys that the row does not see at -inf; the thread's keys: 16 t + quad, + 8
+      // keys that the row does not see at -inf; the thread's keys: 16 t + quad, + 8
       const bool whole = j0 >= full_lo && j0 + KT <= full_hi;
       float vs[MT][2], top[NR][2], v_top[NR][2];
 #pragma unroll
       for (int g = 0; g < NR; ++g) { top[g][0] = top[g][1] = -INFINITY; v_top[g][0] = v_top[g][1] = 0.0f; }
+      if (Q8) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        float ksc[2] = {1.0f, 1.0f};
-        if (Q8) {
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            ksc[i] = lds_f32(st + 2u * Sh::kBytes + (t * 16 + i * 8 + quad) * 4u);
+            const float ksc = lds_f32(st + 2u * Sh::kBytes + (t * 16 + i * 8 + quad) * 4u);
             vs[t][i] = lds_f32(st + 2u * Sh::kBytes + (KT + t * 16 + i * 8 + quad) * 4u);
+#pragma unroll
+            for (int g = 0; g < NR; ++g) { s[g][t][2 * i] *= ksc; s[g][t][2 * i + 1] *= ksc; }
           }
+      }
+      if (whole) {
+        if (Q8) {
+          float x = 0.0f;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) x = fmaxf(x, fmaxf(vs[t][0], vs[t][1]));
+#pragma unroll
+          for (int g = 0; g < NR; ++g) v_top[g][0] = v_top[g][1] = x;
         }
+      } else {
 #pragma unroll
         for (int g = 0; g < NR; ++g)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int32_t j = j0 + t * 16 + static_cast<int32_t>(quad) + 8 * (c >> 1);
-            const int e = c & 1;
-            const bool seen = whole || (j >= sp[g][e].lo && j < sp[g][e].hi);
-            const float x = s[g][t][c] * (Q8 ? sl2[g][e] * ksc[c >> 1] : sl2[g][e]);
-            s[g][t][c] = seen ? x : -INFINITY;
-            // (a NaN is dropped here; the sum of the weights finds it)
-            top[g][e] = fmaxf(top[g][e], s[g][t][c]);
-            if (Q8) v_top[g][e] = fmaxf(v_top[g][e], seen ? vs[t][c >> 1] : 0.0f);
-          }
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int32_t j = j0 + t * 16 + static_cast<int32_t>(quad) + 8 * (c >> 1);
+              const int e = c & 1;
+              const bool seen = j >= sp[g][e].lo && j < sp[g][e].hi;
+              s[g][t][c] = seen ? s[g][t][c] : -INFINITY;
+              if (Q8) v_top[g][e] = fmaxf(v_top[g][e], seen ? vs[t][c >> 1] : 0.0f);
+            }
       }
+      // (a NaN is dropped here; the sum of the weights finds it)
       bool grow = false;
 #pragma unroll
-      for (int g = 0; g < NR; ++g)
+      for (int g = 0; g < NR; ++g) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) grow = grow || top[g][e] > m[g][e] + kGrow || (Q8 && v_top[g][e] >= v_ref[g][e] && v_top[g][e] > 0.0f);
+        for (int t = 0; t < MT; ++t) {
+          top[g][0] = max3(top[g][0], s[g][t][0], s[g][t][2]);
+          top[g][1] = max3(top[g][1], s[g][t][1], s[g][t][3]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) grow = grow || top[g][e] * sl2[g][e] > m[g][e] + kGrow || (Q8 && v_top[g][e] >= v_ref[g][e]);
+      }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int g = 0; g < NR; ++g) {
@@ -438,22 +460,19 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
             float x = top[g][e];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            corr[e] = 1.0f;
-            if (x > m[g][e] + kGrow) {
-              corr[e] = m[g][e] == -INFINITY ? 0.0f : fast_ex2(m[g][e] - x);
-              l[g][e] *= corr[e];
-              m[g][e] = x;
-            }
+            x *= sl2[g][e];
+            if (x > m[g][e] + kGrow) m[g][e] = x;
             if (Q8) {
               float v = v_top[g][e];
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-              const float ref = power_above(v);
-              if (ref > v_ref[g][e]) {
-                corr[e] *= v_ref[g][e] / ref;             // (a power of two, or 0 at first)
-                v_ref[g][e] = ref;
-              }
+              v_ref[g][e] = fmaxf(v_ref[g][e], power_above(v));
             }
+            // p = 2^(s - ref); 8-bit pages: 2^6 / v_ref times as large, so that p times a value's scale is what f16 holds best
+            const float r = m[g][e] == -INFINITY ? -INFINITY : Q8 ? m[g][e] - kPHead + static_cast<float>(static_cast<int>(__float_as_uint(v_ref[g][e]) >> 23) - 127) : m[g][e];
+            corr[e] = r == ref[g][e] ? 1.0f : ref[g][e] == -INFINITY ? 0.0f : fast_ex2(ref[g][e] - r);
+            ref[g][e] = r;
+            l[g][e] *= corr[e];
           }
 #pragma unroll
           for (int i = 0; i < HD / 16; ++i) { o[g][i][0] *= corr[0]; o[g][i][1] *= corr[1]; o[g][i][2] *= corr[0]; o[g][i][3] *= corr[1]; }
@@ -462,21 +481,19 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
       uint32_t pb[NR][MT][2], pl[NR][MT][2];
 #pragma unroll
       for (int g = 0; g < NR; ++g) {
-        float neg[2], mul[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          neg[e] = m[g][e] == -INFINITY ? 0.0f : -m[g][e];
-          // kPScale / v_ref of a power of two: by its exponent
-          mul[e] = Q8 && v_ref[g][e] > 0.0f ? __uint_as_float(__float_as_uint(kPScale) + (127u << 23) - __float_as_uint(v_ref[g][e])) : 0.0f;
-        }
+        const float neg[2] = {ref[g][0] == -INFINITY ? 0.0f : -ref[g][0], ref[g][1] == -INFINITY ? 0.0f : -ref[g][1]};
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int e = c & 1;
-            const float p = fast_ex2(s[g][t][c] + neg[e]);
+            const float p = fast_ex2(fmaf(s[g][t][c], sl2[g][e], neg[e]));
             l[g][e] += p;
-            s[g][t][c] = Q8 ? (p == 0.0f ? 0.0f : p * (vs[t][c >> 1] * mul[e])) : p;
+            s[g][t][c] = p;
+          }
+          if (Q8) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[g][t][c] = !whole && s[g][t][c] == 0.0f ? 0.0f : s[g][t][c] * vs[t][c >> 1];     // (a scale that the row does not see may be anything)
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -534,12 +551,11 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
           const uint32_t r = 8u * g + 2u * t4 + e;
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) l[g][e] += __shfl_xor_sync(0xffffffffu, l[g][e], d);
-          if (quad == 0u) { S.m[w][r] = m[g][e]; S.l[w][r] = l[g][e]; }
-          const float mul = Q8 ? v_ref[g][e] * (1.0f / kPScale) : 1.0f;
+          if (quad == 0u) { S.m[w][r] = ref[g][e]; S.l[w][r] = l[g][e]; }
           if (r < rows) {
 #pragma unroll
             for (int n = 0; n < HD / 16; ++n) {
-              const float lo = o[g][n][e] * mul, hi = o[g][n][2 + e] * mul;
+              const float lo = o[g][n][e], hi = o[g][n][2 + e];
               if (Q8) {
                 *reinterpret_cast<float2 *>(slot + r * kPitch + n * 16 + 2u * quad) = make_float2(lo, hi);
               } else {
@@ -604,30 +620,37 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
     }
     __syncthreads();                                      // the stages may be filled again
     bool joined = whole;
-    if (!whole && w == turn % kStepWarps) {
-      // One warp goes on with it, the others with the next item. The item's CTAs: those whose runs hold its first and its last tile, and
-      // all between.
-      const unsigned long long t0 = x0 + kItemTiles, t1 = t0 + cw.nt;
-      const uint32_t c0 = static_cast<uint32_t>(((t0 + 1ull) * G - 1ull) / U), c1 = static_cast<uint32_t>((t1 * G - 1ull) / U);
+    // A part of an item. Its CTAs: those whose runs hold its first and its last tile, and all between. One warp goes on with it, the others with
+    // the next item; but of many parts all warps join what the last CTA finds.
+    const unsigned long long t0 = x0 + kItemTiles, t1 = t0 + cw.nt;
+    const uint32_t c0 = whole ? 0u : static_cast<uint32_t>(((t0 + 1ull) * G - 1ull) / U), c1 = whole ? 0u : static_cast<uint32_t>((t1 * G - 1ull) / U);
+    const bool together = c1 - c0 >= 4u;
+    if (!whole && (together || w == turn % kStepWarps)) {
       uint32_t last = 0u;
-      if (lane == 0u) {
+      if (together ? tid == 0u : lane == 0u) {
         __threadfence();
         last = atomicAdd(a.arrived + c0, 1u) == c1 - c0 ? 1u : 0u;
         if (last) a.arrived[c0] = 0u;                     // at rest again: nobody else comes
         __threadfence();
       }
-      last = __shfl_sync(0xffffffffu, last, 0);
-      __syncwarp();
+      if (together) {
+        if (tid == 0u) S.last = last;
+        __syncthreads();
+        last = S.last;
+      } else {
+        last = __shfl_sync(0xffffffffu, last, 0);
+        __syncwarp();
+      }
       if (last) {
         joined = true;
-        for (uint32_t i = lane; i < rows * (HD / 4); i += 32u) {
+        for (uint32_t i = together ? tid : lane; i < rows * (HD / 4); i += together ? kStepThreads : 32u) {
           const uint32_t r = i / (HD / 4), d = (i - r * (HD / 4)) * 4u;
           float mm = -INFINITY, ll = 0.0f;
           auto of = [&](uint32_t c) { return a.part + (static_cast<size_t>(c) * 2u + (c == c0 ? 1u : 0u)) * kPart; };
-#pragma unroll 4
+#pragma unroll 8
           for (uint32_t c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(of(c) + 16u * HD + r));
           float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
           for (uint32_t c = c0; c <= c1; ++c) {
             const float *p = of(c);
             const float mc = __ldcg(p + 16u * HD + r), lc = __ldcg(p + 16u * HD + 16u + r);
@@ -638,12 +661,14 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
           }
           finish(r, d, x, mm, ll);
         }
-        __syncwarp();
+        if (together) __syncthreads();
+        else __syncwarp();
       }
     }
     const uint32_t redo = joined ? *reinterpret_cast<volatile uint32_t *>(&S.redo[turn & 1u]) : 0u;
     if (redo) {
-      for (uint32_t r = whole ? w : 0u; r < rows; r += whole ? kStepWarps : 1u)
+      const bool all = whole || together;                 // (else one warp is here)
+      for (uint32_t r = all ? w : 0u; r < rows; r += all ? kStepWarps : 1u)
         if ((redo >> r) & 1u) attend_row_alone(a, cw.b, cw.s, static_cast<int32_t>(r / a.group), cw.h * a.group + r % a.group);
     }
     if (!more) break;
@@ -657,26 +682,31 @@ __global__ void __launch_bounds__(kStepThreads, kStepPerSm) b2_attend_step(const
   cp_async_wait_all();
 }
 
-template <bool BF, bool Q8, int HD, int NR>
+template <bool BF, bool Q8, int HD, int NR, int NW>
 int Launch(const AttendArgs &a, uint32_t sms, cudaStream_t stream) {
-  b2_attend_step<BF, Q8, HD, NR><<<sms * kStepPerSm, kStepThreads, StepShape<Q8, HD>::kSmem, stream>>>(a);
+  b2_attend_step<BF, Q8, HD, NR, NW><<<sms * PerSm(NW), NW * 32, StepShape<Q8, HD, NR, NW>::kSmem, stream>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
-template <bool BF, bool Q8, int HD, int NR>
+template <bool BF, bool Q8, int HD, int NR, int NW>
 cudaError_t Attr() {
-  return cudaFuncSetAttribute(b2_attend_step<BF, Q8, HD, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, StepShape<Q8, HD>::kSmem);
+  return cudaFuncSetAttribute(b2_attend_step<BF, Q8, HD, NR, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, StepShape<Q8, HD, NR, NW>::kSmem);
 }
+// 9 to 16 rows: CTAs of eight warps, whose threads may have 255 registers (with twelve warps and 168, 500 bytes of them were spilled: 32 sequences of 4000 to 8000 tokens, 16 heads to each of 4 cache heads, 8-bit pages: 81 us, 111 so).
+// Up to 8 rows: items (sequences x cache heads) for no more than the SMs go to CTAs of twelve warps, of which few share an item (8 heads of 131000 keys,
+// bf16: 90 us, 137 with CTAs of three); more items to CTAs of three, which lose less at an item's end (64 sequences of 200 to 16000 tokens, 8 heads, 8-bit
+// pages: 110 us, 120 with CTAs of six).
+template <bool BF, bool Q8, int HD>
+int Choose(const AttendArgs &a, uint32_t sms, cudaStream_t s) {
+  if (a.b.max_rows * a.group > 8u) return Launch<BF, Q8, HD, 2, 8>(a, sms, s);
+  return static_cast<uint64_t>(a.b.n_seqs) * a.c.heads <= sms ? Launch<BF, Q8, HD, 1, 12>(a, sms, s) : Launch<BF, Q8, HD, 1, 3>(a, sms, s);
+}
+template <bool BF, bool Q8>
+int Dim(const AttendArgs &a, uint32_t sms, cudaStream_t s) { return a.c.hd > 64u ? Choose<BF, Q8, 128>(a, sms, s) : Choose<BF, Q8, 64>(a, sms, s); }
 template <bool BF, bool Q8>
 cudaError_t Attrs() {
-  for (cudaError_t e : {Attr<BF, Q8, 64, 1>(), Attr<BF, Q8, 64, 2>(), Attr<BF, Q8, 128, 1>(), Attr<BF, Q8, 128, 2>()})
+  for (cudaError_t e : {Attr<BF, Q8, 64, 2, 8>(), Attr<BF, Q8, 64, 1, 12>(), Attr<BF, Q8, 64, 1, 3>(), Attr<BF, Q8, 128, 2, 8>(), Attr<BF, Q8, 128, 1, 12>(), Attr<BF, Q8, 128, 1, 3>()})
     if (e != cudaSuccess) return e;
   return cudaSuccess;
-}
-template <bool BF, bool Q8>
-int Choose(const AttendArgs &a, uint32_t sms, cudaStream_t s) {
-  const bool wide = a.b.max_rows * a.group > 8u;
-  if (a.c.hd > 64u) return wide ? Launch<BF, Q8, 128, 2>(a, sms, s) : Launch<BF, Q8, 128, 1>(a, sms, s);
-  return wide ? Launch<BF, Q8, 64, 2>(a, sms, s) : Launch<BF, Q8, 64, 1>(a, sms, s);
 }
 
 }  // namespace
@@ -686,12 +716,12 @@ int PrepareAttendStep() {
     if (e != cudaSuccess) return static_cast<int>(e);
   return 0;
 }
-size_t AttendStepPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * kStepPerSm * 2u * 16u * (128u + 2u) * sizeof(float); }
+size_t AttendStepPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * PerSm(3) * 2u * 16u * (128u + 2u) * sizeof(float); }
 
 int LaunchAttendStep(const AttendArgs &a, uint32_t sms, CUstream_st *stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (a.e4m3) return a.bf16 ? Choose<true, true>(a, sms, s) : Choose<false, true>(a, sms, s);
-  return a.bf16 ? Choose<true, false>(a, sms, s) : Choose<false, false>(a, sms, s);
+  if (a.e4m3) return a.bf16 ? Dim<true, true>(a, sms, s) : Dim<false, true>(a, sms, s);
+  return a.bf16 ? Dim<true, false>(a, sms, s) : Dim<false, false>(a, sms, s);
 }
 
 }  // namespace b2
