@@ -5,11 +5,12 @@
 //   dx = r h - x r^3 / hd sum(h x),   dw = sum over rows and heads of g x r.
 //
 // Bound: HBM. Every row is read once and written once (backward: x and dy read, dx written).
-// A CTA takes some tokens at a time; the angles of its tokens are worked out once, in 64-bit turns (position x turns, less
-// the nearest whole number: exact for every int32 position; sine and cosine of the rest in f32), and shared by all heads. A row
-// belongs to up to 32 threads; a thread holds V pairs of it, both halves of each, so that neither layout needs an exchange
+// A warp takes a token (few tokens: a part of its heads). It works out the token's angles once, in 64-bit turns (position x turns, less the
+// nearest whole number: exact for every int32 position; sine and cosine of the rest in f32), and keeps those of its pairs in registers for all
+// heads. A row belongs to up to 32 threads; a thread holds V pairs of it, both halves of each, so that neither layout needs an exchange
 // between threads: the half layout is two V-wide accesses rot/2 apart, the neighbouring one two that touch. What lies behind
-// rot is treated the same with no angle. V is as wide as the addresses, strides and rot allow up to 16 bytes.
+// rot is treated the same with no angle. V is as wide as the addresses, strides and rot allow up to 16 bytes. The next rows are on the
+// way while a row is worked on. No barrier stands between tokens.
 // Gradients of the weights stay in registers, are joined in shared memory once a CTA, and a second small launch adds the CTAs'
 // sums in their order, so that a result does not change from call to call.
 #include "operators_dev.cuh"
@@ -18,11 +19,10 @@ namespace b2 {
 namespace {
 
 constexpr int kRopeThreads = 256, kRopeWarps = kRopeThreads / 32;
-constexpr uint32_t kRopeTokens = 8;           // most tokens of a CTA at a time
 constexpr uint32_t kRopeBackPerSm = 2;
 
 struct RopeShape {
-  uint32_t tokens;        // of a CTA at a time
+  uint32_t split;         // warps to a token
   uint32_t lanes;         // threads to a row, a power of two
   uint32_t units;         // V-pair units of a row
   uint32_t rot_units;     // of these turned
@@ -58,12 +58,41 @@ __device__ __forceinline__ void turn(float (&y)[2 * V], const float2 (&cs)[V], b
     }
   }
 }
+// The two accesses of a unit as they come: V values each, in 32-bit words (one value of 16 bits: in the low half).
+template <typename T, int V> struct Raw {
+  static constexpr int W = V * sizeof(T) >= 4 ? V * static_cast<int>(sizeof(T)) / 4 : 1;
+  uint32_t a[W], b[W];
+};
+template <int BYTES>
+__device__ __forceinline__ void load_words(const void *p, uint32_t *w) {
+  if constexpr (BYTES == 16) {
+    const uint4 v = *static_cast<const uint4 *>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = *static_cast<const uint2 *>(p);
+    w[0] = v.x; w[1] = v.y;
+  } else if constexpr (BYTES == 4) {
+    w[0] = *static_cast<const uint32_t *>(p);
+  } else {
+    w[0] = *static_cast<const uint16_t *>(p);
+  }
+}
 template <typename T, int V>
-__device__ __forceinline__ void load_unit(const RowsRef &r, uint32_t tok, uint32_t head, uint32_t e0, uint32_t e1, float (&x)[2 * V]) {
+__device__ __forceinline__ void load_unit(const RowsRef &r, uint32_t tok, uint32_t head, uint32_t e0, uint32_t e1, Raw<T, V> &x) {
   const T *p = reinterpret_cast<const T *>(r.p) + static_cast<int64_t>(tok) * r.row + static_cast<int64_t>(head) * r.head;
-  const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(p + e0), b = *reinterpret_cast<const Vec<T, V> *>(p + e1);
+  load_words<V * sizeof(T)>(p + e0, x.a);
+  load_words<V * sizeof(T)>(p + e1, x.b);
+}
+template <typename T> __device__ __forceinline__ float value_of(const uint32_t *w, int i);
+template <> __device__ __forceinline__ float value_of<float>(const uint32_t *w, int i) { return __uint_as_float(w[i]); }
+template <> __device__ __forceinline__ float value_of<__nv_bfloat16>(const uint32_t *w, int i) { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+template <> __device__ __forceinline__ float value_of<__half>(const uint32_t *w, int i) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu)));
+}
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Raw<T, V> &r, float (&x)[2 * V]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) { x[i] = ToF(a.v[i]); x[V + i] = ToF(b.v[i]); }
+  for (int i = 0; i < V; ++i) { x[i] = value_of<T>(r.a, i); x[V + i] = value_of<T>(r.b, i); }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_unit(const RowsRef &r, uint32_t tok, uint32_t head, uint32_t e0, uint32_t e1, const float (&x)[2 * V]) {
@@ -81,18 +110,19 @@ __device__ __forceinline__ float row_sum(float v, uint32_t lanes) {
 
 // U: units of a row that a thread may have (rows of more than 32 units).
 template <typename T, int V, int U, bool BACK>
-__global__ void __launch_bounds__(kRopeThreads) b2_rope(const __grid_constant__ RopeArgs a, const __grid_constant__ RopeShape s) {
-  extern __shared__ __align__(16) uint8_t sm[];
-  float *w_s = reinterpret_cast<float *>(sm);                                 // [2][hd]
-  float2 *cs_s = reinterpret_cast<float2 *>(w_s + 2u * a.hd);                 // [tokens][rot / 2]
+__global__ void __launch_bounds__(kRopeThreads, BACK ? kRopeBackPerSm : 3) b2_rope(const __grid_constant__ RopeArgs a, const __grid_constant__ RopeShape s) {
+  extern __shared__ __align__(16) uint8_t sm[];           // weights [2][hd], then the warps' angles [warps][rot / 2]
+  float *w_s = reinterpret_cast<float *>(sm);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, half = a.rot / 2u;
-  const uint32_t rows_per_warp = 32u / s.lanes, slot = lane / s.lanes, sub = lane & (s.lanes - 1u);
+  float2 *cs_s = reinterpret_cast<float2 *>(w_s + 2u * a.hd) + warp * half;
+  const uint32_t at_once = 32u / s.lanes, slot = lane / s.lanes, sub = lane & (s.lanes - 1u);
   if (a.norm) {
     for (uint32_t i = tid; i < 2u * a.hd; i += kRopeThreads) {
       const uint32_t t = i >= a.hd ? 1u : 0u, e = i - t * a.hd;
       const void *w = a.w[t];
       w_s[i] = !w ? 1.0f : a.weight_f32 ? static_cast<const float *>(w)[e] : ToF(static_cast<const T *>(w)[e]);
     }
+    __syncthreads();
   }
   uint32_t e0[U], e1[U];
   bool has[U];
@@ -111,97 +141,110 @@ __global__ void __launch_bounds__(kRopeThreads) b2_rope(const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < 2 * V; ++i) acc[t][k][i] = 0.0f;
   }
-  const uint32_t groups[2] = {(a.heads[0] + rows_per_warp - 1u) / rows_per_warp, (a.heads[1] + rows_per_warp - 1u) / rows_per_warp};
-  const uint32_t per_token = groups[0] + groups[1];
   const float inv_hd = 1.0f / static_cast<float>(a.hd);
   const bool inter = a.interleaved != 0u;
-  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * s.tokens; base < a.n_rows; base += static_cast<uint64_t>(gridDim.x) * s.tokens) {
-    // (min(s.tokens, a.n_rows - tok0) came out as s.tokens for the last, shorter run: the compiler of CUDA 12.9 with this loop around it)
-    const uint32_t tok0 = static_cast<uint32_t>(base), n_tok = min(tok0 + s.tokens, a.n_rows) - tok0;
-    __syncthreads();                                      // the angles before have been used
-    for (uint32_t i = tid; i < n_tok * half; i += kRopeThreads) {
-      const uint32_t tk = i / half, f = i - tk * half;
-      double t = static_cast<double>(a.pos[tok0 + tk]) * a.turns[f];
-      t -= rint(t);
-      float sn, cn;
-      sincospif(2.0f * static_cast<float>(t), &sn, &cn);
-      cs_s[i] = make_float2(cn * a.magnitude, sn * a.magnitude);
-    }
-    __syncthreads();
-    for (uint32_t task = warp; task < n_tok * per_token; task += kRopeWarps) {
-      const uint32_t tk = task / per_token, g = task - tk * per_token, t = g >= groups[0] ? 1u : 0u;
-      const uint32_t head = (g - (t ? groups[0] : 0u)) * rows_per_warp + slot, tok = tok0 + tk;
-      const bool live = head < a.heads[t];
-      float x[U][2 * V], y[U][2 * V];
+  const uint32_t me = blockIdx.x * kRopeWarps + warp, step = gridDim.x * kRopeWarps / s.split, part = me % s.split;
+  const uint32_t stride = s.split * at_once;              // of the warp's heads
+  for (uint32_t tok = me / s.split; tok < a.n_rows; tok = a.n_rows - tok > step ? tok + step : a.n_rows) {
+    // ---- the angles of the token ----
+    float2 cs[U][V];
+    if (half) {
+      __syncwarp();                                       // (those of the token before are in registers)
+      const double pos = static_cast<double>(a.pos[tok]);
+      for (uint32_t f = lane; f < half; f += 32u) {
+        double t = pos * a.turns[f];
+        t -= rint(t);
+        float sn, cn;
+        sincospif(2.0f * static_cast<float>(t), &sn, &cn);
+        cs_s[f] = make_float2(cn * a.magnitude, sn * a.magnitude);
+      }
+      __syncwarp();
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        if (live && has[k]) {
-          if (!BACK || a.norm) load_unit<T, V>(a.x[t], tok, head, e0[k], e1[k], x[k]);
-          if (BACK) load_unit<T, V>(a.g[t], tok, head, e0[k], e1[k], y[k]);
-        } else {
+        const uint32_t u = sub + static_cast<uint32_t>(k) * s.lanes;
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) { x[k][i] = 0.0f; y[k][i] = 0.0f; }
-        }
+        for (int i = 0; i < V; ++i) cs[k][i] = u < s.rot_units ? cs_s[V * u + i] : make_float2(1.0f, 0.0f);
       }
-      float r = 1.0f;
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < 2u; ++t) {                   // queries, keys
+      const uint32_t heads = a.heads[t], first = part * at_once + slot;
+      float w[U][2 * V];
       if (a.norm) {
-        float ss = 0.0f;
 #pragma unroll
         for (int k = 0; k < U; ++k)
 #pragma unroll
-          for (int i = 0; i < 2 * V; ++i) ss += x[k][i] * x[k][i];
-        const float sum = row_sum(ss, s.lanes);
-        r = live ? 1.0f / sqrtf(sum * inv_hd + a.eps) : 0.0f;      // (no row: adds nothing to the weights' gradients)
+          for (int i = 0; i < V; ++i) { w[k][i] = w_s[t * a.hd + e0[k] + i]; w[k][V + i] = w_s[t * a.hd + e1[k] + i]; }
       }
-      if (!BACK) {
+      Raw<T, V> xr[U], gr[U];
+      auto fetch = [&](uint32_t head) {
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+          if (head < heads && has[k]) {
+            if (!BACK || a.norm) load_unit<T, V>(a.x[t], tok, head, e0[k], e1[k], xr[k]);
+            if (BACK) load_unit<T, V>(a.g[t], tok, head, e0[k], e1[k], gr[k]);
+          }
+      };
+      fetch(first);
+      for (uint32_t head = first; head - slot < heads; head += stride) {
+        const bool live = head < heads;
+        float x[U][2 * V], y[U][2 * V];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-          if (a.norm) {
+          if (live && has[k]) {
+            if (!BACK || a.norm) widen(xr[k], x[k]);
+            if (BACK) widen(gr[k], y[k]);
+          } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) { x[k][i] *= r * w_s[t * a.hd + e0[k] + i]; x[k][V + i] *= r * w_s[t * a.hd + e1[k] + i]; }
-          }
-          const uint32_t u = sub + static_cast<uint32_t>(k) * s.lanes;
-          if (u < s.rot_units) {
-            float2 cs[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) cs[i] = cs_s[tk * half + V * u + i];
-            turn<V>(x[k], cs, inter, 1.0f);
-          }
-          if (live && has[k]) store_unit<T, V>(a.y[t], tok, head, e0[k], e1[k], x[k]);
-        }
-      } else {
-        float hx = 0.0f;
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const uint32_t u = sub + static_cast<uint32_t>(k) * s.lanes;
-          if (u < s.rot_units) {
-            float2 cs[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) cs[i] = cs_s[tk * half + V * u + i];
-            turn<V>(y[k], cs, inter, -1.0f);
-          }
-          if (a.norm) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float g0 = y[k][i] * x[k][i] * r, g1 = y[k][V + i] * x[k][V + i] * r;
-              if (t) { acc[1][k][i] += g0; acc[1][k][V + i] += g1; }
-              else { acc[0][k][i] += g0; acc[0][k][V + i] += g1; }
-              y[k][i] *= w_s[t * a.hd + e0[k] + i];
-              y[k][V + i] *= w_s[t * a.hd + e1[k] + i];
-              hx += y[k][i] * x[k][i] + y[k][V + i] * x[k][V + i];
-            }
+            for (int i = 0; i < 2 * V; ++i) { x[k][i] = 0.0f; y[k][i] = 0.0f; }
           }
         }
+        fetch(head + stride);
+        float r = 1.0f;
         if (a.norm) {
-          const float c = row_sum(hx, s.lanes) * inv_hd * r * r * r;
+          float ss = 0.0f;
 #pragma unroll
           for (int k = 0; k < U; ++k)
 #pragma unroll
-            for (int i = 0; i < 2 * V; ++i) y[k][i] = r * y[k][i] - c * x[k][i];
+            for (int i = 0; i < 2 * V; ++i) ss += x[k][i] * x[k][i];
+          const float sum = row_sum(ss, s.lanes);
+          r = live ? rsqrtf(sum * inv_hd + a.eps) : 0.0f;       // (no row: adds nothing to the weights' gradients)
         }
+        if (!BACK) {
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-          if (live && has[k]) store_unit<T, V>(a.y[t], tok, head, e0[k], e1[k], y[k]);
+          for (int k = 0; k < U; ++k) {
+            if (a.norm) {
+#pragma unroll
+              for (int i = 0; i < 2 * V; ++i) x[k][i] *= r * w[k][i];
+            }
+            if (half) turn<V>(x[k], cs[k], inter, 1.0f);
+            if (live && has[k]) store_unit<T, V>(a.y[t], tok, head, e0[k], e1[k], x[k]);
+          }
+        } else {
+          float hx = 0.0f;
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            if (half) turn<V>(y[k], cs[k], inter, -1.0f);
+            if (a.norm) {
+#pragma unroll
+              for (int i = 0; i < 2 * V; ++i) {
+                acc[t][k][i] += y[k][i] * (x[k][i] * r);
+                y[k][i] *= w[k][i];
+                hx += y[k][i] * x[k][i];
+              }
+            }
+          }
+          if (a.norm) {
+            const float c = row_sum(hx, s.lanes) * inv_hd * r * r * r;
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+              for (int i = 0; i < 2 * V; ++i) y[k][i] = r * y[k][i] - c * x[k][i];
+          }
+#pragma unroll
+          for (int k = 0; k < U; ++k)
+            if (live && has[k]) store_unit<T, V>(a.y[t], tok, head, e0[k], e1[k], y[k]);
+        }
       }
     }
   }
@@ -229,11 +272,12 @@ __global__ void __launch_bounds__(kRopeThreads) b2_rope(const __grid_constant__ 
   }
 }
 
-// The CTAs' sums in their order: 32 columns to a CTA, its warps an eighth of them each.
-__global__ void __launch_bounds__(kRopeThreads) b2_rope_weights(const __grid_constant__ RopeArgs a, uint32_t ctas) {
-  __shared__ float red[kRopeWarps][32];
+// The CTAs' sums in their order: 32 columns to a CTA, its warps a part of them each.
+constexpr uint32_t kSumWarps = 32;
+__global__ void __launch_bounds__(kSumWarps * 32) b2_rope_weights(const __grid_constant__ RopeArgs a, uint32_t ctas) {
+  __shared__ float red[kSumWarps][32];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, cols = 2u * a.hd, c = blockIdx.x * 32u + lane;
-  const uint32_t per = (ctas + kRopeWarps - 1u) / kRopeWarps, b1 = min(ctas, (warp + 1u) * per);
+  const uint32_t per = (ctas + kSumWarps - 1u) / kSumWarps, b1 = min(ctas, (warp + 1u) * per);
   float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (c < cols) {
     const float *p = a.partial + c;
@@ -252,7 +296,7 @@ __global__ void __launch_bounds__(kRopeThreads) b2_rope_weights(const __grid_con
   if (warp == 0u && c < cols) {
     float sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kRopeWarps; ++k) sum += red[k][lane];
+    for (uint32_t k = 0; k < kSumWarps; ++k) sum += red[k][lane];
     const uint32_t t = c >= a.hd ? 1u : 0u;
     if (a.dw[t]) a.dw[t][c - t * a.hd] = sum;
   }
@@ -270,18 +314,18 @@ int Launch(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
   s.units = a.hd / 2u / V;
   s.rot_units = a.rot / 2u / V;
   s.lanes = Pow2AtLeast(s.units) < 32u ? Pow2AtLeast(s.units) : 32u;
-  // Few tokens: one to a CTA, so that all SMs have some (32 rows of a decode step: 32 CTAs). Many: as many as leave four rounds for
-  // each of the CTAs that fit, up to 8, so that the angles and the barriers around them are shared by more rows.
-  const uint32_t rounds = a.n_rows / (sms * 16u);
-  s.tokens = rounds < 1u ? 1u : rounds > kRopeTokens ? kRopeTokens : rounds;
-  uint32_t ctas = (a.n_rows + s.tokens - 1u) / s.tokens;
+  // Few tokens: a CTA's warps share one, as far as it has heads for them.
+  s.split = 1;
+  const uint32_t heads = a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1];
+  while (s.split < static_cast<uint32_t>(kRopeWarps) && static_cast<uint64_t>(a.n_rows) * s.split < sms * 8u && heads * s.lanes > s.split * 32u) s.split *= 2u;
+  const uint64_t want = (static_cast<uint64_t>(a.n_rows) * s.split + kRopeWarps - 1u) / kRopeWarps;
   const uint32_t most = BACK ? kRopeBackPerSm * sms : sms * 8u;
-  ctas = ctas < 1u ? 1u : ctas > most ? most : ctas;
-  size_t smem = sizeof(float) * 2u * a.hd + sizeof(float2) * s.tokens * (a.rot / 2u);
+  const uint32_t ctas = want < 1u ? 1u : want > most ? most : static_cast<uint32_t>(want);
+  size_t smem = sizeof(float) * 2u * a.hd + sizeof(float2) * kRopeWarps * (a.rot / 2u);
   const size_t red = sizeof(float) * 2u * a.hd * kRopeWarps;
   if (BACK && red > smem) smem = red;
   b2_rope<T, V, U, BACK><<<ctas, kRopeThreads, smem, stream>>>(a, s);
-  if (BACK && a.partial) b2_rope_weights<<<(2u * a.hd + 31u) / 32u, kRopeThreads, 0, stream>>>(a, ctas);
+  if (BACK && a.partial) b2_rope_weights<<<(2u * a.hd + 31u) / 32u, kSumWarps * 32u, 0, stream>>>(a, ctas);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -306,7 +350,8 @@ uint32_t Width(const RopeArgs &a, bool backward) {
 template <typename T, bool BACK>
 int Dispatch(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
   const uint32_t v = Width<T>(a, BACK);
-  if constexpr (sizeof(T) == 2) {
+  // (backward: 8-byte accesses; with 16 the sums of the weights' gradients, of queries and of keys, leave too few registers)
+  if constexpr (sizeof(T) == 2 && !BACK) {
     if (v == 8u) return Launch<T, 8, 1, BACK>(a, sms, stream);
   }
   if (v >= 4u) return Launch<T, 4, 1, BACK>(a, sms, stream);
