@@ -7,6 +7,8 @@
 // Bound: HBM, each row read and written once. A warp takes a token (few tokens: a part of its rows): it looks up the token's sequence, 32 starts
 // at a time, and where its position lies, while the rows of the token before are on the way, and moves the 2 x heads rows, 8 values to a
 // thread, four rows of each group of threads in flight. No barrier anywhere.
+#include <type_traits>
+
 #include "operators_dev.cuh"
 
 namespace b2 {
@@ -15,42 +17,78 @@ namespace {
 constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32;
 constexpr int kAtOnce = 4;                                // rows in flight to each group of threads
 
-template <typename R>
-__device__ __forceinline__ void load8(const R *p, bool vec, float (&x)[8]) {
-  if (vec) {
-    constexpr int W = 16 / sizeof(R);
+// Eight values of a row as they come, in words.
+template <typename R, bool VEC>
+__device__ __forceinline__ void load8(const R *p, uint32_t (&w)[2 * sizeof(R)]) {
+  if constexpr (VEC) {
 #pragma unroll
-    for (int j = 0; j < 8 / W; ++j) {
-      const Vec<R, W> a = reinterpret_cast<const Vec<R, W> *>(p)[j];
-#pragma unroll
-      for (int i = 0; i < W; ++i) x[j * W + i] = ToF(a.v[i]);
+    for (int j = 0; j < static_cast<int>(sizeof(R)) / 2; ++j) {
+      const uint4 v = reinterpret_cast<const uint4 *>(p)[j];
+      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
     }
-  } else {
+  } else if constexpr (sizeof(R) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = ToF(p[i]);
+    for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+  } else {
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
+  }
+}
+template <typename R, bool VEC>
+__device__ __forceinline__ void store8(R *p, const uint32_t (&w)[2 * sizeof(R)]) {
+  if constexpr (VEC) {
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(R)) / 2; ++j) reinterpret_cast<uint4 *>(p)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  } else if constexpr (sizeof(R) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+  } else {
+    uint16_t *h = reinterpret_cast<uint16_t *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { h[2 * i] = static_cast<uint16_t>(w[i]); h[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16); }
   }
 }
 template <typename R>
-__device__ __forceinline__ void store8(R *p, bool vec, const float (&x)[8]) {
-  if (vec) {
-    constexpr int W = 16 / sizeof(R);
+__device__ __forceinline__ void widen8(const uint32_t (&w)[2 * sizeof(R)], float (&x)[8]) {
 #pragma unroll
-    for (int j = 0; j < 8 / W; ++j) {
-      Vec<R, W> a;
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(R) == 4) x[i] = __uint_as_float(w[i]);
+    else if constexpr (std::is_same<R, __nv_bfloat16>::value) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    else x[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu)));
+  }
+}
+template <typename R>
+__device__ __forceinline__ void narrow8(const float (&x)[8], uint32_t (&w)[2 * sizeof(R)]) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) a.v[i] = FromF<R>(x[j * W + i]);
-      reinterpret_cast<Vec<R, W> *>(p)[j] = a;
-    }
-  } else {
+  for (int i = 0; i < static_cast<int>(2 * sizeof(R)); ++i) {
+    if constexpr (sizeof(R) == 4) w[i] = __float_as_uint(x[i]);
+    else if constexpr (std::is_same<R, __nv_bfloat16>::value) w[i] = cvt_bf16x2(x[2 * i + 1], x[2 * i]);
+    else w[i] = cvt_f16x2(x[2 * i + 1], x[2 * i]);
+  }
+}
+// The largest magnitude of a row whose eight values each of `lanes` threads have; by bit patterns, so that a NaN is largest.
+template <typename R>
+__device__ __forceinline__ float largest(const uint32_t (&w)[2 * sizeof(R)], uint32_t lanes) {
+  uint32_t m = 0u;
+  if constexpr (sizeof(R) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = FromF<R>(x[i]);
+    for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+    for (uint32_t o = lanes >> 1; o > 0u; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return __uint_as_float(m);
+  } else {                                                // two at a time
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    for (uint32_t o = lanes >> 1; o > 0u; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same<R, __nv_bfloat16>::value) return __uint_as_float(m << 16);
+    else return __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
   }
 }
 
 struct MoveShape {
   uint32_t lanes;                  // threads to a row, a power of two
   uint32_t split;                  // warps to a token
-  uint32_t vec[2];                 // rows of K, V: 16-byte accesses
 };
 
 // Where a row of the batch lies in the cache: byte offset of its place (-1: it has none, -2: the row is nobody's) and of its scales.
@@ -89,11 +127,92 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], float s) {
   return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
-// R: type of the rows, P: of the pages.
-template <typename R, typename P, bool WRITE>
+// One of a token's K and V: rows of `heads` heads from row (a thread's eight values) to page or back.
+template <typename R, typename P, bool WRITE, bool VEC, typename F>
+__device__ __forceinline__ void move_rows(const CacheView &c, const MoveShape &s, R *row, int64_t row_head, uint8_t *page, float *scales, const Place &at, uint32_t first, uint32_t group,
+                                          uint32_t step, uint32_t sub, bool has, F under) {
+  constexpr bool Q8 = sizeof(P) == 1;
+  constexpr int WR = 2 * sizeof(R);
+  row += sub * 8u;
+  page += at.at + sub * 8u * sizeof(P);
+  scales += at.scale;
+  for (uint32_t h0 = first; h0 - group < c.heads; h0 += kAtOnce * step) {
+    uint32_t w[kAtOnce][WR];
+    uint2 code[kAtOnce];
+    float scale[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const uint32_t h = h0 + static_cast<uint32_t>(j) * step;
+      const bool live = h < c.heads && at.at >= 0 && has;
+      code[j] = make_uint2(0u, 0u);
+      scale[j] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WR; ++i) w[j][i] = 0u;
+      if (!live) continue;
+      if constexpr (WRITE) {
+        load8<R, VEC>(row + static_cast<int64_t>(h) * row_head, w[j]);
+      } else if constexpr (Q8) {
+        code[j] = *reinterpret_cast<const uint2 *>(page + h * c.head_bytes);
+        scale[j] = scales[h * c.s_head];
+      } else {
+        uint32_t pw[2 * sizeof(P)];
+        load8<P, true>(reinterpret_cast<const P *>(page + h * c.head_bytes), pw);
+        if constexpr (std::is_same<R, P>::value) {
+#pragma unroll
+          for (int i = 0; i < WR; ++i) w[j][i] = pw[i];
+        } else {
+          float x[8];
+          widen8<P>(pw, x);
+          narrow8<R>(x, w[j]);
+        }
+      }
+    }
+    under(h0 == first);
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const uint32_t h = h0 + static_cast<uint32_t>(j) * step;
+      if constexpr (WRITE) {
+        float x[8];
+        if constexpr (Q8) {
+          const float sc = __fdiv_rn(largest<R>(w[j], s.lanes), 448.0f);
+          if (h < c.heads && at.at >= 0) {
+            widen8<R>(w[j], x);
+            if (has) *reinterpret_cast<uint2 *>(page + h * c.head_bytes) = codes_of(x, sc);
+            if (sub == 0u) scales[h * c.s_head] = sc;
+          }
+        } else if (h < c.heads && at.at >= 0 && has) {
+          if constexpr (std::is_same<R, P>::value) {
+            store8<P, true>(reinterpret_cast<P *>(page + h * c.head_bytes), w[j]);
+          } else {
+            uint32_t pw[2 * sizeof(P)];
+            widen8<R>(w[j], x);
+            narrow8<P>(x, pw);
+            store8<P, true>(reinterpret_cast<P *>(page + h * c.head_bytes), pw);
+          }
+        }
+      } else if (h < c.heads && at.at != -2 && has) {     // (a position that is not there reads as zeros)
+        if constexpr (Q8) {
+          float x[8];
+          const uint32_t ww[2] = {code[j].x, code[j].y};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(ww[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
+            const float2 f = __half22float2(__half2(hr));
+            x[2 * i] = f.x * scale[j];
+            x[2 * i + 1] = f.y * scale[j];
+          }
+          narrow8<R>(x, w[j]);
+        }
+        store8<R, VEC>(row + static_cast<int64_t>(h) * row_head, w[j]);
+      }
+    }
+  }
+}
+
+// R: type of the rows, P: of the pages. VEC: rows of 16-byte accesses.
+template <typename R, typename P, bool WRITE, bool VEC>
 __global__ void __launch_bounds__(kMoveThreads) b2_cache_move(const __grid_constant__ CacheView c, const __grid_constant__ BatchView b, const __grid_constant__ RowsRef kr,
                                                               const __grid_constant__ RowsRef vr, const __grid_constant__ MoveShape s) {
-  constexpr bool Q8 = sizeof(P) == 1;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint64_t cap = capacity_of(c, b);
   const uint32_t sub = lane & (s.lanes - 1u), group = lane / s.lanes, groups = 32u / s.lanes;
@@ -104,77 +223,16 @@ __global__ void __launch_bounds__(kMoveThreads) b2_cache_move(const __grid_const
       if (q.bad) cache_fault(c.status, kStBadBatch, i, static_cast<uint32_t>(q.bad), static_cast<uint32_t>(q.value));
     }
   }
-  const uint32_t warps = gridDim.x * kMoveWarps, me = blockIdx.x * kMoveWarps + warp, rows = 2u * c.heads;
-  const uint32_t step = warps / s.split, first_row = (me % s.split) * groups + group, row_step = s.split * groups;
+  const uint32_t warps = gridDim.x * kMoveWarps, me = blockIdx.x * kMoveWarps + warp;
+  const uint32_t step = warps / s.split, first = (me % s.split) * groups + group, head_step = s.split * groups;
   uint32_t tok = me / s.split;
-  if (tok >= step) return;                                // (warps that a split leaves over)
   Place now = place_of(c, b, cap, tok);
-  for (; tok < b.n_rows; ) {
+  while (tok < b.n_rows) {
     const uint32_t next = b.n_rows - tok > step ? tok + step : b.n_rows;
     Place after = {-2, 0};
-    for (uint32_t r0 = first_row; r0 - group < rows; r0 += kAtOnce * row_step) {
-      float x[kAtOnce][8], scale[kAtOnce];
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const uint32_t r = r0 + static_cast<uint32_t>(j) * row_step, kv = r >= c.heads ? 1u : 0u, h = r - kv * c.heads;
-        scale[j] = 0.0f;
-        if (r < rows && now.at >= 0) {
-          if (WRITE) {
-            const RowsRef &rr = kv ? vr : kr;
-            if (has) load8(reinterpret_cast<const R *>(rr.p) + static_cast<int64_t>(tok) * rr.row + static_cast<int64_t>(h) * rr.head + sub * 8u, s.vec[kv] != 0u, x[j]);
-          } else {
-            const uint8_t *p = (kv ? c.v : c.k) + now.at + h * c.head_bytes + sub * 8u * sizeof(P);
-            if constexpr (Q8) {
-              scale[j] = (kv ? c.vs : c.ks)[now.scale + h * c.s_head];
-              if (has) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(p);
-                const uint32_t ww[2] = {w.x, w.y};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(ww[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
-                  const float2 f = __half22float2(__half2(hr));
-                  x[j][2 * i] = f.x;
-                  x[j][2 * i + 1] = f.y;
-                }
-              }
-            } else if (has) {
-              load8(reinterpret_cast<const P *>(p), true, x[j]);
-            }
-          }
-        }
-        if (!(r < rows && now.at >= 0 && has)) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
-        }
-      }
-      if (r0 == first_row) after = place_of(c, b, cap, next);      // (under the loads' flight)
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const uint32_t r = r0 + static_cast<uint32_t>(j) * row_step, kv = r >= c.heads ? 1u : 0u, h = r - kv * c.heads;
-        if (WRITE) {
-          if constexpr (Q8) {
-            uint32_t m = 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[j][i]) & 0x7fffffffu);
-            for (uint32_t o = s.lanes >> 1; o > 0u; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float sc = __fdiv_rn(__uint_as_float(m), 448.0f);
-            if (r < rows && now.at >= 0) {
-              if (has) *reinterpret_cast<uint2 *>((kv ? c.v : c.k) + now.at + h * c.head_bytes + sub * 8u) = codes_of(x[j], sc);
-              if (sub == 0u) (kv ? c.vs : c.ks)[now.scale + h * c.s_head] = sc;
-            }
-          } else if (r < rows && now.at >= 0 && has) {
-            store8(reinterpret_cast<P *>((kv ? c.v : c.k) + now.at + h * c.head_bytes) + sub * 8u, true, x[j]);
-          }
-        } else if (r < rows && now.at != -2 && has) {     // (a position that is not there reads as zeros)
-          if constexpr (Q8) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[j][i] = now.at < 0 ? 0.0f : x[j][i] * scale[j];
-          }
-          const RowsRef &rr = kv ? vr : kr;
-          store8(reinterpret_cast<R *>(rr.p) + static_cast<int64_t>(tok) * rr.row + static_cast<int64_t>(h) * rr.head + sub * 8u, s.vec[kv] != 0u, x[j]);
-        }
-      }
-    }
+    move_rows<R, P, WRITE, VEC>(c, s, reinterpret_cast<R *>(kr.p) + static_cast<int64_t>(tok) * kr.row, kr.head, c.k, c.ks, now, first, group, head_step, sub, has,
+                                [&](bool once) { if (once) after = place_of(c, b, cap, next); });      // (under the loads' flight)
+    move_rows<R, P, WRITE, VEC>(c, s, reinterpret_cast<R *>(vr.p) + static_cast<int64_t>(tok) * vr.row, vr.head, c.v, c.vs, now, first, group, head_step, sub, has, [](bool) {});
     tok = next;
     now = after;
   }
@@ -187,15 +245,19 @@ int Launch(const CacheView &c, const BatchView &b, const RowsRef &k, const RowsR
   while (s.lanes * 8u < c.hd) s.lanes *= 2u;
   // Few tokens: a CTA's warps share one, as far as it has rows for them.
   s.split = 1;
-  while (s.split < kMoveWarps && static_cast<uint64_t>(b.n_rows) * s.split < sms * 8u && 2u * c.heads * s.lanes > s.split * 32u) s.split *= 2u;
+  while (s.split < kMoveWarps && static_cast<uint64_t>(b.n_rows) * s.split < sms * 8u && c.heads * s.lanes > s.split * 32u) s.split *= 2u;
   constexpr int64_t W = 16 / sizeof(R);
-  const RowsRef *r[2] = {&k, &v};
-  for (int t = 0; t < 2; ++t)
-    s.vec[t] = reinterpret_cast<uintptr_t>(r[t]->p) % 16 == 0 && r[t]->row % W == 0 && (c.heads == 1u || r[t]->head % W == 0) ? 1u : 0u;
+  bool vec = true;
+  for (const RowsRef *r : {&k, &v}) vec = vec && reinterpret_cast<uintptr_t>(r->p) % 16 == 0 && r->row % W == 0 && (c.heads == 1u || r->head % W == 0);
   const uint64_t want = (static_cast<uint64_t>(b.n_rows) * s.split + kMoveWarps - 1u) / kMoveWarps;
   const uint32_t ctas = want > sms * 8u ? sms * 8u : static_cast<uint32_t>(want);
-  if (write) b2_cache_move<R, P, true><<<ctas, kMoveThreads, 0, stream>>>(c, b, k, v, s);
-  else b2_cache_move<R, P, false><<<ctas, kMoveThreads, 0, stream>>>(c, b, k, v, s);
+  if (write) {
+    if (vec) b2_cache_move<R, P, true, true><<<ctas, kMoveThreads, 0, stream>>>(c, b, k, v, s);
+    else b2_cache_move<R, P, true, false><<<ctas, kMoveThreads, 0, stream>>>(c, b, k, v, s);
+  } else {
+    if (vec) b2_cache_move<R, P, false, true><<<ctas, kMoveThreads, 0, stream>>>(c, b, k, v, s);
+    else b2_cache_move<R, P, false, false><<<ctas, kMoveThreads, 0, stream>>>(c, b, k, v, s);
+  }
   return static_cast<int>(cudaGetLastError());
 }
 
