@@ -61,6 +61,8 @@ ROPE = [  # rows, q heads, k heads, dim, rot, dtype, interleaved, norm, layout, 
     (2500, 4, 2, 128, 96, "bf16", True, True, "fused", "f32", "plain"),
     (9, 2, 2, 200, 8, "f16", False, True, "heads_first", "f32", "plain"),
     (5001, 2, 1, 128, 128, "bf16", False, True, "fused", "f32", "plain"),        # (more than one token to a CTA, the last run shorter)
+    (40, 3, 2, 256, 256, "bf16", False, True, "fused", "f32", "plain"),
+    (17, 2, 2, 256, 128, "f32", True, True, "odd", "f32", "plain"),
     (16384 + 5, 1, 1, 64, 32, "f16", True, True, "fused", "f32", "plain"),
 ]
 
