@@ -20,100 +20,46 @@ namespace {
 
 constexpr int kRopeThreads = 256, kRopeWarps = kRopeThreads / 32;
 constexpr uint32_t kRopeBackPerSm = 2, kRopePerSm = 3;
+constexpr uint32_t kRing = 4;                             // stages of a warp's ring
 
 struct RopeShape {
   uint32_t split;         // warps to a token
   uint32_t lanes;         // threads to a row, a power of two
   uint32_t units;         // V-pair units of a row
   uint32_t rot_units;     // of these turned
+  uint32_t ring_at;       // bytes of shared memory before the rings
 };
 
 // First elements of the two V-wide accesses of unit u.
-template <int V, bool INTER>
+template <int V>
 __device__ __forceinline__ void unit_at(const RopeArgs &a, const RopeShape &s, uint32_t u, uint32_t &e0, uint32_t &e1) {
-  if (INTER) {                                            // (what passes lies in the same way)
-    e0 = 2u * V * u;
-    e1 = e0 + V;
-  } else if (u < s.rot_units) {
-    e0 = V * u;
-    e1 = e0 + a.rot / 2u;
+  if (u < s.rot_units) {
+    if (a.interleaved) { e0 = 2u * V * u; e1 = e0 + V; }
+    else { e0 = V * u; e1 = e0 + a.rot / 2u; }
   } else {
     e0 = a.rot + V * (u - s.rot_units);
     e1 = e0 + (a.hd - a.rot) / 2u;
   }
 }
-// Element of the row that is the first (q 0) or second (q 1) of pair i of a unit.
-template <int V, bool INTER>
-__device__ __forceinline__ uint32_t element(uint32_t e0, uint32_t e1, int i, int q) {
-  if (!INTER) return (q ? e1 : e0) + i;
-  const int at = 2 * i + q;
-  return at < V ? e0 + at : e1 + (at - V);
-}
-
-// Two f32 products at a time, N values.
-__device__ __forceinline__ unsigned long long mul_f32x2(unsigned long long a, unsigned long long b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-template <int N>
-__device__ __forceinline__ void vmul(float (&d)[N], const float (&x)[N], const float (&y)[N]) {
-  if constexpr (N % 2 == 0) {
+// Pair i of a unit in its 2 V values: half layout (i, V + i), neighbours (2 i, 2 i + 1).
+template <int V>
+__device__ __forceinline__ void turn(float (&y)[2 * V], const float2 (&cs)[V], bool inter, float sign) {
+  if (inter) {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) unpack_f32x2(mul_f32x2(pack_f32x2(x[i], x[i + 1]), pack_f32x2(y[i], y[i + 1])), d[i], d[i + 1]);
+    for (int i = 0; i < V; ++i) {
+      const float p = y[2 * i], q = y[2 * i + 1], sn = sign * cs[i].y;
+      y[2 * i] = p * cs[i].x - q * sn;
+      y[2 * i + 1] = p * sn + q * cs[i].x;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) d[i] = x[i] * y[i];
+    for (int i = 0; i < V; ++i) {
+      const float p = y[i], q = y[V + i], sn = sign * cs[i].y;
+      y[i] = p * cs[i].x - q * sn;
+      y[V + i] = p * sn + q * cs[i].x;
+    }
   }
 }
-template <int N>
-__device__ __forceinline__ void vmul(float (&d)[N], const float (&x)[N], float y) {
-  if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) unpack_f32x2(mul_f32x2(pack_f32x2(x[i], x[i + 1]), pack_f32x2(y, y)), d[i], d[i + 1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) d[i] = x[i] * y;
-  }
-}
-// d = x y + c
-template <int N>
-__device__ __forceinline__ void vfma(float (&d)[N], const float (&x)[N], const float (&y)[N], const float (&c)[N]) {
-  if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) unpack_f32x2(fma_f32x2(pack_f32x2(x[i], x[i + 1]), pack_f32x2(y[i], y[i + 1]), pack_f32x2(c[i], c[i + 1])), d[i], d[i + 1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) d[i] = fmaf(x[i], y[i], c[i]);
-  }
-}
-template <int N>
-__device__ __forceinline__ void vfma(float (&d)[N], const float (&x)[N], float y, const float (&c)[N]) {
-  if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) unpack_f32x2(fma_f32x2(pack_f32x2(x[i], x[i + 1]), pack_f32x2(y, y), pack_f32x2(c[i], c[i + 1])), d[i], d[i + 1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) d[i] = fmaf(x[i], y, c[i]);
-  }
-}
-// s + sum x y, in two chains
-template <int N>
-__device__ __forceinline__ float vdot(const float (&x)[N], const float (&y)[N], float s) {
-  if constexpr (N % 2 == 0) {
-    unsigned long long c = pack_f32x2(s, 0.0f);
-#pragma unroll
-    for (int i = 0; i < N; i += 2) c = fma_f32x2(pack_f32x2(x[i], x[i + 1]), pack_f32x2(y[i], y[i + 1]), c);
-    float lo, hi;
-    unpack_f32x2(c, lo, hi);
-    return lo + hi;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(x[i], y[i], s);
-    return s;
-  }
-}
-
 // The two accesses of a unit as they come: V values each, in 32-bit words (one value of 16 bits: in the low half).
 template <typename T, int V> struct Raw {
   static constexpr int W = V * sizeof(T) >= 4 ? V * static_cast<int>(sizeof(T)) / 4 : 1;
@@ -134,8 +80,7 @@ __device__ __forceinline__ void load_words(const void *p, uint32_t *w) {
   }
 }
 template <typename T, int V>
-__device__ __forceinline__ void load_unit(const RowsRef &r, uint32_t tok, uint32_t head, uint32_t e0, uint32_t e1, Raw<T, V> &x) {
-  const T *p = reinterpret_cast<const T *>(r.p) + static_cast<int64_t>(tok) * r.row + static_cast<int64_t>(head) * r.head;
+__device__ __forceinline__ void load_unit(const T *p, uint32_t e0, uint32_t e1, Raw<T, V> &x) {
   load_words<V * sizeof(T)>(p + e0, x.a);
   load_words<V * sizeof(T)>(p + e1, x.b);
 }
@@ -145,44 +90,26 @@ template <> __device__ __forceinline__ float value_of<__nv_bfloat16>(const uint3
 template <> __device__ __forceinline__ float value_of<__half>(const uint32_t *w, int i) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu)));
 }
-// First and second values of the unit's pairs.
-template <typename T, int V, bool INTER>
-__device__ __forceinline__ void widen(const Raw<T, V> &r, float (&p)[V], float (&q)[V]) {
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Raw<T, V> &r, float (&x)[2 * V]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if constexpr (INTER) {
-      p[i] = 2 * i < V ? value_of<T>(r.a, 2 * i) : value_of<T>(r.b, 2 * i - V);
-      q[i] = 2 * i + 1 < V ? value_of<T>(r.a, 2 * i + 1) : value_of<T>(r.b, 2 * i + 1 - V);
-    } else {
-      p[i] = value_of<T>(r.a, i);
-      q[i] = value_of<T>(r.b, i);
-    }
-  }
+  for (int i = 0; i < V; ++i) { x[i] = value_of<T>(r.a, i); x[V + i] = value_of<T>(r.b, i); }
 }
-template <typename T, int V, bool INTER>
-__device__ __forceinline__ void store_unit(const RowsRef &r, uint32_t tok, uint32_t head, uint32_t e0, uint32_t e1, const float (&p)[V], const float (&q)[V]) {
-  T *out = reinterpret_cast<T *>(r.p) + static_cast<int64_t>(tok) * r.row + static_cast<int64_t>(head) * r.head;
+template <typename T, int V>
+__device__ __forceinline__ void store_unit(T *p, uint32_t e0, uint32_t e1, const float (&x)[2 * V]) {
   Vec<T, V> a, b;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if constexpr (INTER) {
-      a.v[i] = FromF<T>(i & 1 ? q[i / 2] : p[i / 2]);
-      b.v[i] = FromF<T>((i + V) & 1 ? q[(i + V) / 2] : p[(i + V) / 2]);
-    } else {
-      a.v[i] = FromF<T>(p[i]);
-      b.v[i] = FromF<T>(q[i]);
-    }
-  }
-  *reinterpret_cast<Vec<T, V> *>(out + e0) = a;
-  *reinterpret_cast<Vec<T, V> *>(out + e1) = b;
+  for (int i = 0; i < V; ++i) { a.v[i] = FromF<T>(x[i]); b.v[i] = FromF<T>(x[V + i]); }
+  *reinterpret_cast<Vec<T, V> *>(p + e0) = a;
+  *reinterpret_cast<Vec<T, V> *>(p + e1) = b;
 }
 __device__ __forceinline__ float row_sum(float v, uint32_t lanes) {
   for (uint32_t o = lanes >> 1; o > 0u; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// U: units of a row that a thread may have (rows of more than 32 units). INTER: neighbouring pairs.
-template <typename T, int V, int U, bool INTER, bool BACK>
+// U: units of a row that a thread may have (rows of more than 32 units).
+template <typename T, int V, int U, bool BACK>
 __global__ void __launch_bounds__(kRopeThreads, BACK ? kRopeBackPerSm : kRopePerSm) b2_rope(const __grid_constant__ RopeArgs a, const __grid_constant__ RopeShape s) {
   extern __shared__ __align__(16) uint8_t sm[];           // weights [2][hd], then the warps' angles [warps][rot / 2]
   float *w_s = reinterpret_cast<float *>(sm);
@@ -203,7 +130,7 @@ __global__ void __launch_bounds__(kRopeThreads, BACK ? kRopeBackPerSm : kRopePer
   for (int k = 0; k < U; ++k) {
     const uint32_t u = sub + static_cast<uint32_t>(k) * s.lanes;
     has[k] = u < s.units;
-    unit_at<V, INTER>(a, s, has[k] ? u : 0u, e0[k], e1[k]);
+    unit_at<V>(a, s, has[k] ? u : 0u, e0[k], e1[k]);
   }
   // sums of the weights' gradients, of a token in registers, of the warp's tokens in shared memory: [warps][2][U][2 V][32]
   const bool sums = BACK && a.partial;
@@ -213,27 +140,70 @@ __global__ void __launch_bounds__(kRopeThreads, BACK ? kRopeBackPerSm : kRopePer
     for (int i = 0; i < 4 * U * V; ++i) acc_s[i * 32] = 0.0f;
   }
   const float inv_hd = 1.0f / static_cast<float>(a.hd);
+  const bool inter = a.interleaved != 0u;
   const uint32_t me = blockIdx.x * kRopeWarps + warp, step = gridDim.x * kRopeWarps / s.split, part = me % s.split;
   const uint32_t stride = s.split * at_once, first = part * at_once + slot;       // the warp's heads
-  Raw<T, V> xr[U], gr[U];                                 // the next rows, on the way
-  auto fetch = [&](uint32_t t, uint32_t tok, uint32_t head) {
+  const bool some[2] = {part * at_once < a.heads[0], part * at_once < a.heads[1]};
+  auto token_after = [&](uint32_t tok) { return a.n_rows - tok > step ? tok + step : a.n_rows; };
+  // The warp's next rows: a unit's two accesses of x and, backward, of the gradient. Of 16 bytes they come through a ring of stages of each thread's own
+  // in shared memory, three on the way while one is worked on; narrower ones straight into registers.
+  constexpr bool RING = V * sizeof(T) == 16;
+  constexpr uint32_t kTensors = BACK ? 2 : 1;
+  Raw<T, V> xr[U], gr[U];
+  uint32_t p_tok = me / s.split, p_t = some[0] ? 0u : 1u, p_head = first, issued = 0, taken = 0;
+  const uint32_t ring = smem_addr(sm) + s.ring_at + warp * (kRing * kTensors * 2u * U * 512u) + lane * 16u;
+  auto issue = [&]() {
+    if (p_tok < a.n_rows) {
+      const bool live = p_head < (p_t ? a.heads[1] : a.heads[0]);
+      const RowsRef &xo = p_t ? a.x[1] : a.x[0], &go = p_t ? a.g[1] : a.g[0];
+      const T *xp = reinterpret_cast<const T *>(xo.p) + (static_cast<int64_t>(p_tok) * xo.row + static_cast<int64_t>(p_head) * xo.head);
+      const T *gp = reinterpret_cast<const T *>(go.p) + (static_cast<int64_t>(p_tok) * go.row + static_cast<int64_t>(p_head) * go.head);
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-      if (head < a.heads[t] && has[k]) {
-        if (!BACK || a.norm) load_unit<T, V>(a.x[t], tok, head, e0[k], e1[k], xr[k]);
-        if (BACK) load_unit<T, V>(a.g[t], tok, head, e0[k], e1[k], gr[k]);
-      } else {                                            // what is not there is 0
+      for (int k = 0; k < U; ++k) {
+        const bool here = live && has[k];
+        if constexpr (RING) {
+          const uint32_t dst = ring + ((issued % kRing) * U + k) * kTensors * 1024u, bytes = here ? 16u : 0u;       // (what is not there is 0)
+          if (!BACK || a.norm) {
+            cp_async_16_zfill(dst, here ? xp + e0[k] : reinterpret_cast<const T *>(xo.p), bytes);
+            cp_async_16_zfill(dst + 512u, here ? xp + e1[k] : reinterpret_cast<const T *>(xo.p), bytes);
+          }
+          if (BACK) {
+            cp_async_16_zfill(dst + 1024u, here ? gp + e0[k] : reinterpret_cast<const T *>(go.p), bytes);
+            cp_async_16_zfill(dst + 1536u, here ? gp + e1[k] : reinterpret_cast<const T *>(go.p), bytes);
+          }
+        } else if (here) {
+          if (!BACK || a.norm) load_unit<T, V>(xp, e0[k], e1[k], xr[k]);
+          if (BACK) load_unit<T, V>(gp, e0[k], e1[k], gr[k]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < Raw<T, V>::W; ++i) { xr[k].a[i] = xr[k].b[i] = 0u; gr[k].a[i] = gr[k].b[i] = 0u; }
+          for (int i = 0; i < Raw<T, V>::W; ++i) { xr[k].a[i] = xr[k].b[i] = 0u; gr[k].a[i] = gr[k].b[i] = 0u; }
+        }
       }
+      p_head += stride;
+      if (p_head - slot >= (p_t ? a.heads[1] : a.heads[0])) {      // the other tensor, or the next token
+        p_head = first;
+        if (p_t == 0u && some[1]) {
+          p_t = 1u;
+        } else {
+          p_t = some[0] ? 0u : 1u;
+          p_tok = token_after(p_tok);
+        }
+      }
+    }
+    if constexpr (RING) cp_async_commit();
+    ++issued;
   };
+  if constexpr (RING) {
+    for (uint32_t i = 0; i + 1u < kRing; ++i) issue();
+  } else {
+    issue();
+  }
   uint32_t tok = me / s.split;
   int32_t pos_next = half && tok < a.n_rows ? a.pos[tok] : 0;
   while (tok < a.n_rows) {
-    const uint32_t next = a.n_rows - tok > step ? tok + step : a.n_rows;
-    fetch(0u, tok, first);
+    const uint32_t next = token_after(tok);
     // ---- the angles of the token ----
-    float cn[U][V], sn[U][V], ns[U][V];                   // cosine, sine, less the sine
+    float2 cs[U][V];
     if (half) {
       __syncwarp();                                       // (those of the token before are in registers)
       const double pos = static_cast<double>(pos_next);
@@ -241,121 +211,112 @@ __global__ void __launch_bounds__(kRopeThreads, BACK ? kRopeBackPerSm : kRopePer
       for (uint32_t f = lane; f < half; f += 32u) {
         double t = pos * a.turns[f];
         t -= rint(t);
-        float sine, cosine;
-        sincospif(2.0f * static_cast<float>(t), &sine, &cosine);
-        cs_s[f] = make_float2(cosine * a.magnitude, sine * a.magnitude);
+        float sn, cn;
+        sincospif(2.0f * static_cast<float>(t), &sn, &cn);
+        cs_s[f] = make_float2(cn * a.magnitude, sn * a.magnitude);
       }
       __syncwarp();
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const uint32_t u = sub + static_cast<uint32_t>(k) * s.lanes;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float2 cs = u < s.rot_units ? cs_s[V * u + i] : make_float2(1.0f, 0.0f);
-          cn[k][i] = cs.x;
-          sn[k][i] = cs.y;
-          ns[k][i] = -cs.y;
-        }
+        for (int i = 0; i < V; ++i) cs[k][i] = u < s.rot_units ? cs_s[V * u + i] : make_float2(1.0f, 0.0f);
       }
     }
 #pragma unroll
     for (uint32_t t = 0; t < 2u; ++t) {                   // queries, keys
       const uint32_t heads = a.heads[t];
-      float wp[U][V], wq[U][V], ap[U][V], aq[U][V];
+      float w[U][2 * V];
       if (a.norm) {
 #pragma unroll
         for (int k = 0; k < U; ++k)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            wp[k][i] = w_s[t * a.hd + element<V, INTER>(e0[k], e1[k], i, 0)];
-            wq[k][i] = w_s[t * a.hd + element<V, INTER>(e0[k], e1[k], i, 1)];
-            ap[k][i] = aq[k][i] = 0.0f;
-          }
+          for (int i = 0; i < V; ++i) { w[k][i] = w_s[t * a.hd + e0[k] + i]; w[k][V + i] = w_s[t * a.hd + e1[k] + i]; }
       }
-      if (t == 1u && part * at_once >= a.heads[0]) fetch(1u, tok, first);       // (else it came with the last of the queries)
+      float acc[U][2 * V];
+      if (BACK) {
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) acc[k][i] = 0.0f;
+      }
+      T *yp = reinterpret_cast<T *>(a.y[t].p) + (static_cast<int64_t>(tok) * a.y[t].row + static_cast<int64_t>(first) * a.y[t].head);
+      const int64_t ys = stride * a.y[t].head;
       for (uint32_t head = first; head - slot < heads; head += stride) {
         const bool live = head < heads;
-        float p[U][V], q[U][V], gp[U][V], gq[U][V];
+        float x[U][2 * V], y[U][2 * V];
+        if constexpr (RING) {
+          cp_async_wait<kRing - 2>();
+          const uint32_t src = ring + (taken % kRing) * U * kTensors * 1024u;
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            auto part_of = [&](uint32_t at, uint32_t *w) {
+              const uint4 v = lds_v4(src + k * kTensors * 1024u + at);
+              w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            };
+            if (!BACK || a.norm) { part_of(0u, xr[k].a); part_of(512u, xr[k].b); }
+            if (BACK) { part_of(1024u, gr[k].a); part_of(1536u, gr[k].b); }
+          }
+          ++taken;
+        }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
-          if (!BACK || a.norm) widen<T, V, INTER>(xr[k], p[k], q[k]);
-          if (BACK) widen<T, V, INTER>(gr[k], gp[k], gq[k]);
+          if (!BACK || a.norm) widen(xr[k], x[k]);
+          if (BACK) widen(gr[k], y[k]);
         }
-        if (head - slot + stride < heads) fetch(t, tok, head + stride);
-        else if (t == 0u) fetch(1u, tok, first);
+        issue();
         float r = 1.0f;
         if (a.norm) {
-          float ss = 0.0f;
+          float ss[2] = {0.0f, 0.0f};
 #pragma unroll
-          for (int k = 0; k < U; ++k) ss += vdot(p[k], p[k], 0.0f) + vdot(q[k], q[k], 0.0f);
-          const float sum = row_sum(ss, s.lanes);
+          for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) { ss[0] += x[k][i] * x[k][i]; ss[1] += x[k][V + i] * x[k][V + i]; }
+          const float sum = row_sum(ss[0] + ss[1], s.lanes);
           r = live ? rsqrtf(sum * inv_hd + a.eps) : 0.0f;       // (no row: adds nothing to the weights' gradients)
         }
         if (!BACK) {
 #pragma unroll
           for (int k = 0; k < U; ++k) {
             if (a.norm) {
-              vmul(p[k], p[k], wp[k]);
-              vmul(q[k], q[k], wq[k]);
+#pragma unroll
+              for (int i = 0; i < 2 * V; ++i) x[k][i] *= r * w[k][i];
             }
-            if (half) {
-              float u[V], v[V];
-              vmul(u, q[k], ns[k]);
-              vmul(v, q[k], cn[k]);
-              vfma(q[k], p[k], sn[k], v);
-              vfma(p[k], p[k], cn[k], u);
-            }
-            if (a.norm) {
-              vmul(p[k], p[k], r);
-              vmul(q[k], q[k], r);
-            }
-            if (live && has[k]) store_unit<T, V, INTER>(a.y[t], tok, head, e0[k], e1[k], p[k], q[k]);
+            if (half) turn<V>(x[k], cs[k], inter, 1.0f);
+            if (live && has[k]) store_unit<T, V>(yp, e0[k], e1[k], x[k]);
           }
         } else {
-          float hx = 0.0f;
+          float hx[2] = {0.0f, 0.0f};
 #pragma unroll
           for (int k = 0; k < U; ++k) {
-            if (half) {
-              float u[V], v[V];
-              vmul(u, gq[k], sn[k]);
-              vmul(v, gq[k], cn[k]);
-              vfma(gq[k], gp[k], ns[k], v);
-              vfma(gp[k], gp[k], cn[k], u);
-            }
+            if (half) turn<V>(y[k], cs[k], inter, -1.0f);
             if (a.norm) {
-              float u[V], v[V];
-              vmul(u, gp[k], p[k]);
-              vmul(v, gq[k], q[k]);
-              vfma(ap[k], u, r, ap[k]);
-              vfma(aq[k], v, r, aq[k]);
-              hx += vdot(u, wp[k], 0.0f) + vdot(v, wq[k], 0.0f);
+#pragma unroll
+              for (int i = 0; i < 2 * V; ++i) {
+                acc[k][i] += y[k][i] * (x[k][i] * r);
+                y[k][i] *= w[k][i];
+                hx[i >= V] += y[k][i] * x[k][i];
+              }
             }
           }
           if (a.norm) {
-            const float c = -(row_sum(hx, s.lanes) * inv_hd * r * r * r);
+            const float c = row_sum(hx[0] + hx[1], s.lanes) * inv_hd * r * r * r;
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-              vmul(gp[k], gp[k], wp[k]);
-              vmul(gq[k], gq[k], wq[k]);
-              vmul(p[k], p[k], c);
-              vmul(q[k], q[k], c);
-              vfma(gp[k], gp[k], r, p[k]);
-              vfma(gq[k], gq[k], r, q[k]);
-            }
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+              for (int i = 0; i < 2 * V; ++i) y[k][i] = r * y[k][i] - c * x[k][i];
           }
 #pragma unroll
           for (int k = 0; k < U; ++k)
-            if (live && has[k]) store_unit<T, V, INTER>(a.y[t], tok, head, e0[k], e1[k], gp[k], gq[k]);
+            if (live && has[k]) store_unit<T, V>(yp, e0[k], e1[k], y[k]);
         }
+        yp += ys;
       }
       if (sums) {
 #pragma unroll
         for (int k = 0; k < U; ++k)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            acc_s[((t * U + k) * 2 * V + 2 * i) * 32] += ap[k][i];
-            acc_s[((t * U + k) * 2 * V + 2 * i + 1) * 32] += aq[k][i];
-          }
+          for (int i = 0; i < 2 * V; ++i) acc_s[((t * U + k) * 2 * V + i) * 32] += acc[k][i];
       }
     }
     tok = next;
@@ -381,7 +342,7 @@ __global__ void __launch_bounds__(kRopeThreads, BACK ? kRopeBackPerSm : kRopePer
     for (int k = 0; k < U; ++k)
 #pragma unroll
       for (int i = 0; i < 2 * V; ++i)
-        if (slot == 0u && has[k]) red[(warp * 2u + t) * a.hd + element<V, INTER>(e0[k], e1[k], i / 2, i & 1)] = v[t][k][i];
+        if (slot == 0u && has[k]) red[(warp * 2u + t) * a.hd + (i < V ? e0[k] + i : e1[k] + i - V)] = v[t][k][i];
   __syncthreads();
   const uint32_t cols = 2u * a.hd;
   for (uint32_t i = tid; i < cols; i += kRopeThreads) {
@@ -428,8 +389,8 @@ uint32_t Pow2AtLeast(uint32_t v) {
   return p;
 }
 
-template <typename T, int V, int U, bool INTER, bool BACK>
-int LaunchAs(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
+template <typename T, int V, int U, bool BACK>
+int Launch(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
   RopeShape s;
   s.units = a.hd / 2u / V;
   s.rot_units = a.rot / 2u / V;
@@ -442,15 +403,17 @@ int LaunchAs(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
   const uint32_t most = (BACK ? kRopeBackPerSm : kRopePerSm) * sms;
   const uint32_t ctas = want < 1u ? 1u : want > most ? most : static_cast<uint32_t>(want);
   size_t smem = sizeof(float) * 2u * a.hd + sizeof(float2) * kRopeWarps * (a.rot / 2u);
-  if (BACK && a.partial) smem += sizeof(float) * kRopeWarps * 2u * U * 2 * V * 32u;       // (43 KB at most)
-  b2_rope<T, V, U, INTER, BACK><<<ctas, kRopeThreads, smem, stream>>>(a, s);
+  if (BACK && a.partial) smem += sizeof(float) * kRopeWarps * 2u * U * 2 * V * 32u;
+  smem = (smem + 15u) & ~size_t(15);
+  s.ring_at = static_cast<uint32_t>(smem);
+  if (V * sizeof(T) == 16) smem += kRopeWarps * kRing * (BACK ? 2u : 1u) * 2u * U * 512u;       // 107 KB at most in all
+  if (smem > 48u * 1024u) {
+    const cudaError_t e = cudaFuncSetAttribute(b2_rope<T, V, U, BACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  b2_rope<T, V, U, BACK><<<ctas, kRopeThreads, smem, stream>>>(a, s);
   if (BACK && a.partial) b2_rope_weights<<<(2u * a.hd + 31u) / 32u, kSumWarps * 32u, 0, stream>>>(a, ctas);
   return static_cast<int>(cudaGetLastError());
-}
-
-template <typename T, int V, int U, bool BACK>
-int Launch(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
-  return a.interleaved ? LaunchAs<T, V, U, true, BACK>(a, sms, stream) : LaunchAs<T, V, U, false, BACK>(a, sms, stream);
 }
 
 // The widest access that every address of the call allows.
