@@ -15,7 +15,10 @@
 // 8-bit pages: codes become f16 on their way into the ring (exact), q is scaled by a power of two for each row to fit f16, a key's scale
 // goes onto its scores and a value's onto p (see attend_step.cu).
 //
-// Few tiles: the keys of a tile are split over as many CTAs as there are SMs for, and a second launch joins their results.
+// Work: one CTA to an SM. The tiles of the batch in a row, sequence by sequence and head by head, each weighed by the keys it sees and something for its
+// beginning and end, are dealt to the CTAs in equal runs, whatever their number and lengths; a run that ends inside a tile ends between
+// two blocks of its keys, and a second launch joins the parts. The filling warps walk the run; the others read what they need of a tile
+// from shared memory. The ring runs on from tile to tile.
 #include "attend_common.cuh"
 #include "tc_common.cuh"
 
@@ -24,8 +27,8 @@ namespace {
 
 constexpr uint32_t kCkRows = 128, kCkKeys = 128;          // rows of a slot, keys of a block
 constexpr uint32_t kSoftWarps = 8, kLoadWarps = 4, kCkThreads = (kSoftWarps + kLoadWarps + 4) * 32;     // (three of the last four warps only hold registers back)
-// Registers of a thread: launched with 128 each, the softmax warps take those that the others give up (2 x 184 + 88 + 56 = 4 x 128).
-constexpr int kSoftRegs = 184, kLoadRegs = 88, kIssueRegs = 56;
+// Registers of a thread: launched with 128 each, the softmax warps take those that the others give up (2 x 184 + 88 + 56 = 2 x 176 + 104 + 56 = 4 x 128).
+constexpr int kSoftRegs = 184, kLoadRegs = 88, kSoftRegs8 = 176, kLoadRegs8 = 104, kIssueRegs = 56;
 constexpr uint32_t kCkCols = 512;                         // tensor memory: S0, S1 (128 columns each), O0, O1
 constexpr float kGrow = 8.0f;                             // log2 of the growth of a row maximum that forces a rescale
 constexpr float kCkPScale = 64.0f;                        // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
@@ -38,10 +41,17 @@ struct ChunkShape {
   static constexpr uint32_t kStages = HD == 128 ? 5 : 8;
   static constexpr uint32_t kQ = 0, kRing = 2 * kBlock, kScales = kRing + kStages * kBlock, kShared = kScales + 2u * 1024u;      // scales of two blocks: K's, V's
 };
+// A tile's part that a CTA works on: packed rows [r0, r0 + rows) of a sequence (row x group + head), blocks [b0, b1) of the `blocks` of keys from
+// keys.lo that any of them sees.
+struct Tile {
+  uint32_t seq, head, r0, rows, blocks, b0, b1, part;     // part: 0 whole, else 1 + where its results go
+  Seq s;
+  Span keys;
+};
 struct ChunkShared {
-  uint64_t q_full, full[8], empty[8], s_full[2], p_full[2], pv_done[2], scales_free[2];
+  uint64_t q_full, q_free, full[8], empty[8], s_full[2], p_full[2], pv_done[2], scales_free[2][2];
   uint32_t tmem, failed;
-  uint32_t redo[8];
+  Tile tile;                                              // no rows: the end
   union {
     unsigned long long find[kCkThreads / 32 + 2];         // (before any row is looked at)
     int8_t q_exp[256];                                    // 8-bit pages: each row of q was scaled by 2^e
@@ -51,122 +61,205 @@ template <int HD>
 constexpr uint32_t ChunkSmem() { return ChunkShape<HD>::kShared + ((sizeof(ChunkShared) + 15u) & ~15u); }
 static_assert(ChunkSmem<128>() <= 227u * 1024u && ChunkSmem<64>() <= 227u * 1024u, "shared memory of an SM");
 
-// A tile of rows: packed rows [r0, r0 + rows) of sequence `seq` (row x group + head), and the blocks of keys that any of them sees.
-struct Tile {
-  uint32_t seq, r0, rows;
-  Seq s;
-  Span keys;
-  uint32_t blocks;
+// ---- how the work is dealt ----
+typedef unsigned long long u64;
+// Weights of a sequence's tiles (of one head): tile t weighs base + slope (t + 1), the last one less by `short_by`; in keys x group, and kTileCost blocks
+// for what a tile costs beside its blocks.
+constexpr uint32_t kTileCost = 3;
+struct Weights {
+  uint32_t tiles;
+  u64 base, slope, short_by;
+  __device__ __forceinline__ u64 before(u64 t) const { return t * base + slope * (t * (t + 1ull) / 2ull); }
+  __device__ __forceinline__ u64 all() const { return tiles ? before(tiles) - short_by : 0ull; }
 };
-__device__ __forceinline__ Tile make_tile(const AttendArgs &a, uint64_t cap, uint32_t seq, uint32_t index) {
-  Tile t;
-  t.seq = seq;
-  t.s = load_seq(a.b, cap, seq);
-  t.r0 = index * kChunkRows;
-  t.rows = min(t.r0 + kChunkRows, static_cast<uint32_t>(t.s.n) * a.group) - t.r0;
-  t.keys = SeenByRows(t.s, static_cast<int32_t>(t.r0 / a.group), static_cast<int32_t>((t.r0 + t.rows - 1u) / a.group) + 1, a.causal, a.window);
-  t.blocks = (static_cast<uint32_t>(t.keys.hi - t.keys.lo) + kCkKeys - 1u) / kCkKeys;
-  return t;
-}
-__device__ __forceinline__ unsigned long long tiles_of_seq(const AttendArgs &a, uint64_t cap, uint32_t i) {
-  const Seq s = load_seq(a.b, cap, i);
-  return (static_cast<unsigned long long>(s.n) * a.group + kChunkRows - 1u) / kChunkRows;
-}
-// The work of a CTA: which tile, cache head, part of the tile's blocks. Tiles with the most keys (a sequence's last) come first.
-struct Work { uint32_t tile, head, split, item; };
-__device__ __forceinline__ Work work_of(const AttendArgs &a, uint32_t index, uint32_t splits) {
-  Work w;
-  w.split = index % splits;
-  w.item = index / splits;
-  w.head = w.item % a.c.heads;
-  w.tile = a.tiles - 1u - w.item / a.c.heads;
+__device__ __forceinline__ Weights weights_of(const AttendArgs &a, const Seq &s) {
+  Weights w;
+  const u64 rows = static_cast<u64>(s.n) * a.group;
+  w.tiles = static_cast<uint32_t>((rows + kChunkRows - 1u) / kChunkRows);
+  const u64 past = s.len > s.n ? static_cast<u64>(s.len - s.n) : 0ull;
+  u64 keys = static_cast<u64>(s.len);
+  w.slope = 0ull;
+  w.short_by = 0ull;
+  if (a.causal && a.window) {
+    keys = min(keys, static_cast<u64>(a.window) + kChunkRows / a.group);
+  } else if (a.causal) {
+    keys = past;
+    w.slope = kChunkRows;
+    w.short_by = w.tiles * static_cast<u64>(kChunkRows) - rows;
+  }
+  w.base = (keys + kTileCost * kCkKeys) * a.group;
   return w;
 }
-// Blocks [b0, b1) of a split, and how many splits have any.
-__device__ __forceinline__ void split_of(uint32_t blocks, uint32_t splits, uint32_t split, uint32_t &b0, uint32_t &b1, uint32_t &used) {
-  const uint32_t per = (blocks + splits - 1u) / splits;
-  b0 = min(blocks, split * per);
-  b1 = min(blocks, b0 + per);
-  used = per ? (blocks + per - 1u) / per : 0u;
+// The whole batch: weight of everything, CTAs that share it (a few blocks at least for each).
+__device__ __forceinline__ u64 units_of_seq(const AttendArgs &a, uint64_t cap, uint32_t i) { return weights_of(a, load_seq(a.b, cap, i)).all() * a.c.heads; }
+__device__ __forceinline__ uint32_t ctas_of(const AttendArgs &a, u64 all, uint32_t most) {
+  const u64 n = all / (static_cast<u64>(kTileCost + 2u) * kCkKeys * a.group);
+  return n < 1ull ? 1u : n > most ? most : static_cast<uint32_t>(n);
 }
+struct Runs {
+  u64 each;
+  uint32_t rest, ctas;
+  __device__ __forceinline__ Runs(u64 all, uint32_t n) : each(all / n), rest(static_cast<uint32_t>(all - all / n * n)), ctas(n) {}
+  __device__ __forceinline__ u64 begin(uint32_t cta) const { return each * cta + rest * cta / ctas; }     // (rest and cta are below the SMs)
+};
+
+// A place in the row of tiles.
+struct Walk {
+  uint32_t seq, head, index;
+  Seq s;
+  Weights w;
+  u64 at;                                                 // weight before the tile
+  __device__ __forceinline__ u64 weight() const { return w.base + w.slope * (index + 1ull) - (index + 1u == w.tiles ? w.short_by : 0ull); }
+  // to the tile that holds unit x, of sequence `seq` whose units begin at x0
+  __device__ __forceinline__ void seek(const AttendArgs &a, uint64_t cap, uint32_t b, u64 x0, u64 x) {
+    seq = b;
+    s = load_seq(a.b, cap, b);
+    w = weights_of(a, s);
+    const u64 one = w.all();
+    head = static_cast<uint32_t>((x - x0) / one);
+    at = x0 + head * one;
+    uint32_t lo = 0, hi = w.tiles;                        // before(lo) <= x - at < before(hi)
+    while (hi - lo > 1u) {
+      const uint32_t mid = (lo + hi) / 2u;
+      if (w.before(mid) <= x - at) lo = mid;
+      else hi = mid;
+    }
+    index = lo;
+    at += w.before(lo);
+  }
+  __device__ __forceinline__ bool next(const AttendArgs &a, uint64_t cap) {
+    at += weight();
+    if (++index < w.tiles) return true;
+    index = 0;
+    if (++head < a.c.heads) return true;
+    head = 0;
+    do {
+      if (++seq >= a.b.n_seqs) return false;
+      s = load_seq(a.b, cap, seq);
+      w = weights_of(a, s);
+    } while (w.tiles == 0u);
+    return true;
+  }
+  // the tile's blocks that a run over units [x, y) has
+  __device__ __forceinline__ void tile(const AttendArgs &a, u64 x, u64 y, Tile &t) const {
+    t.seq = seq;
+    t.head = head;
+    t.s = s;
+    t.r0 = index * kChunkRows;
+    t.rows = min(t.r0 + kChunkRows, static_cast<uint32_t>(s.n) * a.group) - t.r0;
+    t.keys = SeenByRows(s, static_cast<int32_t>(t.r0 / a.group), static_cast<int32_t>((t.r0 + t.rows - 1u) / a.group) + 1, a.causal, a.window);
+    t.blocks = (static_cast<uint32_t>(t.keys.hi - t.keys.lo) + kCkKeys - 1u) / kCkKeys;
+    t.b0 = block_at(t.blocks, x);
+    t.b1 = block_at(t.blocks, y);
+  }
+  // the block at which a run that begins at unit x begins
+  __device__ __forceinline__ uint32_t block_at(uint32_t blocks, u64 x) const {
+    if (x <= at) return 0u;
+    const u64 all = weight();
+    return x - at >= all ? blocks : static_cast<uint32_t>((x - at) * blocks / all);
+  }
+};
 
 __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk) {      // 16-byte chunk of a row of HD values
   return (chunk >> 3) * (128u * 128u) + row * 128u + (((chunk & 7u) ^ (row & 7u)) << 4);
 }
 
+// Rows that see nothing of the cache.
+__device__ __forceinline__ void clear_rows(const AttendArgs &a, const Tile &t, uint32_t thread, uint32_t threads) {
+  for (uint32_t i = thread; i < t.rows * a.c.hd; i += threads) {
+    const uint32_t r = i / a.c.hd, d = i - r * a.c.hd, pr = t.r0 + r, tok = a.by_group.quot(pr), h = t.head * a.group + (pr - tok * a.group);
+    const int32_t row = t.s.first + static_cast<int32_t>(tok);
+    store_row_value(row_at(a.o, row, h) + 2u * d, 0.0f, a.bf16 != 0u);
+    if (d == 0u && a.lse) a.lse[static_cast<int64_t>(row) * a.q_heads + h] = -INFINITY;
+  }
+}
+
 // ---- the filling warps ----------------------------------------------------------------------
+// Rows of q into shared memory, a 16-byte chunk to a thread. As they are they come by asynchronous copies (still under way on return).
 template <bool BF, bool Q8, int HD>
-static __device__ __forceinline__ void chunk_load(const AttendArgs &a, const Tile &t, uint32_t head, uint32_t b0, uint32_t b1, uint8_t *sm, ChunkShared *S) {
+static __device__ __forceinline__ void load_q(const AttendArgs &a, const Tile &t, uint32_t tid, uint32_t base, int8_t *q_exp) {
+  using Sh = ChunkShape<HD>;
+  constexpr uint32_t QL = HD / 8, AT = kLoadWarps * 32u / QL;      // threads to a row, rows at once
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.q.p) & 15u) | ((a.q.row | a.q.head) & 7)) == 0;
+  const uint32_t c = tid % QL, r0 = tid / QL, rows = t.rows > kCkRows ? 256u : 128u;
+  const bool in_hd = c * 8u < a.c.hd;
+  auto place = [&](uint32_t r) {
+    const uint32_t pr = t.r0 + r, tok = a.by_group.quot(pr);
+    return row_at(a.q, t.s.first + static_cast<int32_t>(tok), t.head * a.group + (pr - tok * a.group)) + 16u * c;
+  };
+  auto chunk = [&](uint32_t r) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (r < t.rows && in_hd) {
+      const uint8_t *p = place(r);
+      if (vec) {
+        v = *reinterpret_cast<const uint4 *>(p);
+      } else {
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+        v = make_uint4(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16), h[4] | (static_cast<uint32_t>(h[5]) << 16),
+                       h[6] | (static_cast<uint32_t>(h[7]) << 16));
+      }
+    }
+    return v;
+  };
+  auto dst = [&](uint32_t r) { return base + Sh::kQ + (r >> 7) * Sh::kBlock + swizzled(r & 127u, c); };
+  if (Q8 && BF) {
+#pragma unroll 1
+    for (uint32_t r = r0; r < rows; r += 4u * AT) {
+      uint4 v[4];
+#pragma unroll
+      for (uint32_t k = 0; k < 4u; ++k) v[k] = chunk(r + k * AT);
+#pragma unroll
+      for (uint32_t k = 0; k < 4u; ++k) {
+        const uint32_t ww[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(ww[i] << 16)), fabsf(__uint_as_float(ww[i] & 0xffff0000u))));
+#pragma unroll
+        for (uint32_t o = QL / 2u; o > 0u; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = static_cast<int>(__float_as_uint(top) >> 23);
+        const int e = ex == 0 || ex == 255 ? 0 : max(-100, min(100, 127 + 14 - ex));
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        if (c == 0u) q_exp[r + k * AT] = static_cast<int8_t>(e);
+        auto h2 = [&](uint32_t x) { return cvt_f16x2(__uint_as_float(x & 0xffff0000u) * up, __uint_as_float(x << 16) * up); };
+        sts_v4(dst(r + k * AT), make_uint4(h2(v[k].x), h2(v[k].y), h2(v[k].z), h2(v[k].w)));
+      }
+    }
+  } else if (vec) {
+#pragma unroll 4
+    for (uint32_t r = r0; r < rows; r += AT) {
+      const bool has = r < t.rows && in_hd;
+      cp_async_16_zfill(dst(r), has ? place(r) : a.q.p, has ? 16u : 0u);
+    }
+  } else {
+#pragma unroll 1
+    for (uint32_t r = r0; r < rows; r += AT) sts_v4(dst(r), chunk(r));
+  }
+}
+
+template <bool BF, bool Q8, int HD>
+static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk, u64 x0, u64 x1, uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<HD>;
   constexpr uint32_t NS = Sh::kStages;
   volatile uint32_t *failed = &S->failed;
+  const uint64_t cap = capacity_of(a.c, a.b);
   const uint32_t tid = threadIdx.x - kSoftWarps * 32u, lane = tid & 31u, w = tid >> 5;
   const uint32_t base = smem_addr(sm);
   uint32_t it = 0;                                        // blocks filled so far: K, V, K, V, ..
+  uint32_t used[2][2] = {{0u, 0u}, {0u, 0u}};             // 8-bit pages: how often each slot has used each place for scales
+  Tile t = {};
   // the lane's key of a block: 32 w + lane
   int32_t page = -1;
   uint32_t slot = 0, entry = 0;
   bool live = false;
   auto look_ahead = [&](uint32_t j) {
     const int32_t p = t.keys.lo + static_cast<int32_t>(j * kCkKeys + 32u * w + lane);
-    live = j < b1 && p < t.keys.hi;
+    live = j < t.b1 && p < t.keys.hi;
     if (live) {
       entry = a.c.by_page.quot(static_cast<uint32_t>(p));
       slot = static_cast<uint32_t>(p) - entry * a.c.page_size;
       page = __ldg(a.b.pages + static_cast<int64_t>(t.seq) * a.b.pages_stride + entry);
     }
   };
-  look_ahead(b0);
-  // ---- Q: a thread to a row of each slot ----
-  const bool vec = ((reinterpret_cast<uintptr_t>(a.q.p) & 15u) | ((a.q.row | a.q.head) & 7)) == 0;
-#pragma unroll 1
-  for (uint32_t s = 0; s < 2u; ++s) {
-    const uint32_t r = s * kCkRows + tid;
-    if (s * kCkRows >= t.rows) break;
-    const bool has = r < t.rows;
-    const uint32_t pr = t.r0 + r, tok = pr / a.group;
-    const uint8_t *p = has ? row_at(a.q, t.s.first + static_cast<int32_t>(tok), head * a.group + (pr - tok * a.group)) : a.q.p;
-    auto chunk = [&](uint32_t c) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (has && c * 8u < a.c.hd) {
-        if (vec) {
-          v = *reinterpret_cast<const uint4 *>(p + 16u * c);
-        } else {
-          const uint16_t *h = reinterpret_cast<const uint16_t *>(p) + 8u * c;
-          v = make_uint4(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16), h[4] | (static_cast<uint32_t>(h[5]) << 16),
-                         h[6] | (static_cast<uint32_t>(h[7]) << 16));
-        }
-      }
-      return v;
-    };
-    const uint32_t dst = base + Sh::kQ + s * Sh::kBlock;
-    if (Q8 && BF) {
-      float top = 0.0f;
-#pragma unroll 4
-      for (uint32_t c = 0; c < HD / 8; ++c) {
-        const uint4 v = chunk(c);
-        const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(ww[i] << 16)), fabsf(__uint_as_float(ww[i] & 0xffff0000u))));
-      }
-      const int ex = static_cast<int>(__float_as_uint(top) >> 23);
-      const int e = ex == 0 || ex == 255 ? 0 : max(-100, min(100, 127 + 14 - ex));
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      S->q_exp[r] = static_cast<int8_t>(e);
-#pragma unroll 4
-      for (uint32_t c = 0; c < HD / 8; ++c) {
-        uint4 v = chunk(c);
-        auto h2 = [&](uint32_t x) { return cvt_f16x2(__uint_as_float(x & 0xffff0000u) * up, __uint_as_float(x << 16) * up); };
-        v.x = h2(v.x); v.y = h2(v.y); v.z = h2(v.z); v.w = h2(v.w);
-        sts_v4(dst + swizzled(tid, c), v);
-      }
-    } else {
-#pragma unroll 4
-      for (uint32_t c = 0; c < HD / 8; ++c) sts_v4(dst + swizzled(tid, c), chunk(c));
-    }
-  }
-  fence_proxy_async_smem();
-  mbar_arrive(&S->q_full);
   // ---- K and V ----
   auto place = [&](int64_t &off, int64_t &soff) -> uint32_t {       // the lane's key; which lanes of the warp have one
     bool ok = live;
@@ -174,8 +267,8 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, const Til
       cache_fault(a.c.status, kStBadPage, t.seq, entry, static_cast<uint32_t>(page));
       ok = false;
     }
-    off = ok ? page * a.c.page_bytes + slot * a.c.slot_bytes + head * a.c.head_bytes : 0;
-    soff = ok && Q8 ? page * a.c.s_page + slot * a.c.s_slot + head * a.c.s_head : 0;
+    off = ok ? page * a.c.page_bytes + slot * a.c.slot_bytes + t.head * a.c.head_bytes : 0;
+    soff = ok && Q8 ? page * a.c.s_page + slot * a.c.s_slot + t.head * a.c.s_head : 0;
     return __ballot_sync(0xffffffffu, ok);
   };
   auto room = [&](uint32_t i) { return tc_wait(&S->empty[i % NS], ((i / NS) & 1u) ^ 1u, failed, kBudget); };
@@ -184,99 +277,149 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, const Til
     mbar_arrive(&S->full[i % NS]);
   };
   bool ok = true;
-  if constexpr (!Q8) {
-    constexpr uint32_t CH = HD / 8, AT = 32u / CH;        // chunks of a row; rows at once
-    const uint32_t sub = lane % CH, r1 = lane / CH;
-    const bool in_hd = sub * 8u < a.c.hd;
-    auto copy = [&](const uint8_t *pages, uint32_t i, int64_t off, uint32_t mask) {
-      const uint32_t dst = base + Sh::kRing + (i % NS) * Sh::kBlock;
+  constexpr uint32_t CH = Q8 ? HD / 16 : HD / 8, AT = 32u / CH, N = 32u / AT;     // 16-byte chunks of a row; rows at once; loads of a thread
+  const uint32_t sub = lane % CH, r1 = lane / CH;
+  const bool in_hd = sub * 16u < a.c.hd * (Q8 ? 1u : 2u);
+  auto copy = [&](const uint8_t *pages, uint32_t i, int64_t off, uint32_t mask) {
+    const uint32_t dst = base + Sh::kRing + (i % NS) * Sh::kBlock;
 #pragma unroll
-      for (uint32_t k = 0; k < 32u / AT; ++k) {
-        const uint32_t r = k * AT + r1;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r);
-        const uint32_t bytes = ((mask >> r) & 1u) && in_hd ? 16u : 0u;
-        cp_async_16_zfill(dst + swizzled(32u * w + r, sub), pages + (bytes ? o + 16 * sub : 0), bytes);
+    for (uint32_t k = 0; k < N; ++k) {
+      const uint32_t r = k * AT + r1;
+      const int64_t o = __shfl_sync(0xffffffffu, off, r);
+      const uint32_t bytes = ((mask >> r) & 1u) && in_hd ? 16u : 0u;
+      cp_async_16_zfill(dst + swizzled(32u * w + r, sub), pages + (bytes ? o + 16 * sub : 0), bytes);
+    }
+    cp_async_commit();
+  };
+  auto fetch = [&](const uint8_t *pages, int64_t off, uint32_t mask, uint4 (&x)[N]) {
+#pragma unroll
+    for (uint32_t k = 0; k < N; ++k) {
+      const uint32_t r = k * AT + r1;
+      const int64_t o = __shfl_sync(0xffffffffu, off, r);
+      x[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (((mask >> r) & 1u) && in_hd) x[k] = ldg_v4(pages + o + 16 * sub);
+    }
+  };
+  auto put = [&](uint32_t i, const uint4 (&x)[N], float scale) {
+    const uint32_t dst = base + Sh::kRing + (i % NS) * Sh::kBlock;
+#pragma unroll
+    for (uint32_t k = 0; k < N; ++k) {
+      const uint32_t r = 32u * w + k * AT + r1;
+      const uint32_t c[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+      uint32_t h[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) { h[2 * q] = cvt_e4m3x2_f16x2(c[q] & 0xffffu); h[2 * q + 1] = cvt_e4m3x2_f16x2(c[q] >> 16); }
+      sts_v4(dst + swizzled(r, 2u * sub), make_uint4(h[0], h[1], h[2], h[3]));
+      sts_v4(dst + swizzled(r, 2u * sub + 1u), make_uint4(h[4], h[5], h[6], h[7]));
+    }
+    // (the place for the scales of block i / 2; the softmax is done with those of the block two before)
+    *reinterpret_cast<float *>(sm + Sh::kScales + (i & 3u) * 512u + (32u * w + lane) * 4u) = scale;
+  };
+  uint32_t settled = 0;                                   // 16-bit pages: blocks that have landed and are said to have
+  auto settle = [&](uint32_t n) {
+    for (; settled < n; ++settled) done(settled);
+  };
+  uint32_t turn = 0;                                      // tiles so far
+  for (bool more = true; ok; ++turn) {
+    // ---- the next tile of the run that has blocks there ----
+    bool found = false;
+    while (more && !found) {
+      more = wk.at < x1;
+      if (!more) break;
+      wk.tile(a, x0, x1, t);
+      // (rows that see no key are cleared by the CTA in whose run the tile begins)
+      if (t.blocks == 0u) {
+        if (wk.at >= x0) clear_rows(a, t, tid, kLoadWarps * 32u);
       }
+      found = t.b0 < t.b1;
+      t.part = t.b0 == 0u && t.b1 == t.blocks ? 0u : 1u + blockIdx.x * 2u + (t.b0 == 0u ? 1u : 0u);
+      more = wk.next(a, cap);
+    }
+    if (!found) t.rows = 0u;
+    const uint32_t slots = t.rows > kCkRows ? 2u : 1u;
+    if (found) look_ahead(t.b0);
+    bool q_there = false;
+    auto q_to_all = [&]() {                               // Q and the tile, when the scores of the tile before are done
+      q_there = true;
+      ok = ok && __all_sync(0xffffffffu, tc_wait(&S->q_free, (turn & 1u) ^ 1u, failed, kBudget));
+      if (!ok) return;
+      if (tid == 0u) S->tile = t;
+      if (found) load_q<BF, Q8, HD>(a, t, tid, base, S->q_exp);
       cp_async_commit();
+      cp_async_wait_all();
+      fence_proxy_async_smem();
+      mbar_arrive(&S->q_full);
     };
-    for (uint32_t j = b0; ok && j < b1; ++j) {
+    if (!found) {
+      if constexpr (!Q8) {
+        cp_async_wait_all();
+        settle(it);
+      }
+      q_to_all();
+      break;
+    }
+    if constexpr (!Q8) {
+      for (uint32_t j = t.b0; ok && j < t.b1; ++j) {
+        int64_t off, soff;
+        const uint32_t mask = place(off, soff);
+        look_ahead(j + 1u);
+#pragma unroll
+        for (uint32_t v = 0; v < 2u; ++v) {
+          // (a lane that gave up takes its warp with it)
+          ok = __all_sync(0xffffffffu, ok && room(it));
+          if (!ok) break;
+          copy(v ? a.c.v : a.c.k, it, off, mask);
+          ++it;
+          if (it > settled + 2u) { cp_async_wait<2>(); settle(it - 2u); }
+        }
+        if (ok && !q_there) {                             // (the products wait for these blocks and for Q)
+          q_to_all();                                     // (waits for what is on the way)
+          if (ok) settle(it);
+        }
+      }
+    } else {
+      uint4 kw[N], vw[N];
       int64_t off, soff;
-      const uint32_t mask = place(off, soff);
-      look_ahead(j + 1u);
-#pragma unroll
-      for (uint32_t v = 0; v < 2u; ++v) {
-        // (a lane that gave up takes its warp with it)
-        ok = __all_sync(0xffffffffu, ok && room(it));
-        if (!ok) break;
-        copy(v ? a.c.v : a.c.k, it, off, mask);
-        if (it >= 2u) { cp_async_wait<2>(); done(it - 2u); }
-        ++it;
-      }
-    }
-    cp_async_wait_all();
-    if (ok) {
-      if (it >= 2u) done(it - 2u);
-      if (it >= 1u) done(it - 1u);
-    }
-  } else {
-    constexpr uint32_t CH = HD / 16, AT = 32u / CH, N = 32u / AT;     // 16-code chunks of a row; rows at once; loads of a thread
-    const uint32_t sub = lane % CH, r1 = lane / CH;
-    const bool in_hd = sub * 16u < a.c.hd;
-    uint4 kw[N], vw[N];
-    float ksc = 0.0f, vsc = 0.0f;
-    auto fetch = [&](const uint8_t *pages, int64_t off, uint32_t mask, uint4 (&x)[N]) {
-#pragma unroll
-      for (uint32_t k = 0; k < N; ++k) {
-        const uint32_t r = k * AT + r1;
-        const int64_t o = __shfl_sync(0xffffffffu, off, r);
-        x[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (((mask >> r) & 1u) && in_hd) x[k] = ldg_v4(pages + o + 16 * sub);
-      }
-    };
-    auto put = [&](uint32_t i, const uint4 (&x)[N], float scale) {
-      // (block i / 2's place for scales; the softmax is done with those of the block two before)
-      const uint32_t dst = base + Sh::kRing + (i % NS) * Sh::kBlock;
-#pragma unroll
-      for (uint32_t k = 0; k < N; ++k) {
-        const uint32_t r = 32u * w + k * AT + r1;
-        const uint32_t c[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-        uint32_t h[8];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) { h[2 * q] = cvt_e4m3x2_f16x2(c[q] & 0xffffu); h[2 * q + 1] = cvt_e4m3x2_f16x2(c[q] >> 16); }
-        sts_v4(dst + swizzled(r, 2u * sub), make_uint4(h[0], h[1], h[2], h[3]));
-        sts_v4(dst + swizzled(r, 2u * sub + 1u), make_uint4(h[4], h[5], h[6], h[7]));
-      }
-      *reinterpret_cast<float *>(sm + Sh::kScales + (i & 3u) * 512u + (32u * w + lane) * 4u) = scale;
-    };
-    int64_t off, soff;
-    uint32_t mask = place(off, soff);
-    fetch(a.c.k, off, mask, kw);
-    ksc = (mask >> lane) & 1u ? a.c.ks[soff] : 0.0f;
-    for (uint32_t j = b0; ok && j < b1; ++j) {
-      fetch(a.c.v, off, mask, vw);
-      vsc = (mask >> lane) & 1u ? a.c.vs[soff] : 0.0f;
-      look_ahead(j + 1u);
-      const uint32_t n = j - b0;
-      ok = __all_sync(0xffffffffu, room(it) && tc_wait(&S->scales_free[n & 1u], ((n >> 1) & 1u) ^ 1u, failed, kBudget));
-      if (!ok) break;
-      put(it, kw, ksc);
-      done(it++);
-      mask = place(off, soff);
+      uint32_t mask = place(off, soff);
       fetch(a.c.k, off, mask, kw);
-      ksc = (mask >> lane) & 1u ? a.c.ks[soff] : 0.0f;
-      ok = __all_sync(0xffffffffu, room(it));
-      if (!ok) break;
-      put(it, vw, vsc);
-      done(it++);
+      float ksc = (mask >> lane) & 1u ? a.c.ks[soff] : 0.0f;
+      for (uint32_t j = t.b0; ok && j < t.b1; ++j) {
+        fetch(a.c.v, off, mask, vw);
+        const float vsc = (mask >> lane) & 1u ? a.c.vs[soff] : 0.0f;
+        look_ahead(j + 1u);
+        const uint32_t buf = (it >> 1) & 1u;
+        bool free = room(it);
+        for (uint32_t s = 0; s < 2u; ++s) {
+          uint32_t &n = used[s][buf];
+          if (n) free = free && tc_wait(&S->scales_free[s][buf], (n - 1u) & 1u, failed, kBudget);
+          if (s < slots) ++n;
+        }
+        ok = __all_sync(0xffffffffu, free);
+        if (!ok) break;
+        put(it, kw, ksc);
+        done(it++);
+        mask = place(off, soff);
+        fetch(a.c.k, off, mask, kw);
+        ksc = (mask >> lane) & 1u ? a.c.ks[soff] : 0.0f;
+        ok = __all_sync(0xffffffffu, room(it));
+        if (!ok) break;
+        put(it, vw, vsc);
+        done(it++);
+        if (!q_there) q_to_all();
+      }
     }
   }
+  cp_async_wait_all();
   // the products have read what was filled last, and their arrivals on the ring's barriers are in
-  if (ok && tid == 0u) tc_drain(S->empty, NS, it, failed, kBudget);
+  if (ok && tid == 0u) {
+    tc_drain(S->empty, NS, it, failed, kBudget);
+    tc_wait(&S->q_free, (turn & 1u) ^ 1u, failed, kBudget);
+  }
 }
 
 // ---- the issuing warp -----------------------------------------------------------------------
 template <bool F16, int HD>
-static __device__ __forceinline__ void chunk_products(uint32_t blocks, uint32_t slots, uint8_t *sm, ChunkShared *S) {
+static __device__ __forceinline__ void chunk_products(uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<HD>;
   constexpr uint32_t NS = Sh::kStages;
   volatile uint32_t *failed = &S->failed;
@@ -309,63 +452,74 @@ static __device__ __forceinline__ void chunk_products(uint32_t blocks, uint32_t 
     if (leader) tc_commit(&S->empty[st]);
     __syncwarp();
   };
-  uint32_t it = 0;
-  bool ok = tc_wait_uniform(&S->q_full, 0u, failed, kBudget) && tc_wait_uniform(&S->full[0], 0u, failed, kBudget);
-  if (!ok) return;
-  tc_fence_after_sync();
-  for (uint32_t s = 0; s < slots; ++s) scores(s, 0u);
-  release(0u);
-  ++it;
-  for (uint32_t j = 0; j < blocks; ++j) {
-    const uint32_t sv = it % NS, pv = (it / NS) & 1u, sk = (it + 1u) % NS, pk = ((it + 1u) / NS) & 1u;
-    const bool more = j + 1u < blocks;
-    ok = tc_wait_uniform(&S->full[sv], pv, failed, kBudget);
-    for (uint32_t s = 0; ok && s < slots; ++s) {
-      ok = tc_wait_uniform(&S->p_full[s], j & 1u, failed, kBudget);
-      if (!ok) break;
-      tc_fence_after_sync();
-      values(s, sv, j == 0u);
-      if (s + 1u == slots) release(sv);
-      if (more) {
-        if (s == 0u) ok = tc_wait_uniform(&S->full[sk], pk, failed, kBudget);
-        if (!ok) break;
+  auto full = [&](uint32_t i) { return tc_wait_uniform(&S->full[i % NS], (i / NS) & 1u, failed, kBudget); };
+  uint32_t it = 0, n[2] = {0u, 0u};                       // the ring's blocks; each slot's blocks
+  for (uint32_t turn = 0;; ++turn) {
+    if (!tc_wait_uniform(&S->q_full, turn & 1u, failed, kBudget)) return;
+    const uint32_t rows = *const_cast<volatile uint32_t *>(&S->tile.rows);
+    const uint32_t blocks = *const_cast<volatile uint32_t *>(&S->tile.b1) - *const_cast<volatile uint32_t *>(&S->tile.b0);
+    if (rows == 0u) return;
+    const uint32_t slots = rows > kCkRows ? 2u : 1u;
+    if (!full(it)) return;
+    tc_fence_after_sync();
+    for (uint32_t s = 0; s < slots; ++s) scores(s, it % NS);
+    release(it % NS);
+    for (uint32_t j = 0; j < blocks; ++j, it += 2u) {
+      const bool more = j + 1u < blocks;
+      if (!more && leader) tc_commit(&S->q_free);         // (all of the tile's scores are on their way)
+      __syncwarp();
+      if (!full(it + 1u)) return;
+      for (uint32_t s = 0; s < slots; ++s) {
+        if (!tc_wait_uniform(&S->p_full[s], n[s] & 1u, failed, kBudget)) return;
+        ++n[s];
         tc_fence_after_sync();
-        scores(s, sk);
-        if (s + 1u == slots) release(sk);
-      } else {
-        if (leader) tc_commit(&S->pv_done[s]);
-        __syncwarp();
+        values(s, (it + 1u) % NS, j == 0u);
+        if (s + 1u == slots) release((it + 1u) % NS);
+        if (more) {
+          if (s == 0u && !full(it + 2u)) return;
+          tc_fence_after_sync();
+          scores(s, (it + 2u) % NS);
+          if (s + 1u == slots) release((it + 2u) % NS);
+        } else {
+          if (leader) tc_commit(&S->pv_done[s]);
+          __syncwarp();
+        }
       }
     }
-    if (!ok) return;
-    it += 2u;
   }
 }
 
 // ---- the softmax warps ----------------------------------------------------------------------
-// One block's scores of a row: their maximum and, for 8-bit pages, the largest scale among the keys that the row sees.
 template <bool BF, bool Q8, int HD>
-static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, const Tile &t, const Work &wk, uint32_t b0, uint32_t b1, uint8_t *sm, ChunkShared *S) {
+static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<HD>;
   constexpr uint32_t NS = Sh::kStages;
   volatile uint32_t *failed = &S->failed;
   const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u, s = w >> 2, q4 = w & 3u;
-  if (s * kCkRows >= t.rows) return;
   const uint32_t r = s * kCkRows + 32u * q4 + lane;
-  const bool has = r < t.rows;
-  const uint32_t pr = t.r0 + r, tok = pr / a.group, head = wk.head * a.group + (pr - tok * a.group);
-  Span sp = has ? SeenBy(t.s, static_cast<int32_t>(tok), a.causal, a.window) : Span{0, 0};
   const uint32_t s_addr = S->tmem + ((32u * q4) << 16) + s * 128u, o_addr = S->tmem + ((32u * q4) << 16) + 256u + s * HD;
-  float sl2 = a.scale_log2;
-  if (Q8 && BF) {
-    if (!tc_wait_uniform(&S->q_full, 0u, failed, kBudget)) return;
-    sl2 *= __uint_as_float(static_cast<uint32_t>(127 - S->q_exp[r]) << 23);
-  }
-  float m_used = -INFINITY, l = 0.0f, v_ref = 0.0f;
-  uint32_t it = 0;                                        // the ring's blocks: K of block j is 2 j, V 2 j + 1
+  uint32_t it = 0, n = 0, mine = 0;                       // the ring's blocks: K of a block, V behind it; the slot's blocks and tiles
 #pragma unroll 1
-  for (uint32_t j = b0; j < b1; ++j, it += 2u) {
-    if (!tc_wait_uniform(&S->s_full[s], (j - b0) & 1u, failed, kBudget)) return;
+  for (uint32_t turn = 0;; ++turn) {
+  if (!tc_wait_uniform(&S->q_full, turn & 1u, failed, kBudget)) return;
+  const Tile t = S->tile;
+  const int32_t e = Q8 && BF ? S->q_exp[r] : 0;
+  __syncwarp();
+  if (lane == 0u) mbar_arrive(&S->q_free);
+  if (t.rows == 0u) return;
+  if (s * kCkRows >= t.rows) {                            // the other slot's alone
+    it += 2u * (t.b1 - t.b0);
+    continue;
+  }
+  const bool has = r < t.rows;
+  const uint32_t pr = t.r0 + r, tok = a.by_group.quot(pr), head = t.head * a.group + (pr - tok * a.group);
+  const Span sp = has ? SeenBy(t.s, static_cast<int32_t>(tok), a.causal, a.window) : Span{0, 0};
+  const float sl2 = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  const uint32_t b0 = t.b0, b1 = t.b1;
+  float m_used = -INFINITY, l = 0.0f, v_ref = 0.0f;
+#pragma unroll 1
+  for (uint32_t j = b0; j < b1; ++j, it += 2u, ++n) {
+    if (!tc_wait_uniform(&S->s_full[s], n & 1u, failed, kBudget)) return;
     const float *ks = reinterpret_cast<const float *>(sm + Sh::kScales + (it & 3u) * 512u);
     const float *vs = ks + 128;
     if (Q8 && !tc_wait_uniform(&S->full[(it + 1u) % NS], ((it + 1u) / NS) & 1u, failed, kBudget)) return;      // (the values' scales)
@@ -466,22 +620,23 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, const Til
     __syncwarp();
     if (lane == 0u) {
       mbar_arrive(&S->p_full[s]);
-      if (Q8) mbar_arrive(&S->scales_free[(j - b0) & 1u]);
+      if (Q8) mbar_arrive(&S->scales_free[s][(it >> 1) & 1u]);
     }
     float a0, a1;
     unpack_f32x2(add_f32x2(sum[0], sum[1]), a0, a1);
     l += a0 + a1;
   }
   // ---- the result ----
-  if (!tc_wait_uniform(&S->pv_done[s], 0u, failed, kBudget)) return;
+  if (!tc_wait_uniform(&S->pv_done[s], mine & 1u, failed, kBudget)) return;
+  ++mine;
   tc_fence_after_sync();
-  const bool split = a.splits > 1u;
-  float *part = a.part + static_cast<size_t>(wk.item * a.splits + wk.split) * (kChunkRows * (HD + 2u));
+  const bool split = t.part != 0u;
+  float *part = a.part + static_cast<size_t>(split ? t.part - 1u : 0u) * (kChunkRows * (HD + 2u));
   const bool none = m_used == -INFINITY && l == 0.0f;
   float mul = split ? 1.0f : none ? 0.0f : 1.0f / l;
   if (Q8) mul *= v_ref * (1.0f / kCkPScale);
   uint8_t *out = has ? row_at(a.o, t.s.first + static_cast<int32_t>(tok), head) : a.o.p;
-  const bool vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0u;
+  const bool vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0u, wide = (reinterpret_cast<uintptr_t>(out) & 31u) == 0u;
   bool fine = true;
 #pragma unroll 1
   for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
@@ -498,7 +653,15 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, const Til
     }
     if (split) {
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4 *>(part + r * HD + c0 + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      for (int i = 0; i < 32; i += 8) stg_v8(part + r * HD + c0 + i, x + i);
+      continue;
+    }
+    if (wide) {                                           // whole sectors: a row is 32-byte aligned, and so is its end
+      uint32_t h[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) h[e] = BF ? cvt_bf16x2(__uint_as_float(x[2 * e + 1]), __uint_as_float(x[2 * e])) : cvt_f16x2(__uint_as_float(x[2 * e + 1]), __uint_as_float(x[2 * e]));
+      if (c0 < a.c.hd) stg_v8(out + 2u * c0, h);
+      if (c0 + 16u < a.c.hd) stg_v8(out + 2u * c0 + 32u, h + 8);
       continue;
     }
 #pragma unroll
@@ -523,23 +686,19 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, const Til
     }
   }
   tc_fence_before_sync();
-  if (!has) return;
-  if (split) {
+  bool redo = false;
+  if (has && split) {
     part[kChunkRows * HD + r] = m_used;
     part[kChunkRows * HD + kChunkRows + r] = l;
-  } else {
+  } else if (has) {
     if (a.lse) a.lse[static_cast<int64_t>(t.s.first + static_cast<int32_t>(tok)) * a.q_heads + head] = (m_used + log2f(l)) * 0.69314718055994531f;
-    if (!fine && (sp.lo > t.keys.lo || sp.hi < t.keys.hi)) atomicOr(&S->redo[r >> 5], 1u << (r & 31u));
+    redo = !fine && (sp.lo > t.keys.lo || sp.hi < t.keys.hi);
   }
-}
-
-// Rows that see nothing of the cache.
-__device__ __forceinline__ void clear_rows(const AttendArgs &a, const Tile &t, uint32_t head, uint32_t threads) {
-  for (uint32_t i = threadIdx.x; i < t.rows * a.c.hd; i += threads) {
-    const uint32_t r = i / a.c.hd, d = i - r * a.c.hd, pr = t.r0 + r, tok = pr / a.group, h = head * a.group + (pr - tok * a.group);
-    const int32_t row = t.s.first + static_cast<int32_t>(tok);
-    store_row_value(row_at(a.o, row, h) + 2u * d, 0.0f, a.bf16 != 0u);
-    if (d == 0u && a.lse) a.lse[static_cast<int64_t>(row) * a.q_heads + h] = -INFINITY;
+  for (uint32_t again = __ballot_sync(0xffffffffu, redo); again; again &= again - 1u) {      // (rows of this warp, one after another)
+    const uint32_t k = __ffs(again) - 1u, q = t.r0 + s * kCkRows + 32u * q4 + k;
+    __syncwarp();
+    attend_row_alone(a, t.seq, t.s, static_cast<int32_t>(q / a.group), t.head * a.group + q % a.group);
+  }
   }
 }
 
@@ -556,24 +715,29 @@ __global__ void __launch_bounds__(kCkThreads, 1) b2_attend_chunk(const __grid_co
       if (q.bad) cache_fault(a.c.status, kStBadBatch, i, static_cast<uint32_t>(q.bad), static_cast<uint32_t>(q.value));
     }
   }
-  const Work wk = work_of(a, blockIdx.x, a.splits);
+  u64 all = 0ull;
+  for (uint32_t i = tid; i < a.b.n_seqs; i += kCkThreads) all += units_of_seq(a, cap, i);
+  all = warp_reduce(all, [](u64 x, u64 y) { return x + y; });
+  if ((tid & 31u) == 0u) S->find[w] = all;
+  __syncthreads();
+  all = 0ull;
+  for (uint32_t i = 0; i < kCkThreads / 32u; ++i) all += S->find[i];
+  const uint32_t ctas = ctas_of(a, all, gridDim.x);
+  if (all == 0ull || blockIdx.x >= ctas) return;
+  const Runs runs(all, ctas);
+  const u64 x0 = runs.begin(blockIdx.x), x1 = runs.begin(blockIdx.x + 1u);
   uint32_t seq;
-  unsigned long long before;
-  if (!find_unit<kCkThreads>(a.b.n_seqs, wk.tile, S->find, [&](uint32_t i) { return tiles_of_seq(a, cap, i); }, seq, before)) return;
-  const Tile t = make_tile(a, cap, seq, static_cast<uint32_t>(wk.tile - before));
-  if (t.blocks == 0u) {
-    if (wk.split == 0u) clear_rows(a, t, wk.head, kCkThreads);
-    return;
-  }
-  uint32_t b0, b1, used;
-  split_of(t.blocks, a.splits, wk.split, b0, b1, used);
-  if (b0 >= b1) return;
+  u64 before;
+  if (!find_unit<kCkThreads>(a.b.n_seqs, x0, S->find, [&](uint32_t i) { return units_of_seq(a, cap, i); }, seq, before)) return;
   if (tid == 0u) {
     mbar_init(&S->q_full, kLoadWarps * 32u);
+    mbar_init(&S->q_free, 1u + kSoftWarps);
     for (uint32_t i = 0; i < Sh::kStages; ++i) { mbar_init(&S->full[i], kLoadWarps * 32u); mbar_init(&S->empty[i], 1u); }
-    for (uint32_t s = 0; s < 2u; ++s) { mbar_init(&S->s_full[s], 1u); mbar_init(&S->p_full[s], 4u); mbar_init(&S->pv_done[s], 1u); mbar_init(&S->scales_free[s], t.rows > kCkRows ? 8u : 4u); }
+    for (uint32_t s = 0; s < 2u; ++s) {
+      mbar_init(&S->s_full[s], 1u); mbar_init(&S->p_full[s], 4u); mbar_init(&S->pv_done[s], 1u);
+      for (uint32_t i = 0; i < 2u; ++i) mbar_init(&S->scales_free[s][i], 4u);
+    }
     S->failed = 0u;
-    for (uint32_t i = 0; i < 8u; ++i) S->redo[i] = 0u;
     fence_mbar_init();
   }
   if (w == kSoftWarps + kLoadWarps) {
@@ -584,14 +748,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) b2_attend_chunk(const __grid_co
   __syncthreads();
   tc_fence_after_sync();
   if (w < kSoftWarps) {
-    more_registers<kSoftRegs>();
-    chunk_rows<BF, Q8, HD>(a, t, wk, b0, b1, sm, S);
+    more_registers<Q8 ? kSoftRegs8 : kSoftRegs>();
+    chunk_rows<BF, Q8, HD>(a, sm, S);
   } else if (w < kSoftWarps + kLoadWarps) {
-    fewer_registers<kLoadRegs>();
-    chunk_load<BF, Q8, HD>(a, t, wk.head, b0, b1, sm, S);
+    fewer_registers<Q8 ? kLoadRegs8 : kLoadRegs>();
+    Walk wk;
+    wk.seek(a, cap, seq, before, x0);
+    chunk_load<BF, Q8, HD>(a, wk, x0, x1, sm, S);
   } else {
     fewer_registers<kIssueRegs>();
-    if (w == kSoftWarps + kLoadWarps) chunk_products<Q8 || !BF, HD>(b1 - b0, t.rows > kCkRows ? 2u : 1u, sm, S);
+    if (w == kSoftWarps + kLoadWarps) chunk_products<Q8 || !BF, HD>(sm, S);
   }
   __syncwarp();
   tc_fence_before_sync();
@@ -600,53 +766,89 @@ __global__ void __launch_bounds__(kCkThreads, 1) b2_attend_chunk(const __grid_co
   if (gave_up) {                                          // products of other roles may still be landing: give them time
     const unsigned long long t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 50000ull) nanosleep_ns(1000);
-    if (tid == 0u) cache_fault(a.c.status, kStTcTimeout, t.seq, wk.tile, 0u);
+    if (tid == 0u) cache_fault(a.c.status, kStTcTimeout, seq, blockIdx.x, 0u);
   }
   if (w == kSoftWarps + kLoadWarps) {
     __syncwarp();
     tc_fence_after_sync();
     tmem_dealloc(S->tmem, kCkCols);
   }
-  if (gave_up || a.splits > 1u) return;
-  for (uint32_t r = w; r < t.rows; r += kCkThreads / 32u)
-    if ((S->redo[r >> 5] >> (r & 31u)) & 1u) attend_row_alone(a, t.seq, t.s, static_cast<int32_t>((t.r0 + r) / a.group), wk.head * a.group + (t.r0 + r) % a.group);
 }
 
-// Tiles whose keys were split: a warp to a row, the parts in their order.
-constexpr uint32_t kJoinThreads = 256, kJoinRows = 32;    // rows of a CTA
+// Tiles that lie in the runs of several CTAs: a warp to a row, the parts in their order. A CTA for each border between two runs (and 32 rows): it has
+// something to do if the border lies between two blocks of a tile, and is the tile's first that does.
+constexpr uint32_t kJoinThreads = 256, kJoinRows = 32, kMostRuns = 1024;
 template <int HD>
-__global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_constant__ AttendArgs a) {
-  __shared__ unsigned long long find[kJoinThreads / 32 + 2];
+__global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_constant__ AttendArgs a, uint32_t most) {
+  __shared__ u64 find[kJoinThreads / 32 + 2];
   const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint64_t cap = capacity_of(a.c, a.b);
-  const Work wk = work_of(a, blockIdx.x / (kChunkRows / kJoinRows), 1u);
+  u64 all = 0ull;
+  for (uint32_t i = threadIdx.x; i < a.b.n_seqs; i += kJoinThreads) all += units_of_seq(a, cap, i);
+  all = warp_reduce(all, [](u64 x, u64 y) { return x + y; });
+  if (lane == 0u) find[w] = all;
+  __syncthreads();
+  all = 0ull;
+  for (uint32_t i = 0; i < kJoinThreads / 32u; ++i) all += find[i];
+  const uint32_t ctas = ctas_of(a, all, most), border = 1u + blockIdx.x / (kChunkRows / kJoinRows);
+  if (all == 0ull || border >= ctas) return;
+  const Runs runs(all, ctas);
+  const u64 x = runs.begin(border), x_before = runs.begin(border - 1u);
   uint32_t seq;
-  unsigned long long before;
-  if (!find_unit<kJoinThreads>(a.b.n_seqs, wk.tile, find, [&](uint32_t i) { return tiles_of_seq(a, cap, i); }, seq, before)) return;
-  const Tile t = make_tile(a, cap, seq, static_cast<uint32_t>(wk.tile - before));
-  uint32_t b0, b1, used;
-  split_of(t.blocks, a.splits, 0u, b0, b1, used);
-  if (used == 0u) return;                                 // (rows without keys are cleared already)
-  const uint32_t first = (blockIdx.x % (kChunkRows / kJoinRows)) * kJoinRows;
-  const float *part = a.part + static_cast<size_t>(wk.item) * a.splits * (kChunkRows * (HD + 2u));
-  for (uint32_t r = first + w; r < min(t.rows, first + kJoinRows); r += kJoinThreads / 32u) {
-    const uint32_t pr = t.r0 + r, tok = pr / a.group, head = wk.head * a.group + (pr - tok * a.group), d = lane * (HD / 32);
-    const int32_t row = t.s.first + static_cast<int32_t>(tok);
-    float mm = -INFINITY, ll = 0.0f, x[HD / 32] = {};
-    for (uint32_t k = 0; k < used; ++k) mm = fmaxf(mm, part[static_cast<size_t>(k) * (kChunkRows * (HD + 2u)) + kChunkRows * HD + r]);
-#pragma unroll 4
-    for (uint32_t k = 0; k < used; ++k) {
-      const float *p = part + static_cast<size_t>(k) * (kChunkRows * (HD + 2u));
-      const float mk = p[kChunkRows * HD + r], f = mk == mm ? 1.0f : fast_ex2(mk - mm);
-      ll += p[kChunkRows * HD + kChunkRows + r] * f;
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) x[i] += p[r * HD + d + i] * f;
+  u64 before;
+  if (!find_unit<kJoinThreads>(a.b.n_seqs, x, find, [&](uint32_t i) { return units_of_seq(a, cap, i); }, seq, before)) return;
+  Walk wk;
+  wk.seek(a, cap, seq, before, x);
+  Tile t;
+  wk.tile(a, x_before, x, t);
+  if (t.b0 != 0u || t.b1 == 0u || t.b1 == t.blocks) return;
+  // the parts: CTAs from `border` - 1 on whose runs have blocks of the tile, the first of them from block 0
+  constexpr uint32_t kPart = kChunkRows * (HD + 2u);
+  __shared__ uint32_t part_s[kMostRuns], n_parts;
+  if (threadIdx.x == 0u) n_parts = 0u;
+  __syncthreads();
+  if (w == 0u) {
+    uint32_t n = 0u;
+    for (uint32_t c0 = border - 1u; c0 < ctas; c0 += 32u) {
+      const uint32_t c = c0 + lane;
+      const uint32_t lo = c < ctas ? wk.block_at(t.blocks, runs.begin(c)) : t.blocks, hi = c < ctas ? wk.block_at(t.blocks, runs.begin(c + 1u)) : t.blocks;
+      const uint32_t m = __ballot_sync(0xffffffffu, lo < hi);
+      if (lo < hi) part_s[n + __popc(m & ((1u << lane) - 1u))] = c * 2u + (lo == 0u ? 1u : 0u);
+      n += __popc(m);
+      if (__any_sync(0xffffffffu, hi == t.blocks)) break;
     }
+    if (lane == 0u) n_parts = n;
+  }
+  __syncthreads();
+  const uint32_t parts = n_parts, first = (blockIdx.x % (kChunkRows / kJoinRows)) * kJoinRows;
+  for (uint32_t r = first + w; r < min(t.rows, first + kJoinRows); r += kJoinThreads / 32u) {
+    const uint32_t pr = t.r0 + r, tok = a.by_group.quot(pr), head = t.head * a.group + (pr - tok * a.group), d = lane * (HD / 32);
+    const int32_t row = t.s.first + static_cast<int32_t>(tok);
+    float mm = -INFINITY, ll = 0.0f, o[HD / 32] = {};
+    for (uint32_t k = lane; k < parts; k += 32u) mm = fmaxf(mm, a.part[static_cast<size_t>(part_s[k]) * kPart + kChunkRows * HD + r]);
+    mm = warp_reduce(mm, [](float u, float v) { return fmaxf(u, v); });
+    for (uint32_t k0 = 0; k0 < parts; k0 += 32u) {
+      float f = 0.0f;
+      if (k0 + lane < parts) {
+        const float *p = a.part + static_cast<size_t>(part_s[k0 + lane]) * kPart + kChunkRows * HD + r;
+        f = p[0] == mm ? 1.0f : fast_ex2(p[0] - mm);
+        ll += p[kChunkRows] * f;
+      }
+      const uint32_t n = min(32u, parts - k0);
+#pragma unroll 4
+      for (uint32_t k = 0; k < n; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        const float *p = a.part + static_cast<size_t>(part_s[k0 + k]) * kPart + r * HD + d;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) o[i] += p[i] * fk;
+      }
+    }
+    ll = warp_reduce(ll, [](float u, float v) { return u + v; });
     const float inv = mm == -INFINITY && ll == 0.0f ? 0.0f : 1.0f / ll;
     bool fine = true;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
-      const float v = x[i] * inv;
+      const float v = o[i] * inv;
       fine = fine && isfinite(v);
       if (d + i < a.c.hd) store_row_value(row_at(a.o, row, head) + 2u * (d + i), v, a.bf16 != 0u);
     }
@@ -660,10 +862,10 @@ __global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_cons
 }
 
 template <bool BF, bool Q8, int HD>
-int Launch(const AttendArgs &a, cudaStream_t stream) {
-  const uint32_t items = a.tiles * a.c.heads;
-  b2_attend_chunk<BF, Q8, HD><<<items * a.splits, kCkThreads, ChunkSmem<HD>(), stream>>>(a);
-  if (a.splits > 1u) b2_attend_join<HD><<<items * (kChunkRows / kJoinRows), kJoinThreads, 0, stream>>>(a);
+int Launch(const AttendArgs &a, uint32_t sms, cudaStream_t stream) {
+  if (sms > kMostRuns) sms = kMostRuns;
+  b2_attend_chunk<BF, Q8, HD><<<sms, kCkThreads, ChunkSmem<HD>(), stream>>>(a);
+  if (sms > 1u) b2_attend_join<HD><<<(sms - 1u) * (kChunkRows / kJoinRows), kJoinThreads, 0, stream>>>(a, sms);
   return static_cast<int>(cudaGetLastError());
 }
 template <bool BF, bool Q8, int HD>
@@ -679,17 +881,17 @@ int PrepareAttendChunk() {
     if (e != cudaSuccess) return static_cast<int>(e);
   return 0;
 }
-size_t AttendChunkPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * kChunkRows * (128u + 2u) * sizeof(float); }
+size_t AttendChunkPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * 2u * kChunkRows * (128u + 2u) * sizeof(float); }
 
-int LaunchAttendChunk(const AttendArgs &a, CUstream_st *stream) {
+int LaunchAttendChunk(const AttendArgs &a, uint32_t sms, CUstream_st *stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool big = a.c.hd > 64u;
   if (a.e4m3) {
-    if (a.bf16) return big ? Launch<true, true, 128>(a, s) : Launch<true, true, 64>(a, s);
-    return big ? Launch<false, true, 128>(a, s) : Launch<false, true, 64>(a, s);
+    if (a.bf16) return big ? Launch<true, true, 128>(a, sms, s) : Launch<true, true, 64>(a, sms, s);
+    return big ? Launch<false, true, 128>(a, sms, s) : Launch<false, true, 64>(a, sms, s);
   }
-  if (a.bf16) return big ? Launch<true, false, 128>(a, s) : Launch<true, false, 64>(a, s);
-  return big ? Launch<false, false, 128>(a, s) : Launch<false, false, 64>(a, s);
+  if (a.bf16) return big ? Launch<true, false, 128>(a, sms, s) : Launch<true, false, 64>(a, sms, s);
+  return big ? Launch<false, false, 128>(a, sms, s) : Launch<false, false, 64>(a, sms, s);
 }
 
 }  // namespace b2

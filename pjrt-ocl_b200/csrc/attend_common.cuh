@@ -10,6 +10,11 @@ namespace b2 {
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// 32 bytes at once, 32-byte aligned.
+__device__ __forceinline__ void stg_v8(void *p, const uint32_t *w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
 // Two e4m3 values as two f16 (exact).
 __device__ __forceinline__ uint32_t cvt_e4m3x2_f16x2(uint32_t lo16) {
   uint32_t r;

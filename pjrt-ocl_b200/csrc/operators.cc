@@ -198,6 +198,7 @@ b2_status b2_rope_create(b2_runtime *rt, const b2_rope_desc *desc, b2_rope **out
     for (uint32_t i = 0; i < desc->rot_dim / 2; ++i) turns[i] = desc->frequencies[i] / (2.0 * 3.14159265358979323846);
     OnDevice on(r.device);
     cudaError_t e = on.error();
+    if (e == cudaSuccess) e = static_cast<cudaError_t>(b2::PrepareRope());
     if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&r.turns), sizeof turns);
     if (e != cudaSuccess) return CudaFail(err, err_cap, name, e, B2_RESOURCE_EXHAUSTED);
     e = cudaMemcpy(r.turns, turns, sizeof(double) * (desc->rot_dim / 2), cudaMemcpyHostToDevice);
@@ -359,6 +360,7 @@ b2_status b2_cache_attend(b2_cache *cache, b2_scratch *scratch, const b2_batch *
     a.scale_log2 = scale * 1.4426950408889634f;
     a.q_heads = d.q_heads;
     a.group = d.q_heads / d.heads;
+    a.by_group = b2::FastDiv(a.group);
     a.causal = causal ? 1u : 0u;
     a.window = window;
     a.bf16 = d.row_dtype == B2_BF16 ? 1u : 0u;
@@ -371,13 +373,7 @@ b2_status b2_cache_attend(b2_cache *cache, b2_scratch *scratch, const b2_batch *
       if (static_cast<uint64_t>(a.b.max_rows) * a.group <= b2::kStepRows) {
         e = static_cast<cudaError_t>(b2::LaunchAttendStep(a, cache->sms, static_cast<cudaStream_t>(cuda_stream)));
       } else {
-        // tiles: every sequence ends in one that is not full
-        const uint64_t tiles = static_cast<uint64_t>(a.b.n_rows) * a.group / b2::kChunkRows + a.b.n_seqs;
-        if (tiles * d.heads > 0x3fffffffull) return Refuse(name, err, err_cap, "more than 2^30 tiles of rows");
-        a.tiles = static_cast<uint32_t>(tiles);
-        const uint64_t items = tiles * d.heads;
-        a.splits = items >= cache->sms ? 1u : static_cast<uint32_t>(cache->sms / items);
-        e = static_cast<cudaError_t>(b2::LaunchAttendChunk(a, static_cast<cudaStream_t>(cuda_stream)));
+        e = static_cast<cudaError_t>(b2::LaunchAttendChunk(a, cache->sms, static_cast<cudaStream_t>(cuda_stream)));
       }
     }
     return e == cudaSuccess ? B2_OK : CudaFail(err, err_cap, name, e);

@@ -90,11 +90,11 @@ struct AttendArgs {
   BatchView b;
   RowsRef q, o;
   float *lse;
-  float *part;                     // partial results of keys that were split over CTAs
+  float *part;                     // results of parts of a tile's keys
   uint32_t *arrived;               // counters, zero at rest
   float scale_log2;                // softmax scale x log2(e)
   uint32_t q_heads, group, causal, window;
-  uint32_t splits, tiles;          // attend_chunk: CTAs to a tile of rows, tiles of rows of the batch (a bound)
+  FastDiv by_group;
   uint32_t bf16;                   // type of the rows
   uint32_t e4m3;
 };
@@ -133,13 +133,14 @@ std::string CheckRows(const char *what, const b2_rows *r, uint32_t n_rows, uint3
 std::string CheckAttend(const b2_cache_desc &d, const b2_batch *b, const b2_rows *q, const b2_rows *o, float scale, int causal, uint32_t window, const void *lse);
 
 // ---- launches; each returns a cudaError_t's value ----
+int PrepareRope();                        // shared-memory attributes on the current device
 int LaunchRope(const RopeArgs &a, uint32_t dtype, bool backward, uint32_t sms, CUstream_st *stream);
 uint32_t RopeBackwardCtas(uint32_t sms);
 int LaunchCacheMove(const CacheView &c, const BatchView &b, const RowsRef &k, const RowsRef &v, uint32_t dtype, uint32_t row_dtype, bool write, uint32_t sms, CUstream_st *stream);
-int PrepareAttendStep();                  // shared-memory attributes on the current device
+int PrepareAttendStep();                  // (as PrepareRope)
 int PrepareAttendChunk();
 int LaunchAttendStep(const AttendArgs &a, uint32_t sms, CUstream_st *stream);
-int LaunchAttendChunk(const AttendArgs &a, CUstream_st *stream);
+int LaunchAttendChunk(const AttendArgs &a, uint32_t sms, CUstream_st *stream);
 size_t AttendStepPartialBytes(uint32_t sms);
 size_t AttendChunkPartialBytes(uint32_t sms);
 

@@ -407,10 +407,6 @@ int Launch(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
   smem = (smem + 15u) & ~size_t(15);
   s.ring_at = static_cast<uint32_t>(smem);
   if (V * sizeof(T) == 16) smem += kRopeWarps * kRing * (BACK ? 2u : 1u) * 2u * U * 512u;       // 107 KB at most in all
-  if (smem > 48u * 1024u) {
-    const cudaError_t e = cudaFuncSetAttribute(b2_rope<T, V, U, BACK>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return static_cast<int>(e);
-  }
   b2_rope<T, V, U, BACK><<<ctas, kRopeThreads, smem, stream>>>(a, s);
   if (BACK && a.partial) b2_rope_weights<<<(2u * a.hd + 31u) / 32u, kSumWarps * 32u, 0, stream>>>(a, ctas);
   return static_cast<int>(cudaGetLastError());
@@ -446,6 +442,19 @@ int Dispatch(const RopeArgs &a, uint32_t sms, cudaStream_t stream) {
 
 }  // namespace
 
+namespace {
+constexpr int kRopeSmem = 110 * 1024;                     // more than any shape takes
+template <typename T, int V, int U>
+cudaError_t Attr() {
+  const cudaError_t e = cudaFuncSetAttribute(b2_rope<T, V, U, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRopeSmem);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(b2_rope<T, V, U, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRopeSmem);
+}
+}  // namespace
+int PrepareRope() {
+  for (cudaError_t e : {Attr<float, 4, 1>(), Attr<__half, 8, 1>(), Attr<__nv_bfloat16, 8, 1>()})
+    if (e != cudaSuccess) return static_cast<int>(e);
+  return 0;
+}
 uint32_t RopeBackwardCtas(uint32_t sms) { return kRopeBackPerSm * sms; }
 
 int LaunchRope(const RopeArgs &a, uint32_t dtype, bool backward, uint32_t sms, CUstream_st *stream) {

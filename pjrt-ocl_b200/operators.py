@@ -8,6 +8,7 @@ device) and not waited for; a refusal raises the same errors as the rest of the 
 from __future__ import annotations
 
 import ctypes
+import threading
 
 from .runtime import _ERRCAP, InvalidArgument, Runtime, _check, _errbuf, _ExecStatus, lib
 
@@ -40,6 +41,16 @@ class _BatchC(ctypes.Structure):
                 ("row_start", _vp), ("length", _vp), ("pages", _vp)]
 
 
+class _Local(threading.local):
+    """A thread's buffer for messages: what a call writes there is read before the thread makes another."""
+
+    def __init__(self):
+        self.err = _errbuf()
+
+
+_local = _Local()
+
+
 def _dtype(name: str) -> int:
     if name not in DTYPES:
         raise InvalidArgument(f"unknown type {name!r} (one of {', '.join(DTYPES)})")
@@ -49,7 +60,7 @@ def _dtype(name: str) -> int:
 class Rows:
     """rows x heads x head_dim on the device, the last axis without gaps; strides in elements (default: no gaps)."""
 
-    __slots__ = ("ptr", "dtype", "shape", "device", "_ref", "_keep")
+    __slots__ = ("ptr", "dtype", "shape", "device", "_ref", "_keep", "_kind")
 
     def __init__(self, ptr: int, dtype: str, shape, strides=None, device=None):
         n, heads, dim = (int(x) for x in shape)
@@ -58,6 +69,7 @@ class Rows:
         self.ptr, self.dtype, self.shape, self.device = int(ptr), dtype, (n, heads, dim), device
         self._keep = _RowsC(self.ptr, strides[0], strides[1])
         self._ref = ctypes.byref(self._keep)
+        self._kind = (dtype, heads, dim)
 
     @staticmethod
     def Of(tensor) -> "Rows":
@@ -75,14 +87,14 @@ class Rows:
         return Rows(tensor.data_ptr(), dt, tensor.shape, tensor.stride()[:2], tensor.device.index)
 
 
-def _rows(what: str, r, device: int, dtype: str, n: int, heads: int, dim: int):
-    """The C struct of rows that fit a call."""
+def _rows(what: str, r, device: int, n: int, kind: tuple):
+    """The C struct of rows that fit a call: (type, heads, head_dim) are `kind`, at least n rows."""
     if r is None:
-        if n and heads:
+        if n and kind[1]:
             raise InvalidArgument(f"{what}: missing")
         return None
-    if r.dtype != dtype or r.shape[0] < n or r.shape[1] != heads or r.shape[2] != dim:
-        raise InvalidArgument(f"{what}: {r.dtype}{list(r.shape)}, want {dtype}[{n} or more, {heads}, {dim}]")
+    if r._kind != kind or r.shape[0] < n:
+        raise InvalidArgument(f"{what}: {r.dtype}{list(r.shape)}, want {kind[0]}[{n} or more, {kind[1]}, {kind[2]}]")
     if r.device is not None and r.device != device:
         raise InvalidArgument(f"{what}: on device {r.device}, the runtime is on {device}")
     return r._ref
@@ -128,8 +140,9 @@ class Rope:
 
     def __init__(self, rt: Runtime, handle, desc: dict):
         self._rt, self._h, self.desc = rt, handle, desc
-        self._dev, self._dt = rt.device_ordinal, desc["dtype"]
-        self._q, self._k, self._d = desc["q_heads"], desc["k_heads"], desc["head_dim"]
+        self._dev = rt.device_ordinal
+        self._q, self._k = ((desc["dtype"], desc[heads], desc["head_dim"]) for heads in ("q_heads", "k_heads"))
+        self._apply, self._back = lib().b2_rope_apply, lib().b2_rope_apply_backward
 
     @staticmethod
     def Create(rt: Runtime, head_dim: int, q_heads: int, k_heads: int, dtype: str, rot_dim=None, frequencies=None, interleaved: bool = False,
@@ -145,22 +158,21 @@ class Rope:
         return Rope(rt, h, {"head_dim": head_dim, "q_heads": q_heads, "k_heads": k_heads, "dtype": dtype, "norm": bool(norm)})
 
     def Apply(self, n_rows: int, positions: int, q, k, q_out, k_out, q_weight: int = 0, k_weight: int = 0, stream: int = 0) -> None:
-        a = (self._dev, self._dt, n_rows)
-        err = _errbuf()
-        st = lib().b2_rope_apply(self._h, n_rows, positions, _rows("q", q, *a, self._q, self._d), _rows("k", k, *a, self._k, self._d), q_weight, k_weight,
-                                 _rows("q_out", q_out, *a, self._q, self._d), _rows("k_out", k_out, *a, self._k, self._d), stream, err, _ERRCAP)
+        dev, qk, kk, err = self._dev, self._q, self._k, _local.err
+        st = self._apply(self._h, n_rows, positions, _rows("q", q, dev, n_rows, qk), _rows("k", k, dev, n_rows, kk), q_weight, k_weight,
+                         _rows("q_out", q_out, dev, n_rows, qk), _rows("k_out", k_out, dev, n_rows, kk), stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
     def ApplyBackward(self, n_rows: int, positions: int, q, k, dq_out, dk_out, dq, dk, q_weight: int = 0, k_weight: int = 0, dq_weight: int = 0, dk_weight: int = 0,
                       scratch: Scratch = None, stream: int = 0) -> None:
         """Gradients; q and k (the inputs of Apply) are needed with norm only, `scratch` for those of the weights."""
-        a = (self._dev, self._dt, n_rows)
-        x = [None if r is None and not self.desc["norm"] else _rows(what, r, *a, heads, self._d) for what, r, heads in (("q", q, self._q), ("k", k, self._k))]
-        err = _errbuf()
-        st = lib().b2_rope_apply_backward(self._h, scratch._h if scratch is not None else None, n_rows, positions, x[0], x[1], q_weight, k_weight,
-                                          _rows("dq_out", dq_out, *a, self._q, self._d), _rows("dk_out", dk_out, *a, self._k, self._d),
-                                          _rows("dq", dq, *a, self._q, self._d), _rows("dk", dk, *a, self._k, self._d), dq_weight, dk_weight, stream, err, _ERRCAP)
+        dev, qk, kk, err = self._dev, self._q, self._k, _local.err
+        norm = self.desc["norm"]
+        x = [None if r is None and not norm else _rows(what, r, dev, n_rows, kind) for what, r, kind in (("q", q, qk), ("k", k, kk))]
+        st = self._back(self._h, scratch._h if scratch is not None else None, n_rows, positions, x[0], x[1], q_weight, k_weight,
+                        _rows("dq_out", dq_out, dev, n_rows, qk), _rows("dk_out", dk_out, dev, n_rows, kk),
+                        _rows("dq", dq, dev, n_rows, qk), _rows("dk", dk, dev, n_rows, kk), dq_weight, dk_weight, stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
@@ -196,8 +208,10 @@ class PagedCache:
 
     def __init__(self, rt: Runtime, handle, desc: dict):
         self._rt, self._h, self.desc = rt, handle, desc
-        self._dev, self._dt = rt.device_ordinal, desc["row_dtype"]
-        self._heads, self._q, self._d = desc["heads"], desc["q_heads"], desc["head_dim"]
+        self._dev = rt.device_ordinal
+        self._kv, self._q = ((desc["row_dtype"], desc[heads], desc["head_dim"]) for heads in ("heads", "q_heads"))
+        self._scale = desc["head_dim"] ** -0.5
+        self._write, self._read, self._attend = lib().b2_cache_write, lib().b2_cache_read, lib().b2_cache_attend
 
     @staticmethod
     def Create(rt: Runtime, dtype: str, row_dtype: str, heads: int, head_dim: int, page_size: int, n_pages: int, k_pages: int, v_pages: int, q_heads=None,
@@ -212,16 +226,14 @@ class PagedCache:
         return PagedCache(rt, h, {"dtype": dtype, "row_dtype": row_dtype, "heads": heads, "q_heads": q_heads, "head_dim": head_dim})
 
     def Write(self, batch: Batch, k: Rows, v: Rows, stream: int = 0) -> None:
-        a = (self._dev, self._dt, batch.n_rows, self._heads, self._d)
-        err = _errbuf()
-        st = lib().b2_cache_write(self._h, batch._ref, _rows("k", k, *a), _rows("v", v, *a), stream, err, _ERRCAP)
+        n, err = batch.n_rows, _local.err
+        st = self._write(self._h, batch._ref, _rows("k", k, self._dev, n, self._kv), _rows("v", v, self._dev, n, self._kv), stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
     def Read(self, batch: Batch, k: Rows, v: Rows, stream: int = 0) -> None:
-        a = (self._dev, self._dt, batch.n_rows, self._heads, self._d)
-        err = _errbuf()
-        st = lib().b2_cache_read(self._h, batch._ref, _rows("k", k, *a), _rows("v", v, *a), stream, err, _ERRCAP)
+        n, err = batch.n_rows, _local.err
+        st = self._read(self._h, batch._ref, _rows("k", k, self._dev, n, self._kv), _rows("v", v, self._dev, n, self._kv), stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
@@ -229,10 +241,9 @@ class PagedCache:
         """`scale` defaults to 1 / sqrt(head_dim); `lse`: device f32 [n_rows][q_heads], or 0."""
         if not 0 <= window <= 0xFFFFFFFF:
             raise InvalidArgument(f"window {window} is out of range")
-        a = (self._dev, self._dt, batch.n_rows, self._q, self._d)
-        err = _errbuf()
-        st = lib().b2_cache_attend(self._h, scratch._h if scratch is not None else None, batch._ref, _rows("q", q, *a), self._d ** -0.5 if scale is None else scale,
-                                   1 if causal else 0, window, _rows("out", out, *a), lse, stream, err, _ERRCAP)
+        n, err = batch.n_rows, _local.err
+        st = self._attend(self._h, scratch._h if scratch is not None else None, batch._ref, _rows("q", q, self._dev, n, self._q), self._scale if scale is None else scale,
+                          1 if causal else 0, window, _rows("out", out, self._dev, n, self._q), lse, stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
