@@ -19,6 +19,8 @@
 // beginning and end, are dealt to the CTAs in equal runs, whatever their number and lengths; a run that ends inside a tile ends between
 // two blocks of its keys, and a second launch joins the parts. The filling warps walk the run; the others read what they need of a tile
 // from shared memory. The ring runs on from tile to tile.
+#include <type_traits>
+
 #include "attend_common.cuh"
 #include "tc_common.cuh"
 
@@ -490,6 +492,32 @@ static __device__ __forceinline__ void chunk_products(uint8_t *sm, ChunkShared *
 }
 
 // ---- the softmax warps ----------------------------------------------------------------------
+// The largest of three; a NaN wins.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two finite values by products: x = n + f with n the nearest whole number (what adding and taking away 1.5 x 2^23 leaves), 2^f by the polynomial of
+// degree 4 whose relative error on [-1/2, 1/2] is least (2.6e-6; fitted by Remez' exchange), n into the exponent. The special-function unit gives 16
+// exponentials a cycle and SM: with it alone 128 x 128 weights take the 1024 cycles that the products of a block of 128 values take, one after
+// the other; of every kPolyOf pairs of weights kPoly come this way.
+constexpr int kPoly = 0, kPolyOf = 2;
+__device__ __forceinline__ void ex2_poly(u64 x, float &e0, float &e1) {
+  float x0, x1;
+  unpack_f32x2(x, x0, x1);
+  x = pack_f32x2(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
+  const u64 y = add_f32x2(x, pack_f32x2(12582912.0f, 12582912.0f)), f = fma_f32x2(add_f32x2(y, pack_f32x2(-12582912.0f, -12582912.0f)), pack_f32x2(-1.0f, -1.0f), x);
+  u64 p = fma_f32x2(f, pack_f32x2(0.009570102207362652f, 0.009570102207362652f), pack_f32x2(0.05591785907745361f, 0.05591785907745361f));
+  p = fma_f32x2(p, f, pack_f32x2(0.240247443318367f, 0.240247443318367f));
+  p = fma_f32x2(p, f, pack_f32x2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma_f32x2(p, f, pack_f32x2(0.9999992847442627f, 0.9999992847442627f));
+  float y0, y1;
+  unpack_f32x2(y, y0, y1);
+  unpack_f32x2(p, e0, e1);
+  e0 = __uint_as_float(__float_as_uint(e0) + (__float_as_uint(y0) << 23));
+  e1 = __uint_as_float(__float_as_uint(e1) + (__float_as_uint(y1) << 23));
+}
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<HD>;
@@ -556,12 +584,14 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
       float m4[4] = {mx, mx, mx, mx};
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        m4[i & 1] = max3(m4[i & 1], __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
-        m4[2 + (i & 1)] = max3(m4[2 + (i & 1)], __uint_as_float(x[2][i]), __uint_as_float(x[3][i]));
+        m4[i & 1] = max3_nan(m4[i & 1], __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
+        m4[2 + (i & 1)] = max3_nan(m4[2 + (i & 1)], __uint_as_float(x[2][i]), __uint_as_float(x[3][i]));
       }
-      mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      mx = max3_nan(m4[0], m4[1], max3_nan(m4[2], m4[3], m4[2]));
     }
     mx *= sl2;
+    // (a NaN, or an infinity, among the scores: every exponential by the special-function unit, which hands it on)
+    const bool plain = whole && __all_sync(0xffffffffu, fabsf(mx) < INFINITY);
     bool grow = mx > m_used + kGrow;
     float alpha = 1.0f, v_mul = 1.0f;
     if (grow) {
@@ -595,26 +625,35 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
     const float neg = m_used == -INFINITY ? 0.0f : -m_used;
     const unsigned long long sl2_2 = pack_f32x2(sl2, sl2), neg_2 = pack_f32x2(neg, neg);
     unsigned long long sum[2] = {0ull, 0ull};
+    auto weights = [&](auto poly) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t pk[16];
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float e0, e1;
-        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), sl2_2, neg_2), e0, e1);
-        e0 = fast_ex2(e0);
-        e1 = fast_ex2(e1);
-        sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
-        if (Q8) {
-          const float2 v2 = *reinterpret_cast<const float2 *>(vs + 32 * c + 2 * i);
-          e0 = e0 == 0.0f ? 0.0f : e0 * (v2.x * v_mul);
-          e1 = e1 == 0.0f ? 0.0f : e1 * (v2.y * v_mul);
+        for (int i = 0; i < 16; ++i) {
+          const u64 x2 = fma_f32x2(pack_f32x2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), sl2_2, neg_2);
+          float e0, e1;
+          if (decltype(poly)::value && (i % kPolyOf) < kPoly) {
+            ex2_poly(x2, e0, e1);
+          } else {
+            unpack_f32x2(x2, e0, e1);
+            e0 = fast_ex2(e0);
+            e1 = fast_ex2(e1);
+          }
+          sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
+          if (Q8) {
+            const float2 v2 = *reinterpret_cast<const float2 *>(vs + 32 * c + 2 * i);
+            e0 = !decltype(poly)::value && e0 == 0.0f ? 0.0f : e0 * (v2.x * v_mul);      // (a scale that the row does not see may be anything)
+            e1 = !decltype(poly)::value && e1 == 0.0f ? 0.0f : e1 * (v2.y * v_mul);
+          }
+          pk[i] = BF && !Q8 ? cvt_bf16x2(e1, e0) : cvt_f16x2(e1, e0);
         }
-        pk[i] = BF && !Q8 ? cvt_bf16x2(e1, e0) : cvt_f16x2(e1, e0);
+        __syncwarp();
+        tc_st16(s_addr + 16u * c, pk);
       }
-      __syncwarp();
-      tc_st16(s_addr + 16u * c, pk);
-    }
+    };
+    if (plain) weights(std::true_type{});
+    else weights(std::false_type{});
     tc_wait_st();
     tc_fence_before_sync();
     __syncwarp();
@@ -821,38 +860,81 @@ __global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_cons
   }
   __syncthreads();
   const uint32_t parts = n_parts, first = (blockIdx.x % (kChunkRows / kJoinRows)) * kJoinRows;
-  for (uint32_t r = first + w; r < min(t.rows, first + kJoinRows); r += kJoinThreads / 32u) {
-    const uint32_t pr = t.r0 + r, tok = a.by_group.quot(pr), head = t.head * a.group + (pr - tok * a.group), d = lane * (HD / 32);
-    const int32_t row = t.s.first + static_cast<int32_t>(tok);
-    float mm = -INFINITY, ll = 0.0f, o[HD / 32] = {};
-    for (uint32_t k = lane; k < parts; k += 32u) mm = fmaxf(mm, a.part[static_cast<size_t>(part_s[k]) * kPart + kChunkRows * HD + r]);
-    mm = warp_reduce(mm, [](float u, float v) { return fmaxf(u, v); });
-    for (uint32_t k0 = 0; k0 < parts; k0 += 32u) {
-      float f = 0.0f;
-      if (k0 + lane < parts) {
-        const float *p = a.part + static_cast<size_t>(part_s[k0 + lane]) * kPart + kChunkRows * HD + r;
-        f = p[0] == mm ? 1.0f : fast_ex2(p[0] - mm);
-        ll += p[kChunkRows] * f;
-      }
-      const uint32_t n = min(32u, parts - k0);
-#pragma unroll 4
-      for (uint32_t k = 0; k < n; ++k) {
-        const float fk = __shfl_sync(0xffffffffu, f, k);
-        const float *p = a.part + static_cast<size_t>(part_s[k0 + k]) * kPart + r * HD + d;
+  // a warp's rows: first + w, + 8, + 16, + 24, side by side
+  constexpr uint32_t kWarps = kJoinThreads / 32u, kRows = kJoinRows / kWarps, V = HD / 32;
+  if (first + w >= t.rows) return;
+  float mm[kRows], ll[kRows], o[kRows][V] = {};
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) o[i] += p[i] * fk;
+  for (uint32_t q = 0; q < kRows; ++q) { mm[q] = -INFINITY; ll[q] = 0.0f; }
+  auto row_of = [&](uint32_t q) { return min(first + w + q * kWarps, t.rows - 1u); };       // (rows that are not there: the last one again, not stored)
+  for (uint32_t k = lane; k < parts; k += 32u) {
+    const float *p = a.part + static_cast<size_t>(part_s[k]) * kPart + kChunkRows * HD;
+#pragma unroll
+    for (uint32_t q = 0; q < kRows; ++q) mm[q] = fmaxf(mm[q], p[row_of(q)]);
+  }
+#pragma unroll
+  for (uint32_t q = 0; q < kRows; ++q) mm[q] = warp_reduce(mm[q], [](float u, float v) { return fmaxf(u, v); });
+  for (uint32_t k0 = 0; k0 < parts; k0 += 32u) {
+    float f[kRows] = {};
+    if (k0 + lane < parts) {
+      const float *p = a.part + static_cast<size_t>(part_s[k0 + lane]) * kPart + kChunkRows * HD;
+#pragma unroll
+      for (uint32_t q = 0; q < kRows; ++q) {
+        const uint32_t r = row_of(q);
+        f[q] = p[r] == mm[q] ? 1.0f : fast_ex2(p[r] - mm[q]);
+        ll[q] += p[kChunkRows + r] * f[q];
       }
     }
-    ll = warp_reduce(ll, [](float u, float v) { return u + v; });
-    const float inv = mm == -INFINITY && ll == 0.0f ? 0.0f : 1.0f / ll;
+    const uint32_t n = min(32u, parts - k0);
+#pragma unroll 2
+    for (uint32_t k = 0; k < n; ++k) {
+      const float *p = a.part + static_cast<size_t>(part_s[k0 + k]) * kPart + lane * V;
+#pragma unroll
+      for (uint32_t q = 0; q < kRows; ++q) {
+        const float fk = __shfl_sync(0xffffffffu, f[q], k);
+        const Vec<float, V> x = *reinterpret_cast<const Vec<float, V> *>(p + row_of(q) * HD);
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) o[q][i] += x.v[i] * fk;
+      }
+    }
+  }
+#pragma unroll 1
+  for (uint32_t q = 0; q < kRows; ++q) {
+    const uint32_t r = first + w + q * kWarps;
+    if (r >= t.rows) break;
+    const uint32_t pr = t.r0 + r, tok = a.by_group.quot(pr), head = t.head * a.group + (pr - tok * a.group), d = lane * V;
+    const int32_t row = t.s.first + static_cast<int32_t>(tok);
+    float m = mm[0], sum = ll[0], x[V];
+#pragma unroll
+    for (uint32_t k = 0; k < kRows; ++k)
+      if (k == q) {
+        m = mm[k];
+        sum = ll[k];
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) x[i] = o[k][i];
+      }
+    sum = warp_reduce(sum, [](float u, float v) { return u + v; });
+    const float inv = m == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
     bool fine = true;
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      const float v = o[i] * inv;
-      fine = fine && isfinite(v);
-      if (d + i < a.c.hd) store_row_value(row_at(a.o, row, head) + 2u * (d + i), v, a.bf16 != 0u);
+    for (uint32_t i = 0; i < V; ++i) {
+      x[i] *= inv;
+      fine = fine && isfinite(x[i]);
     }
-    if (lane == 0u && a.lse) a.lse[static_cast<int64_t>(row) * a.q_heads + head] = (mm + log2f(ll)) * 0.69314718055994531f;
+    uint8_t *p = row_at(a.o, row, head) + 2u * d;
+    if (d < a.c.hd) {
+#pragma unroll
+      for (uint32_t i = 0; i < V; i += 2) {
+        const uint32_t h = a.bf16 ? cvt_bf16x2(x[i + 1], x[i]) : cvt_f16x2(x[i + 1], x[i]);
+        if ((reinterpret_cast<uintptr_t>(p) & 3u) == 0u) {
+          reinterpret_cast<uint32_t *>(p)[i / 2u] = h;
+        } else {
+          reinterpret_cast<uint16_t *>(p)[i] = static_cast<uint16_t>(h);
+          reinterpret_cast<uint16_t *>(p)[i + 1] = static_cast<uint16_t>(h >> 16);
+        }
+      }
+    }
+    if (lane == 0u && a.lse) a.lse[static_cast<int64_t>(row) * a.q_heads + head] = (m + log2f(sum)) * 0.69314718055994531f;
     const Span sp = SeenBy(t.s, static_cast<int32_t>(tok), a.causal, a.window);
     if (__any_sync(0xffffffffu, !fine) && (sp.lo > t.keys.lo || sp.hi < t.keys.hi)) {
       __syncwarp();
