@@ -6,14 +6,16 @@
 // O stays in tensor memory; it is rescaled in place only when a row's maximum grew by more than 2^8 since the one in use was set
 // (p then stays below 256 and the result is mathematically the same). P overwrites the scores it came from.
 //
-// Roles of a CTA: a warp to issue the products, four warps that fill the ring of K and V blocks (and Q), four softmax warps for each
-// slot, one thread to a row. The products of one slot run while the other slot's softmax does:
+// Roles of a CTA: a warp to issue the products, four warps that fill the ring of K and V blocks (and Q), eight softmax warps for each
+// slot, two threads to a row with half of the keys each (one thread to a row waits for itself most of the time: SOFT8). The products of one slot run
+// while the other slot's softmax does:
 //   issue:    O0 += P0 V(j), S0 = Q0 K(j+1), O1 += P1 V(j), S1 = Q1 K(j+1), ..
 // A product waits for P of its slot; a softmax for S, whose arrival says that everything issued before is done as well.
 // The ring holds blocks in the 128-byte-swizzled layout that the tensor cores read, filled page by page: pages have any size, so a row
 // of the cache is found by itself (one page number a row, looked up a block ahead).
-// 8-bit pages: codes become f16 on their way into the ring (exact), q is scaled by a power of two for each row to fit f16, a key's scale
-// goes onto its scores and a value's onto p (see attend_step.cu).
+// 8-bit pages: K's codes become f16 on their way into the ring (exact), q is scaled by a power of two for each row to fit f16, and a key's scale
+// goes onto its scores. V becomes code x scale / 2^e in f16, e the same for 32 keys (one rounding of 2^-12, of the same size as that of p), and p
+// is multiplied by 2^e relative to the largest such power that the row has met.
 //
 // Work: one CTA to an SM. The tiles of the batch in a row, sequence by sequence and head by head, each weighed by the keys it sees and something for its
 // beginning and end, are dealt to the CTAs in equal runs, whatever their number and lengths; a run that ends inside a tile ends between
@@ -28,9 +30,11 @@ namespace b2 {
 namespace {
 
 constexpr uint32_t kCkRows = 128, kCkKeys = 128;          // rows of a slot, keys of a block
-constexpr uint32_t kSoftWarps = 8, kLoadWarps = 4, kCkThreads = (kSoftWarps + kLoadWarps + 4) * 32;     // (three of the last four warps only hold registers back)
-// Registers of a thread: launched with 128 each, the softmax warps take those that the others give up (2 x 184 + 88 + 56 = 2 x 176 + 104 + 56 = 4 x 128).
-constexpr int kSoftRegs = 184, kLoadRegs = 88, kSoftRegs8 = 176, kLoadRegs8 = 104, kIssueRegs = 56;
+constexpr uint32_t kSoftWarps = 16, kLoadWarps = 4, kCkThreads = (kSoftWarps + kLoadWarps + 4) * 32;      // (three of the last four warps only hold registers back)
+// Registers of a thread: launched with 80 each, the softmax warps take what the others give up (4 x 96 + 56 + 40 = 4 x 88 + 88 + 40 = 6 x 80).
+constexpr int kLaunchRegs = 80, kSoftRegs = 96, kLoadRegs = 56, kSoftRegs8 = 88, kLoadRegs8 = 88, kIssueRegs = 40;
+static_assert(4 * kSoftRegs + kLoadRegs + kIssueRegs == 6 * kLaunchRegs && 4 * kSoftRegs8 + kLoadRegs8 + kIssueRegs == 6 * kLaunchRegs, "the launch's registers");
+static_assert(kSoftRegs > kLaunchRegs && kSoftRegs8 > kLaunchRegs && kLoadRegs < kLaunchRegs && kLoadRegs8 > kLaunchRegs && kIssueRegs < kLaunchRegs, "raised or lowered");
 constexpr uint32_t kCkCols = 512;                         // tensor memory: S0, S1 (128 columns each), O0, O1
 constexpr float kGrow = 8.0f;                             // log2 of the growth of a row maximum that forces a rescale
 constexpr float kCkPScale = 64.0f;                        // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
@@ -41,7 +45,7 @@ struct ChunkShape {
   static constexpr uint32_t kHalf = 128u * 128u;          // 128 rows of 64 values
   static constexpr uint32_t kBlock = kHalf * (HD / 64);   // Q of a slot, K or V of a block
   static constexpr uint32_t kStages = HD == 128 ? 5 : 8;
-  static constexpr uint32_t kQ = 0, kRing = 2 * kBlock, kScales = kRing + kStages * kBlock, kShared = kScales + 2u * 1024u;      // scales of two blocks: K's, V's
+  static constexpr uint32_t kQ = 0, kRing = 2 * kBlock, kScales = kRing + kStages * kBlock, kShared = kScales + 2u * 1024u;      // scales of K of two blocks; what the softmax warps tell each other
 };
 // A tile's part that a CTA works on: packed rows [r0, r0 + rows) of a sequence (row x group + head), blocks [b0, b1) of the `blocks` of keys from
 // keys.lo that any of them sees.
@@ -53,6 +57,7 @@ struct Tile {
 struct ChunkShared {
   uint64_t q_full, q_free, full[8], empty[8], s_full[2], p_full[2], pv_done[2], scales_free[2][2];
   uint32_t tmem, failed;
+  alignas(16) float v_ref[2][4];                          // 8-bit pages: V of two blocks, 32 keys each, is held over these powers of two; negative: scales far apart
   Tile tile;                                              // no rows: the end
   union {
     unsigned long long find[kCkThreads / 32 + 2];         // (before any row is looked at)
@@ -302,20 +307,27 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
       if (((mask >> r) & 1u) && in_hd) x[k] = ldg_v4(pages + o + 16 * sub);
     }
   };
-  auto put = [&](uint32_t i, const uint4 (&x)[N], float scale) {
+  // a block as f16, K exact, V times the key's `mul`
+  auto put = [&](uint32_t i, const uint4 (&x)[N], float mul, bool value) {
     const uint32_t dst = base + Sh::kRing + (i % NS) * Sh::kBlock;
 #pragma unroll
     for (uint32_t k = 0; k < N; ++k) {
-      const uint32_t r = 32u * w + k * AT + r1;
+      const uint32_t r0 = k * AT + r1, r = 32u * w + r0;
       const uint32_t c[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
       uint32_t h[8];
 #pragma unroll
       for (int q = 0; q < 4; ++q) { h[2 * q] = cvt_e4m3x2_f16x2(c[q] & 0xffffu); h[2 * q + 1] = cvt_e4m3x2_f16x2(c[q] >> 16); }
+      if (value) {
+        const float m = __shfl_sync(0xffffffffu, mul, r0);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[q]));
+          h[q] = cvt_f16x2(f.y * m, f.x * m);
+        }
+      }
       sts_v4(dst + swizzled(r, 2u * sub), make_uint4(h[0], h[1], h[2], h[3]));
       sts_v4(dst + swizzled(r, 2u * sub + 1u), make_uint4(h[4], h[5], h[6], h[7]));
     }
-    // (the place for the scales of block i / 2; the softmax is done with those of the block two before)
-    *reinterpret_cast<float *>(sm + Sh::kScales + (i & 3u) * 512u + (32u * w + lane) * 4u) = scale;
   };
   uint32_t settled = 0;                                   // 16-bit pages: blocks that have landed and are said to have
   auto settle = [&](uint32_t n) {
@@ -398,14 +410,20 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         }
         ok = __all_sync(0xffffffffu, free);
         if (!ok) break;
-        put(it, kw, ksc);
+        put(it, kw, 1.0f, false);
+        *reinterpret_cast<float *>(sm + Sh::kScales + buf * 512u + (32u * w + lane) * 4u) = ksc;
+        // V's power of two: above the scales of the warp's 32 keys that are finite
+        const uint32_t vb = (__float_as_uint(vsc) & 0x7fffffffu) < 0x7f800000u ? __float_as_uint(vsc) & 0x7fffffffu : 0u;
+        const uint32_t most = __reduce_max_sync(0xffffffffu, vb), least = __reduce_min_sync(0xffffffffu, vb ? vb : 0x7f7fffffu);
+        const float ref = power_above(__uint_as_float(most));
+        if (lane == 0u) S->v_ref[buf][w] = most && (most >> 23) > (least >> 23) + 8u ? -ref : ref;
         done(it++);
         mask = place(off, soff);
         fetch(a.c.k, off, mask, kw);
         ksc = (mask >> lane) & 1u ? a.c.ks[soff] : 0.0f;
         ok = __all_sync(0xffffffffu, room(it));
         if (!ok) break;
-        put(it, vw, vsc);
+        put(it, vw, vsc * __uint_as_float((254u << 23) - __float_as_uint(ref)), true);
         done(it++);
         if (!q_there) q_to_all();
       }
@@ -498,246 +516,237 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of two finite values by products: x = n + f with n the nearest whole number (what adding and taking away 1.5 x 2^23 leaves), 2^f by the polynomial of
-// degree 4 whose relative error on [-1/2, 1/2] is least (2.6e-6; fitted by Remez' exchange), n into the exponent. The special-function unit gives 16
-// exponentials a cycle and SM: with it alone 128 x 128 weights take the 1024 cycles that the products of a block of 128 values take, one after
-// the other; of every kPolyOf pairs of weights kPoly come this way.
-constexpr int kPoly = 0, kPolyOf = 2;
-__device__ __forceinline__ void ex2_poly(u64 x, float &e0, float &e1) {
-  float x0, x1;
-  unpack_f32x2(x, x0, x1);
-  x = pack_f32x2(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
-  const u64 y = add_f32x2(x, pack_f32x2(12582912.0f, 12582912.0f)), f = fma_f32x2(add_f32x2(y, pack_f32x2(-12582912.0f, -12582912.0f)), pack_f32x2(-1.0f, -1.0f), x);
-  u64 p = fma_f32x2(f, pack_f32x2(0.009570102207362652f, 0.009570102207362652f), pack_f32x2(0.05591785907745361f, 0.05591785907745361f));
-  p = fma_f32x2(p, f, pack_f32x2(0.240247443318367f, 0.240247443318367f));
-  p = fma_f32x2(p, f, pack_f32x2(0.6931217908859253f, 0.6931217908859253f));
-  p = fma_f32x2(p, f, pack_f32x2(0.9999992847442627f, 0.9999992847442627f));
-  float y0, y1;
-  unpack_f32x2(y, y0, y1);
-  unpack_f32x2(p, e0, e1);
-  e0 = __uint_as_float(__float_as_uint(e0) + (__float_as_uint(y0) << 23));
-  e1 = __uint_as_float(__float_as_uint(e1) + (__float_as_uint(y1) << 23));
+// x as the next bf16 that is not below it (its bits).
+__device__ __forceinline__ uint32_t rounded_up(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (x > 0.0f ? u + 0xffffu : u) >> 16;              // (NaN and what is below 0: cut off)
 }
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<HD>;
-  constexpr uint32_t NS = Sh::kStages;
   volatile uint32_t *failed = &S->failed;
-  const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u, s = w >> 2, q4 = w & 3u;
-  const uint32_t r = s * kCkRows + 32u * q4 + lane;
-  const uint32_t s_addr = S->tmem + ((32u * q4) << 16) + s * 128u, o_addr = S->tmem + ((32u * q4) << 16) + 256u + s * HD;
-  uint32_t it = 0, n = 0, mine = 0;                       // the ring's blocks: K of a block, V behind it; the slot's blocks and tiles
+  const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u, s = w >> 3, half = (w >> 2) & 1u, q4 = w & 3u;
+  const uint32_t r = s * kCkRows + 32u * q4 + lane;       // the thread's row, of whose keys it has columns 64 half .. + 63
+  const uint32_t row_addr = S->tmem + ((32u * q4) << 16), s_addr = row_addr + s * 128u, o_addr = row_addr + 256u + s * HD + half * (HD / 2);
+  const int pair = 1 + static_cast<int>(s * 4u + q4);     // the two warps of 32 rows
+  uint16_t *top_s = reinterpret_cast<uint16_t *>(sm + Sh::kScales + 1024u) + s * 256u + 32u * q4 + lane;      // [slot][half][row]
+  float *sum_s = reinterpret_cast<float *>(sm + Sh::kScales + 1024u + s * 512u + (lane >> 4) * 256u + 64u * q4) + (lane & 15u);      // (in the same two warps' bytes)
+  uint32_t g = 0, n = 0, mine = 0;                        // blocks of all tiles; the slot's blocks and tiles
 #pragma unroll 1
   for (uint32_t turn = 0;; ++turn) {
-  if (!tc_wait_uniform(&S->q_full, turn & 1u, failed, kBudget)) return;
-  const Tile t = S->tile;
-  const int32_t e = Q8 && BF ? S->q_exp[r] : 0;
-  __syncwarp();
-  if (lane == 0u) mbar_arrive(&S->q_free);
-  if (t.rows == 0u) return;
-  if (s * kCkRows >= t.rows) {                            // the other slot's alone
-    it += 2u * (t.b1 - t.b0);
-    continue;
-  }
-  const bool has = r < t.rows;
-  const uint32_t pr = t.r0 + r, tok = a.by_group.quot(pr), head = t.head * a.group + (pr - tok * a.group);
-  const Span sp = has ? SeenBy(t.s, static_cast<int32_t>(tok), a.causal, a.window) : Span{0, 0};
-  const float sl2 = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  const uint32_t b0 = t.b0, b1 = t.b1;
-  float m_used = -INFINITY, l = 0.0f, v_ref = 0.0f;
-#pragma unroll 1
-  for (uint32_t j = b0; j < b1; ++j, it += 2u, ++n) {
-    if (!tc_wait_uniform(&S->s_full[s], n & 1u, failed, kBudget)) return;
-    const float *ks = reinterpret_cast<const float *>(sm + Sh::kScales + (it & 3u) * 512u);
-    const float *vs = ks + 128;
-    if (Q8 && !tc_wait_uniform(&S->full[(it + 1u) % NS], ((it + 1u) / NS) & 1u, failed, kBudget)) return;      // (the values' scales)
-    tc_fence_after_sync();
-    const int32_t j0 = t.keys.lo + static_cast<int32_t>(j * kCkKeys);
-    const int32_t lo = sp.lo - j0, hi = sp.hi - j0;       // columns [lo, hi) are seen
-    const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= static_cast<int32_t>(kCkKeys));
-    // 1: the row's scores into registers, and their maximum
-    uint32_t x[4][32];
+    if (!tc_wait_uniform(&S->q_full, turn & 1u, failed, kBudget)) return;
+    const Tile &t = S->tile;
+    const uint32_t rows = t.rows, seq = t.seq, part_at = t.part, r0 = t.r0, t_head = t.head;
+    const int32_t keys_lo = t.keys.lo, keys_hi = t.keys.hi;
+    const uint32_t b0 = t.b0, b1 = t.b1;
+    const Seq ts = t.s;
+    const int32_t e = Q8 && BF ? S->q_exp[r] : 0;
     __syncwarp();
+    if (lane == 0u) mbar_arrive(&S->q_free);
+    if (rows == 0u) return;
+    if (s * kCkRows >= rows) {                            // the other slot's alone
+      g += b1 - b0;
+      continue;
+    }
+    const bool has = r < rows;
+    const uint32_t pr = r0 + r, tok = a.by_group.quot(pr), head = t_head * a.group + (pr - tok * a.group);
+    const Span sp = has ? SeenBy(ts, static_cast<int32_t>(tok), a.causal, a.window) : Span{0, 0};
+    const float sl2 = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    float m_used = -INFINITY, l = 0.0f, v_ref = 0.0f;
+    bool redo = false;
+#pragma unroll 1
+    for (uint32_t j = b0; j < b1; ++j, ++g, ++n) {
+      if (!tc_wait_uniform(&S->s_full[s], n & 1u, failed, kBudget)) return;
+      tc_fence_after_sync();
+      const int32_t j0 = keys_lo + static_cast<int32_t>(j * kCkKeys);
+      const int32_t lo = sp.lo - j0, hi = sp.hi - j0;     // columns [lo, hi) of the block are seen
+      const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= static_cast<int32_t>(kCkKeys));
+      // 1: the scores into registers, and the row's maximum
+      uint32_t x[2][32];
+      __syncwarp();
+      tc_ld32(s_addr + 64u * half, x[0]);
+      tc_ld32(s_addr + 64u * half + 32u, x[1]);
+      tc_wait_ld();
+      if (Q8) {
+        const float *ks = reinterpret_cast<const float *>(sm + Sh::kScales + (g & 1u) * 512u) + 64u * half;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) tc_ld32(s_addr + 32u * c, x[c]);
-    tc_wait_ld();
-    float mx = -INFINITY, v_top = 0.0f;
-    if (Q8) {
-#pragma unroll
-      for (int i = 0; i < 128; i += 4) {
-        const float4 k4 = *reinterpret_cast<const float4 *>(ks + i), v4 = *reinterpret_cast<const float4 *>(vs + i);
-        const float kk[4] = {k4.x, k4.y, k4.z, k4.w}, vv[4] = {v4.x, v4.y, v4.z, v4.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[i >> 5][(i & 31) + e] = __float_as_uint(__uint_as_float(x[i >> 5][(i & 31) + e]) * kk[e]);
-          const bool seen = whole || (i + e >= lo && i + e < hi);
-          v_top = fmaxf(v_top, seen ? vv[e] : 0.0f);
+        for (int i = 0; i < 64; i += 4) {
+          const float4 k4 = *reinterpret_cast<const float4 *>(ks + i);
+          uint32_t *y = &x[i >> 5][i & 31];
+          y[0] = __float_as_uint(__uint_as_float(y[0]) * k4.x); y[1] = __float_as_uint(__uint_as_float(y[1]) * k4.y);
+          y[2] = __float_as_uint(__uint_as_float(y[2]) * k4.z); y[3] = __float_as_uint(__uint_as_float(y[3]) * k4.w);
         }
       }
-    }
-    if (!whole) {
+      if (!whole) {
+        const int32_t lo_h = lo - 64 * static_cast<int32_t>(half), hi_h = hi - 64 * static_cast<int32_t>(half);
 #pragma unroll
-      for (int i = 0; i < 128; ++i)
-        if (i < lo || i >= hi) x[i >> 5][i & 31] = 0xff800000u;
-    }
-    {
-      float m4[4] = {mx, mx, mx, mx};
+        for (int i = 0; i < 64; ++i)
+          if (i < lo_h || i >= hi_h) x[i >> 5][i & 31] = 0xff800000u;
+      }
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        m4[i & 1] = max3_nan(m4[i & 1], __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
-        m4[2 + (i & 1)] = max3_nan(m4[2 + (i & 1)], __uint_as_float(x[2][i]), __uint_as_float(x[3][i]));
+      for (int i = 0; i < 32; ++i) m4[i & 3] = max3_nan(m4[i & 3], __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
+      const uint32_t own = rounded_up(max3_nan(m4[0], m4[1], max3_nan(m4[2], m4[3], m4[2])));
+      top_s[half * 128u] = static_cast<uint16_t>(own);
+      bar_sync(pair, 64);                                 // (both have the scores in registers, too: P may go over them)
+      const float mx = max3_nan(__uint_as_float(own << 16), __uint_as_float(static_cast<uint32_t>(top_s[(half ^ 1u) * 128u]) << 16), -INFINITY) * sl2;
+      bool grow = mx > m_used + kGrow;
+      float alpha = 1.0f;
+      if (grow) {
+        alpha = m_used == -INFINITY ? 0.0f : fast_ex2(m_used - mx);
+        l *= alpha;
+        m_used = mx;
       }
-      mx = max3_nan(m4[0], m4[1], max3_nan(m4[2], m4[3], m4[2]));
-    }
-    mx *= sl2;
-    // (a NaN, or an infinity, among the scores: every exponential by the special-function unit, which hands it on)
-    const bool plain = whole && __all_sync(0xffffffffu, fabsf(mx) < INFINITY);
-    bool grow = mx > m_used + kGrow;
-    float alpha = 1.0f, v_mul = 1.0f;
-    if (grow) {
-      alpha = m_used == -INFINITY ? 0.0f : fast_ex2(m_used - mx);
-      l *= alpha;
-      m_used = mx;
-    }
-    if (Q8) {
-      const float ref = power_above(v_top);
-      if (ref > v_ref) {
-        alpha *= v_ref / ref;
-        v_ref = ref;
-        grow = true;
+      float v_mul[2] = {1.0f, 1.0f};
+      if (Q8) {
+        const float4 v4 = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u]);
+        const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+        float top = v_ref;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool seen = hi > 32 * k && lo < 32 * k + 32;
+          top = seen ? fmaxf(top, fabsf(vv[k])) : top;
+          // scales far apart, and some of the keys not seen by the row: they may have set the power
+          redo = redo || (seen && vv[k] < 0.0f && (lo > 32 * k || hi < 32 * k + 32));
+        }
+        if (top > v_ref) {
+          alpha *= v_ref / top;                           // (a power of two, or 0 at first)
+          v_ref = top;
+          grow = true;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v_mul[k] = v_ref > 0.0f ? fminf(fabsf(half ? vv[2 + k] : vv[k]) / v_ref, 1.0f) * kCkPScale : 0.0f;
       }
-      v_mul = kCkPScale / v_ref;
-    }
-    if (j > b0 && __any_sync(0xffffffffu, grow)) {        // (these scores came after the products before them: O is at rest)
+      if (j > b0 && __any_sync(0xffffffffu, grow)) {      // (these scores came after the products before them: O is at rest)
 #pragma unroll 1
-      for (uint32_t c0 = 0; c0 < HD; c0 += 16u) {
-        uint32_t y[16];
-        __syncwarp();
-        tc_ld16(o_addr + c0, y);
-        tc_wait_ld();
+        for (uint32_t c0 = 0; c0 < HD / 2; c0 += 16u) {
+          uint32_t y[16];
+          __syncwarp();
+          tc_ld16(o_addr + c0, y);
+          tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
-        tc_st16(o_addr + c0, y);
+          for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+          tc_st16(o_addr + c0, y);
+        }
       }
-      tc_wait_st();
-    }
-    // 2: the weights, over the scores they came from
-    const float neg = m_used == -INFINITY ? 0.0f : -m_used;
-    const unsigned long long sl2_2 = pack_f32x2(sl2, sl2), neg_2 = pack_f32x2(neg, neg);
-    unsigned long long sum[2] = {0ull, 0ull};
-    auto weights = [&](auto poly) {
+      // 2: the weights, over the scores
+      const float neg = m_used == -INFINITY ? 0.0f : -m_used;
+      const u64 sl2_2 = pack_f32x2(sl2, sl2), neg_2 = pack_f32x2(neg, neg);
+      u64 sum[2] = {0ull, 0ull};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t pk[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const u64 x2 = fma_f32x2(pack_f32x2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), sl2_2, neg_2);
           float e0, e1;
-          if (decltype(poly)::value && (i % kPolyOf) < kPoly) {
-            ex2_poly(x2, e0, e1);
-          } else {
-            unpack_f32x2(x2, e0, e1);
-            e0 = fast_ex2(e0);
-            e1 = fast_ex2(e1);
-          }
+          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), sl2_2, neg_2), e0, e1);
+          e0 = fast_ex2(e0);
+          e1 = fast_ex2(e1);
           sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
           if (Q8) {
-            const float2 v2 = *reinterpret_cast<const float2 *>(vs + 32 * c + 2 * i);
-            e0 = !decltype(poly)::value && e0 == 0.0f ? 0.0f : e0 * (v2.x * v_mul);      // (a scale that the row does not see may be anything)
-            e1 = !decltype(poly)::value && e1 == 0.0f ? 0.0f : e1 * (v2.y * v_mul);
+            e0 *= v_mul[c];
+            e1 *= v_mul[c];
           }
           pk[i] = BF && !Q8 ? cvt_bf16x2(e1, e0) : cvt_f16x2(e1, e0);
         }
         __syncwarp();
-        tc_st16(s_addr + 16u * c, pk);
+        tc_st16(s_addr + 32u * half + 16u * c, pk);
       }
-    };
-    if (plain) weights(std::true_type{});
-    else weights(std::false_type{});
-    tc_wait_st();
-    tc_fence_before_sync();
-    __syncwarp();
-    if (lane == 0u) {
-      mbar_arrive(&S->p_full[s]);
-      if (Q8) mbar_arrive(&S->scales_free[s][(it >> 1) & 1u]);
+      tc_wait_st();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0u) {
+        mbar_arrive(&S->p_full[s]);
+        if (Q8) mbar_arrive(&S->scales_free[s][g & 1u]);
+      }
+      float a0, a1;
+      unpack_f32x2(add_f32x2(sum[0], sum[1]), a0, a1);
+      l += a0 + a1;
     }
-    float a0, a1;
-    unpack_f32x2(add_f32x2(sum[0], sum[1]), a0, a1);
-    l += a0 + a1;
-  }
-  // ---- the result ----
-  if (!tc_wait_uniform(&S->pv_done[s], mine & 1u, failed, kBudget)) return;
-  ++mine;
-  tc_fence_after_sync();
-  const bool split = t.part != 0u;
-  float *part = a.part + static_cast<size_t>(split ? t.part - 1u : 0u) * (kChunkRows * (HD + 2u));
-  const bool none = m_used == -INFINITY && l == 0.0f;
-  float mul = split ? 1.0f : none ? 0.0f : 1.0f / l;
-  if (Q8) mul *= v_ref * (1.0f / kCkPScale);
-  uint8_t *out = has ? row_at(a.o, t.s.first + static_cast<int32_t>(tok), head) : a.o.p;
-  const bool vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0u, wide = (reinterpret_cast<uintptr_t>(out) & 31u) == 0u;
-  bool fine = true;
+    // ---- the result: half of the row's values each ----
+    bar_sync(pair, 64);                                   // (the other's maximum has been read)
+    if (half) *sum_s = l;
+    bar_sync(pair, 64);
+    if (!half) {
+      l += *sum_s;
+      *sum_s = l;
+    }
+    bar_sync(pair, 64);
+    if (half) l = *sum_s;
+    bar_sync(pair, 64);                                   // (and the sum)
+    if (!tc_wait_uniform(&S->pv_done[s], mine & 1u, failed, kBudget)) return;
+    ++mine;
+    tc_fence_after_sync();
+    const bool split = part_at != 0u;
+    float *part = a.part + static_cast<size_t>(split ? part_at - 1u : 0u) * (kChunkRows * (HD + 2u));
+    const bool none = m_used == -INFINITY && l == 0.0f;
+    float mul = split ? 1.0f : none ? 0.0f : 1.0f / l;
+    if (Q8) mul *= v_ref * (1.0f / kCkPScale);
+    if (redo && split) mul = __int_as_float(0x7fc00000);  // (for the launch that joins)
+    const uint32_t d0 = half * (HD / 2);
+    uint8_t *out = has ? row_at(a.o, ts.first + static_cast<int32_t>(tok), head) + 2u * d0 : a.o.p;
+    const bool vec = (reinterpret_cast<uintptr_t>(out) & 15u) == 0u, wide = (reinterpret_cast<uintptr_t>(out) & 31u) == 0u;
+    bool fine = true;
 #pragma unroll 1
-  for (uint32_t c0 = 0; c0 < HD; c0 += 32u) {
-    uint32_t x[32];
-    __syncwarp();
-    tc_ld32(o_addr + c0, x);
-    tc_wait_ld();
-    if (!has) continue;
+    for (uint32_t c0 = 0; c0 < HD / 2; c0 += 32u) {
+      uint32_t x[32];
+      __syncwarp();
+      tc_ld32(o_addr + c0, x);
+      tc_wait_ld();
+      if (!has) continue;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float v = __uint_as_float(x[i]) * mul;
-      x[i] = __float_as_uint(v);
-      fine = fine && isfinite(v);
-    }
-    if (split) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 8) stg_v8(part + r * HD + c0 + i, x + i);
-      continue;
-    }
-    if (wide) {                                           // whole sectors: a row is 32-byte aligned, and so is its end
-      uint32_t h[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) h[e] = BF ? cvt_bf16x2(__uint_as_float(x[2 * e + 1]), __uint_as_float(x[2 * e])) : cvt_f16x2(__uint_as_float(x[2 * e + 1]), __uint_as_float(x[2 * e]));
-      if (c0 < a.c.hd) stg_v8(out + 2u * c0, h);
-      if (c0 + 16u < a.c.hd) stg_v8(out + 2u * c0 + 32u, h + 8);
-      continue;
-    }
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      if (c0 + i >= a.c.hd) break;
-      uint32_t h[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float u = __uint_as_float(x[i + 2 * e]), v = __uint_as_float(x[i + 2 * e + 1]);
-        h[e] = BF ? cvt_bf16x2(v, u) : cvt_f16x2(v, u);
+      for (int i = 0; i < 32; ++i) {
+        const float v = __uint_as_float(x[i]) * mul;
+        x[i] = __float_as_uint(v);
+        fine = fine && isfinite(v);
       }
-      uint8_t *p = out + 2u * (c0 + i);
-      if (vec) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(h[0], h[1], h[2], h[3]);
-      } else {
+      if (split) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          reinterpret_cast<uint16_t *>(p)[2 * e] = static_cast<uint16_t>(h[e]);
-          reinterpret_cast<uint16_t *>(p)[2 * e + 1] = static_cast<uint16_t>(h[e] >> 16);
+        for (int i = 0; i < 32; i += 8) stg_v8(part + r * HD + d0 + c0 + i, x + i);
+        continue;
+      }
+      if (wide) {                                         // whole sectors: a row is 32-byte aligned, and so is its end
+        uint32_t h[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) h[k] = BF ? cvt_bf16x2(__uint_as_float(x[2 * k + 1]), __uint_as_float(x[2 * k])) : cvt_f16x2(__uint_as_float(x[2 * k + 1]), __uint_as_float(x[2 * k]));
+        if (d0 + c0 < a.c.hd) stg_v8(out + 2u * c0, h);
+        if (d0 + c0 + 16u < a.c.hd) stg_v8(out + 2u * c0 + 32u, h + 8);
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        if (d0 + c0 + i >= a.c.hd) break;
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float u = __uint_as_float(x[i + 2 * k]), v = __uint_as_float(x[i + 2 * k + 1]);
+          h[k] = BF ? cvt_bf16x2(v, u) : cvt_f16x2(v, u);
+        }
+        uint8_t *p = out + 2u * (c0 + i);
+        if (vec) {
+          *reinterpret_cast<uint4 *>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            reinterpret_cast<uint16_t *>(p)[2 * k] = static_cast<uint16_t>(h[k]);
+            reinterpret_cast<uint16_t *>(p)[2 * k + 1] = static_cast<uint16_t>(h[k] >> 16);
+          }
         }
       }
     }
-  }
-  tc_fence_before_sync();
-  bool redo = false;
-  if (has && split) {
-    part[kChunkRows * HD + r] = m_used;
-    part[kChunkRows * HD + kChunkRows + r] = l;
-  } else if (has) {
-    if (a.lse) a.lse[static_cast<int64_t>(t.s.first + static_cast<int32_t>(tok)) * a.q_heads + head] = (m_used + log2f(l)) * 0.69314718055994531f;
-    redo = !fine && (sp.lo > t.keys.lo || sp.hi < t.keys.hi);
-  }
-  for (uint32_t again = __ballot_sync(0xffffffffu, redo); again; again &= again - 1u) {      // (rows of this warp, one after another)
-    const uint32_t k = __ffs(again) - 1u, q = t.r0 + s * kCkRows + 32u * q4 + k;
-    __syncwarp();
-    attend_row_alone(a, t.seq, t.s, static_cast<int32_t>(q / a.group), t.head * a.group + q % a.group);
-  }
+    tc_fence_before_sync();
+    if (has && split && !half) {
+      part[kChunkRows * HD + r] = m_used;
+      part[kChunkRows * HD + kChunkRows + r] = l;
+    } else if (has && !split && !half && a.lse) {
+      a.lse[static_cast<int64_t>(ts.first + static_cast<int32_t>(tok)) * a.q_heads + head] = (m_used + log2f(l)) * 0.69314718055994531f;
+    }
+    redo = has && !split && (redo || (!fine && (sp.lo > keys_lo || sp.hi < keys_hi)));
+    for (uint32_t again = __ballot_sync(0xffffffffu, redo); again; again &= again - 1u) {      // (rows of this warp, one after another, its half of the values)
+      const uint32_t k = __ffs(again) - 1u, q = r0 + s * kCkRows + 32u * q4 + k;
+      __syncwarp();
+      attend_row_alone(a, seq, ts, static_cast<int32_t>(q / a.group), t_head * a.group + q % a.group, d0, HD / 2);
+    }
   }
 }
 
@@ -773,8 +782,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) b2_attend_chunk(const __grid_co
     mbar_init(&S->q_free, 1u + kSoftWarps);
     for (uint32_t i = 0; i < Sh::kStages; ++i) { mbar_init(&S->full[i], kLoadWarps * 32u); mbar_init(&S->empty[i], 1u); }
     for (uint32_t s = 0; s < 2u; ++s) {
-      mbar_init(&S->s_full[s], 1u); mbar_init(&S->p_full[s], 4u); mbar_init(&S->pv_done[s], 1u);
-      for (uint32_t i = 0; i < 2u; ++i) mbar_init(&S->scales_free[s][i], 4u);
+      mbar_init(&S->s_full[s], 1u); mbar_init(&S->p_full[s], 8u); mbar_init(&S->pv_done[s], 1u);
+      for (uint32_t i = 0; i < 2u; ++i) mbar_init(&S->scales_free[s][i], 8u);
     }
     S->failed = 0u;
     fence_mbar_init();
@@ -790,7 +799,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) b2_attend_chunk(const __grid_co
     more_registers<Q8 ? kSoftRegs8 : kSoftRegs>();
     chunk_rows<BF, Q8, HD>(a, sm, S);
   } else if (w < kSoftWarps + kLoadWarps) {
-    fewer_registers<Q8 ? kLoadRegs8 : kLoadRegs>();
+    if constexpr (Q8) more_registers<kLoadRegs8>();       // (a count above the launch's is raised, one below it lowered: the other way round is no instruction)
+    else fewer_registers<kLoadRegs>();
     Walk wk;
     wk.seek(a, cap, seq, before, x0);
     chunk_load<BF, Q8, HD>(a, wk, x0, x1, sm, S);
@@ -938,7 +948,7 @@ __global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_cons
     const Span sp = SeenBy(t.s, static_cast<int32_t>(tok), a.causal, a.window);
     if (__any_sync(0xffffffffu, !fine) && (sp.lo > t.keys.lo || sp.hi < t.keys.hi)) {
       __syncwarp();
-      attend_row_alone(a, t.seq, t.s, static_cast<int32_t>(tok), head);
+      attend_row_alone(a, t.seq, t.s, static_cast<int32_t>(tok), head, 0u, HD);
     }
   }
 }

@@ -40,7 +40,8 @@ __device__ __forceinline__ uint8_t *row_at(const RowsRef &r, int32_t row, uint32
 // One row of the result by itself, over the keys that it sees and no others, by one warp. A product over a tile of keys gives a
 // key that a row does not see the weight 0, and 0 times a NaN or an infinity is a NaN: where a tile's result is not finite, the
 // rows that do not see all of its keys are worked out here again. Slow, and only reached by caches that hold such values.
-static __device__ __noinline__ void attend_row_alone(const AttendArgs &a, uint32_t seq, const Seq s, int32_t i, uint32_t head) {
+// (of its values [v0, v0 + nv), and lse with the first)
+static __device__ __noinline__ void attend_row_alone(const AttendArgs &a, uint32_t seq, const Seq s, int32_t i, uint32_t head, uint32_t v0, uint32_t nv) {
   const uint32_t lane = threadIdx.x & 31u, h = head / a.group, d0 = lane * 4u;
   const bool has = d0 < a.c.hd, bf = a.bf16 != 0u;
   const Span sp = SeenBy(s, i, a.causal, a.window);
@@ -81,12 +82,12 @@ static __device__ __noinline__ void attend_row_alone(const AttendArgs &a, uint32
     }
   }
   const bool none = m == -INFINITY && l == 0.0f;
-  if (has) {
+  if (has && d0 >= v0 && d0 < v0 + nv) {
     uint8_t *p = row_at(a.o, s.first + i, head) + 2u * d0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) store_row_value(p + 2 * k, none ? 0.0f : acc[k] / l, bf);
   }
-  if (lane == 0u && a.lse) a.lse[static_cast<int64_t>(s.first + i) * a.q_heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  if (lane == 0u && v0 == 0u && a.lse) a.lse[static_cast<int64_t>(s.first + i) * a.q_heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
 // The sequence b whose units hold unit `target` of all sequences' units in a row, and the number of those before b's; false where

@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
     if (redo) {
       const bool all = whole || together;                 // (else one warp is here)
       for (uint32_t r = all ? w : 0u; r < rows; r += all ? kStepWarps : 1u)
-        if ((redo >> r) & 1u) attend_row_alone(a, cw.b, cw.s, static_cast<int32_t>(r / a.group), cw.h * a.group + r % a.group);
+        if ((redo >> r) & 1u) attend_row_alone(a, cw.b, cw.s, static_cast<int32_t>(r / a.group), cw.h * a.group + r % a.group, 0u, HD);
     }
     if (!more) break;
     w_tile -= t_end;                                      // (the warps take the CTA's tiles in turn, across items)
