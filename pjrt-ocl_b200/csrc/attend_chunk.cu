@@ -6,16 +6,18 @@
 // O stays in tensor memory; it is rescaled in place only when a row's maximum grew by more than 2^8 since the one in use was set
 // (p then stays below 256 and the result is mathematically the same). P overwrites the scores it came from.
 //
-// Roles of a CTA: a warp to issue the products, four warps that fill the ring of K and V blocks (and Q), eight softmax warps for each
-// slot, two threads to a row with half of the keys each (one thread to a row waits for itself most of the time: SOFT8). The products of one slot run
-// while the other slot's softmax does:
+// Roles of a CTA: a warp to issue the products, four warps (8-bit pages: eight) that fill the ring of K and V blocks (and Q), eight softmax
+// warps for each slot, two threads to a row with half of the keys each (one thread to a row: as fast with 128 values a head, 5 % slower
+// with 64). The products of one slot run while the other slot's softmax does:
 //   issue:    O0 += P0 V(j), S0 = Q0 K(j+1), O1 += P1 V(j), S1 = Q1 K(j+1), ..
 // A product waits for P of its slot; a softmax for S, whose arrival says that everything issued before is done as well.
 // The ring holds blocks in the 128-byte-swizzled layout that the tensor cores read, filled page by page: pages have any size, so a row
 // of the cache is found by itself (one page number a row, looked up a block ahead).
-// 8-bit pages: K's codes become f16 on their way into the ring (exact), q is scaled by a power of two for each row to fit f16, and a key's scale
-// goes onto its scores. V becomes code x scale / 2^e in f16, e the same for 32 keys (one rounding of 2^-12, of the same size as that of p), and p
-// is multiplied by 2^e relative to the largest such power that the row has met.
+// 8-bit pages: codes become f16 on their way into the ring. K's exactly, its scales go onto the scores, in f32; q is scaled by a power of two
+// for each row to fit f16. V's times their key's scale relative to a power of two above the scales of 16 keys side by side (rounded to 2^-12
+// of themselves, as the weights are); the power goes onto the weights. (V exact, too, with its scales on the weights: 1015 us instead of
+// 793 for 2048 rows behind 14336 of 32 heads of 128 values. A warp that reads 64 scales waits for 8 KB of them.) The codes of a block
+// ahead wait in shared memory as they are, copied asynchronously (in registers: 1045 us).
 //
 // Work: one CTA to an SM. The tiles of the batch in a row, sequence by sequence and head by head, each weighed by the keys it sees and something for its
 // beginning and end, are dealt to the CTAs in equal runs, whatever their number and lengths; a run that ends inside a tile ends between
@@ -30,22 +32,27 @@ namespace b2 {
 namespace {
 
 constexpr uint32_t kCkRows = 128, kCkKeys = 128;          // rows of a slot, keys of a block
-constexpr uint32_t kSoftWarps = 16, kLoadWarps = 4, kCkThreads = (kSoftWarps + kLoadWarps + 4) * 32;      // (three of the last four warps only hold registers back)
-// Registers of a thread: launched with 80 each, the softmax warps take what the others give up (4 x 96 + 56 + 40 = 4 x 88 + 88 + 40 = 6 x 80).
-constexpr int kLaunchRegs = 80, kSoftRegs = 96, kLoadRegs = 56, kSoftRegs8 = 88, kLoadRegs8 = 88, kIssueRegs = 40;
-static_assert(4 * kSoftRegs + kLoadRegs + kIssueRegs == 6 * kLaunchRegs && 4 * kSoftRegs8 + kLoadRegs8 + kIssueRegs == 6 * kLaunchRegs, "the launch's registers");
-static_assert(kSoftRegs > kLaunchRegs && kSoftRegs8 > kLaunchRegs && kLoadRegs < kLaunchRegs && kLoadRegs8 > kLaunchRegs && kIssueRegs < kLaunchRegs, "raised or lowered");
+constexpr uint32_t kSoftWarps = 16;
+// What goes by the pages' type: filling warps (codes are converted by them), registers of a thread. Launched with as many as the threads divide the SM's by, the
+// softmax warps take what the others give up; three of the last four warps only hold registers back.
+template <bool Q8>
+struct ChunkWarps {
+  static constexpr uint32_t kLoad = Q8 ? 8 : 4, kThreads = (kSoftWarps + kLoad + 4) * 32;
+  static constexpr int kLaunch = Q8 ? 72 : 80, kSoft = Q8 ? 80 : 96, kFill = Q8 ? 72 : 56, kIssue = 40;
+  static_assert(4 * kSoft + static_cast<int>(kLoad) / 4 * kFill + kIssue == (5 + static_cast<int>(kLoad) / 4) * kLaunch, "the launch's registers");
+  static_assert(kSoft > kLaunch && kFill <= kLaunch && kIssue < kLaunch, "raised or lowered (the other way round is no instruction)");
+};
 constexpr uint32_t kCkCols = 512;                         // tensor memory: S0, S1 (128 columns each), O0, O1
 constexpr float kGrow = 8.0f;                             // log2 of the growth of a row maximum that forces a rescale
 constexpr float kCkPScale = 64.0f;                        // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
 constexpr unsigned long long kBudget = 2000000000ull;     // ns that a wait may take
 
-template <int HD>
+template <bool Q8, int HD>
 struct ChunkShape {
   static constexpr uint32_t kHalf = 128u * 128u;          // 128 rows of 64 values
   static constexpr uint32_t kBlock = kHalf * (HD / 64);   // Q of a slot, K or V of a block
-  static constexpr uint32_t kStages = HD == 128 ? 5 : 8;
-  static constexpr uint32_t kQ = 0, kRing = 2 * kBlock, kScales = kRing + kStages * kBlock, kShared = kScales + 2u * 1024u;      // scales of K of two blocks; what the softmax warps tell each other
+  static constexpr uint32_t kStages = HD == 64 ? 8 : Q8 ? 4 : 5;
+  static constexpr uint32_t kQ = 0, kRing = 2 * kBlock, kCodes = kRing + kStages * kBlock, kScales = kCodes + (Q8 ? kBlock : 0u), kTops = kScales + (Q8 ? 1024u : 0u), kShared = kTops + 1024u;      // codes of K and V of a block; K's scales of two; what the softmax warps tell each other
 };
 // A tile's part that a CTA works on: packed rows [r0, r0 + rows) of a sequence (row x group + head), blocks [b0, b1) of the `blocks` of keys from
 // keys.lo that any of them sees.
@@ -57,16 +64,16 @@ struct Tile {
 struct ChunkShared {
   uint64_t q_full, q_free, full[8], empty[8], s_full[2], p_full[2], pv_done[2], scales_free[2][2];
   uint32_t tmem, failed;
-  alignas(16) float v_ref[2][4];                          // 8-bit pages: V of two blocks, 32 keys each, is held over these powers of two; negative: scales far apart
+  alignas(16) float v_ref[2][8];                          // 8-bit pages: powers of two above V's scales of two blocks, 16 keys each; negative: scales far apart
   Tile tile;                                              // no rows: the end
   union {
-    unsigned long long find[kCkThreads / 32 + 2];         // (before any row is looked at)
+    unsigned long long find[30];                          // (before any row is looked at)
     int8_t q_exp[256];                                    // 8-bit pages: each row of q was scaled by 2^e
   };
 };
-template <int HD>
-constexpr uint32_t ChunkSmem() { return ChunkShape<HD>::kShared + ((sizeof(ChunkShared) + 15u) & ~15u); }
-static_assert(ChunkSmem<128>() <= 227u * 1024u && ChunkSmem<64>() <= 227u * 1024u, "shared memory of an SM");
+template <bool Q8, int HD>
+constexpr uint32_t ChunkSmem() { return ChunkShape<Q8, HD>::kShared + ((sizeof(ChunkShared) + 15u) & ~15u); }
+static_assert(ChunkSmem<false, 128>() <= 227u * 1024u && ChunkSmem<true, 128>() <= 227u * 1024u && ChunkSmem<true, 64>() <= 227u * 1024u, "shared memory of an SM");
 
 // ---- how the work is dealt ----
 typedef unsigned long long u64;
@@ -185,8 +192,8 @@ __device__ __forceinline__ void clear_rows(const AttendArgs &a, const Tile &t, u
 // Rows of q into shared memory, a 16-byte chunk to a thread. As they are they come by asynchronous copies (still under way on return).
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void load_q(const AttendArgs &a, const Tile &t, uint32_t tid, uint32_t base, int8_t *q_exp) {
-  using Sh = ChunkShape<HD>;
-  constexpr uint32_t QL = HD / 8, AT = kLoadWarps * 32u / QL;      // threads to a row, rows at once
+  using Sh = ChunkShape<Q8, HD>;
+  constexpr uint32_t QL = HD / 8, AT = ChunkWarps<Q8>::kLoad * 32u / QL;      // threads to a row, rows at once
   const bool vec = ((reinterpret_cast<uintptr_t>(a.q.p) & 15u) | ((a.q.row | a.q.head) & 7)) == 0;
   const uint32_t c = tid % QL, r0 = tid / QL, rows = t.rows > kCkRows ? 256u : 128u;
   const bool in_hd = c * 8u < a.c.hd;
@@ -245,7 +252,7 @@ static __device__ __forceinline__ void load_q(const AttendArgs &a, const Tile &t
 
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk, u64 x0, u64 x1, uint8_t *sm, ChunkShared *S) {
-  using Sh = ChunkShape<HD>;
+  using Sh = ChunkShape<Q8, HD>;
   constexpr uint32_t NS = Sh::kStages;
   volatile uint32_t *failed = &S->failed;
   const uint64_t cap = capacity_of(a.c, a.b);
@@ -254,13 +261,14 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
   uint32_t it = 0;                                        // blocks filled so far: K, V, K, V, ..
   uint32_t used[2][2] = {{0u, 0u}, {0u, 0u}};             // 8-bit pages: how often each slot has used each place for scales
   Tile t = {};
-  // the lane's key of a block: 32 w + lane
+  // the lane's key of a block: RW w + lane
+  constexpr uint32_t RW = kCkKeys / ChunkWarps<Q8>::kLoad;
   int32_t page = -1;
   uint32_t slot = 0, entry = 0;
   bool live = false;
   auto look_ahead = [&](uint32_t j) {
-    const int32_t p = t.keys.lo + static_cast<int32_t>(j * kCkKeys + 32u * w + lane);
-    live = j < t.b1 && p < t.keys.hi;
+    const int32_t p = t.keys.lo + static_cast<int32_t>(j * kCkKeys + RW * w + lane);
+    live = j < t.b1 && p < t.keys.hi && lane < RW;
     if (live) {
       entry = a.c.by_page.quot(static_cast<uint32_t>(p));
       slot = static_cast<uint32_t>(p) - entry * a.c.page_size;
@@ -284,7 +292,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
     mbar_arrive(&S->full[i % NS]);
   };
   bool ok = true;
-  constexpr uint32_t CH = Q8 ? HD / 16 : HD / 8, AT = 32u / CH, N = 32u / AT;     // 16-byte chunks of a row; rows at once; loads of a thread
+  constexpr uint32_t CH = Q8 ? HD / 16 : HD / 8, AT = 32u / CH, N = RW / AT;     // 16-byte chunks of a row; rows at once; loads of a thread
   const uint32_t sub = lane % CH, r1 = lane / CH;
   const bool in_hd = sub * 16u < a.c.hd * (Q8 ? 1u : 2u);
   auto copy = [&](const uint8_t *pages, uint32_t i, int64_t off, uint32_t mask) {
@@ -294,30 +302,35 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
       const uint32_t r = k * AT + r1;
       const int64_t o = __shfl_sync(0xffffffffu, off, r);
       const uint32_t bytes = ((mask >> r) & 1u) && in_hd ? 16u : 0u;
-      cp_async_16_zfill(dst + swizzled(32u * w + r, sub), pages + (bytes ? o + 16 * sub : 0), bytes);
+      cp_async_16_zfill(dst + swizzled(RW * w + r, sub), pages + (bytes ? o + 16 * sub : 0), bytes);
     }
     cp_async_commit();
   };
-  auto fetch = [&](const uint8_t *pages, int64_t off, uint32_t mask, uint4 (&x)[N]) {
+  // 8-bit pages: the thread's own 16 bytes of each of its rows wait as they are, K (v: 0) and V (1) of a block ahead
+  const uint32_t codes = base + Sh::kCodes + tid * 16u;
+  constexpr uint32_t kCodeRow = ChunkWarps<Q8>::kLoad * 512u;
+  auto fetch = [&](const uint8_t *pages, uint32_t v, int64_t off, uint32_t mask) {
 #pragma unroll
     for (uint32_t k = 0; k < N; ++k) {
       const uint32_t r = k * AT + r1;
       const int64_t o = __shfl_sync(0xffffffffu, off, r);
-      x[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (((mask >> r) & 1u) && in_hd) x[k] = ldg_v4(pages + o + 16 * sub);
+      const uint32_t bytes = ((mask >> r) & 1u) && in_hd ? 16u : 0u;
+      cp_async_16_zfill(codes + (v * N + k) * kCodeRow, pages + (bytes ? o + 16 * sub : 0), bytes);
     }
+    cp_async_commit();
   };
-  // a block as f16, K exact, V times the key's `mul`
-  auto put = [&](uint32_t i, const uint4 (&x)[N], float mul, bool value) {
+  // the warp's keys of a block; V's times `mul`
+  auto put = [&](uint32_t i, uint32_t v, float mul) {
     const uint32_t dst = base + Sh::kRing + (i % NS) * Sh::kBlock;
 #pragma unroll
     for (uint32_t k = 0; k < N; ++k) {
-      const uint32_t r0 = k * AT + r1, r = 32u * w + r0;
-      const uint32_t c[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+      const uint32_t r0 = k * AT + r1, r = RW * w + r0;
+      const uint4 x = lds_v4(codes + (v * N + k) * kCodeRow);
+      const uint32_t c[4] = {x.x, x.y, x.z, x.w};
       uint32_t h[8];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) { h[2 * q] = cvt_e4m3x2_f16x2(c[q] & 0xffffu); h[2 * q + 1] = cvt_e4m3x2_f16x2(c[q] >> 16); }
-      if (value) {
+      for (int q = 0; q < 8; ++q) h[q] = cvt_e4m3x2_f16x2(q & 1 ? c[q >> 1] >> 16 : c[q >> 1] & 0xffffu);
+      if (v) {
         const float m = __shfl_sync(0xffffffffu, mul, r0);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
@@ -325,8 +338,11 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
           h[q] = cvt_f16x2(f.y * m, f.x * m);
         }
       }
-      sts_v4(dst + swizzled(r, 2u * sub), make_uint4(h[0], h[1], h[2], h[3]));
-      sts_v4(dst + swizzled(r, 2u * sub + 1u), make_uint4(h[4], h[5], h[6], h[7]));
+      // (the threads of a row's second 64 values the other way round: other banks)
+      const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
+      const uint32_t late = HD == 128 ? sub >> 2 : 0u;
+      sts_v4(dst + swizzled(r, 2u * sub + late), late ? h1 : h0);
+      sts_v4(dst + swizzled(r, 2u * sub + (late ^ 1u)), late ? h0 : h1);
     }
   };
   uint32_t settled = 0;                                   // 16-bit pages: blocks that have landed and are said to have
@@ -343,7 +359,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
       wk.tile(a, x0, x1, t);
       // (rows that see no key are cleared by the CTA in whose run the tile begins)
       if (t.blocks == 0u) {
-        if (wk.at >= x0) clear_rows(a, t, tid, kLoadWarps * 32u);
+        if (wk.at >= x0) clear_rows(a, t, tid, ChunkWarps<Q8>::kLoad * 32u);
       }
       found = t.b0 < t.b1;
       t.part = t.b0 == 0u && t.b1 == t.blocks ? 0u : 1u + blockIdx.x * 2u + (t.b0 == 0u ? 1u : 0u);
@@ -392,15 +408,13 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         }
       }
     } else {
-      uint4 kw[N], vw[N];
       int64_t off, soff;
       uint32_t mask = place(off, soff);
-      fetch(a.c.k, off, mask, kw);
-      float ksc = (mask >> lane) & 1u ? a.c.ks[soff] : 0.0f;
+      fetch(a.c.k, 0u, off, mask);
+      fetch(a.c.v, 1u, off, mask);
+      float ksc = (mask >> lane) & 1u ? a.c.ks[soff] : 0.0f, vsc = (mask >> lane) & 1u ? a.c.vs[soff] : 0.0f;
+      look_ahead(t.b0 + 1u);
       for (uint32_t j = t.b0; ok && j < t.b1; ++j) {
-        fetch(a.c.v, off, mask, vw);
-        const float vsc = (mask >> lane) & 1u ? a.c.vs[soff] : 0.0f;
-        look_ahead(j + 1u);
         const uint32_t buf = (it >> 1) & 1u;
         bool free = room(it);
         for (uint32_t s = 0; s < 2u; ++s) {
@@ -410,21 +424,28 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         }
         ok = __all_sync(0xffffffffu, free);
         if (!ok) break;
-        put(it, kw, 1.0f, false);
-        *reinterpret_cast<float *>(sm + Sh::kScales + buf * 512u + (32u * w + lane) * 4u) = ksc;
-        // V's power of two: above the scales of the warp's 32 keys that are finite
-        const uint32_t vb = (__float_as_uint(vsc) & 0x7fffffffu) < 0x7f800000u ? __float_as_uint(vsc) & 0x7fffffffu : 0u;
+        if (lane < RW) *reinterpret_cast<float *>(sm + Sh::kScales + buf * 512u + (RW * w + lane) * 4u) = ksc;
+        // V's power of two: above the scales of the warp's keys that are finite
+        const uint32_t vb = lane < RW && (__float_as_uint(vsc) & 0x7fffffffu) < 0x7f800000u ? __float_as_uint(vsc) & 0x7fffffffu : 0u;
         const uint32_t most = __reduce_max_sync(0xffffffffu, vb), least = __reduce_min_sync(0xffffffffu, vb ? vb : 0x7f7fffffu);
-        const float ref = power_above(__uint_as_float(most));
-        if (lane == 0u) S->v_ref[buf][w] = most && (most >> 23) > (least >> 23) + 8u ? -ref : ref;
+        const float v_ref = power_above(__uint_as_float(most));
+        if (lane == 0u) S->v_ref[buf][w] = most && (most >> 23) > (least >> 23) + 8u ? -v_ref : v_ref;
+        cp_async_wait<1>();                               // (K's codes)
+        put(it, 0u, 1.0f);
         done(it++);
         mask = place(off, soff);
-        fetch(a.c.k, off, mask, kw);
+        look_ahead(j + 2u);
+        if (j + 1u < t.b1) fetch(a.c.k, 0u, off, mask);
+        else cp_async_commit();                           // (nothing: zeros would meet the next tile's copies)
         ksc = (mask >> lane) & 1u ? a.c.ks[soff] : 0.0f;
         ok = __all_sync(0xffffffffu, room(it));
         if (!ok) break;
-        put(it, vw, vsc * __uint_as_float((254u << 23) - __float_as_uint(ref)), true);
+        cp_async_wait<1>();                               // (V's)
+        put(it, 1u, vsc * __uint_as_float((254u << 23) - __float_as_uint(v_ref)));
         done(it++);
+        if (j + 1u < t.b1) fetch(a.c.v, 1u, off, mask);
+        else cp_async_commit();
+        vsc = (mask >> lane) & 1u ? a.c.vs[soff] : 0.0f;
         if (!q_there) q_to_all();
       }
     }
@@ -438,9 +459,9 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
 }
 
 // ---- the issuing warp -----------------------------------------------------------------------
-template <bool F16, int HD>
+template <bool F16, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_products(uint8_t *sm, ChunkShared *S) {
-  using Sh = ChunkShape<HD>;
+  using Sh = ChunkShape<Q8, HD>;
   constexpr uint32_t NS = Sh::kStages;
   volatile uint32_t *failed = &S->failed;
   const uint32_t base = smem_addr(sm), tmem = S->tmem;
@@ -464,7 +485,7 @@ static __device__ __forceinline__ void chunk_products(uint8_t *sm, ChunkShared *
     if (leader) {
 #pragma unroll
       for (uint32_t k = 0; k < kCkKeys / 16u; ++k)
-        tc_mma_f16_ts(tmem + 256u + s * HD, tmem + s * 128u + 8u * k, dv + ((st * Sh::kBlock) >> 4) + k * (2048u >> 4), idesc_o, (!first || k) ? 1u : 0u);
+        tc_mma_f16_ts(tmem + 256u + s * HD, tmem + s * 128u + 8u * k + (k >> 2) * 32u, dv + ((st * Sh::kBlock) >> 4) + k * (2048u >> 4), idesc_o, (!first || k) ? 1u : 0u);
     }
     __syncwarp();
   };
@@ -523,14 +544,14 @@ __device__ __forceinline__ uint32_t rounded_up(float x) {
 }
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *sm, ChunkShared *S) {
-  using Sh = ChunkShape<HD>;
+  using Sh = ChunkShape<Q8, HD>;
   volatile uint32_t *failed = &S->failed;
   const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u, s = w >> 3, half = (w >> 2) & 1u, q4 = w & 3u;
   const uint32_t r = s * kCkRows + 32u * q4 + lane;       // the thread's row, of whose keys it has columns 64 half .. + 63
   const uint32_t row_addr = S->tmem + ((32u * q4) << 16), s_addr = row_addr + s * 128u, o_addr = row_addr + 256u + s * HD + half * (HD / 2);
   const int pair = 1 + static_cast<int>(s * 4u + q4);     // the two warps of 32 rows
-  uint16_t *top_s = reinterpret_cast<uint16_t *>(sm + Sh::kScales + 1024u) + s * 256u + 32u * q4 + lane;      // [slot][half][row]
-  float *sum_s = reinterpret_cast<float *>(sm + Sh::kScales + 1024u + s * 512u + (lane >> 4) * 256u + 64u * q4) + (lane & 15u);      // (in the same two warps' bytes)
+  uint16_t *top_s = reinterpret_cast<uint16_t *>(sm + Sh::kTops) + s * 256u + 32u * q4 + lane;      // [slot][half][row]
+  float *sum_s = reinterpret_cast<float *>(sm + Sh::kTops + s * 512u + (lane >> 4) * 256u + 64u * q4) + (lane & 15u);      // (in the same two warps' bytes)
   uint32_t g = 0, n = 0, mine = 0;                        // blocks of all tiles; the slot's blocks and tiles
 #pragma unroll 1
   for (uint32_t turn = 0;; ++turn) {
@@ -561,34 +582,38 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
       const int32_t j0 = keys_lo + static_cast<int32_t>(j * kCkKeys);
       const int32_t lo = sp.lo - j0, hi = sp.hi - j0;     // columns [lo, hi) of the block are seen
       const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= static_cast<int32_t>(kCkKeys));
-      // 1: the scores into registers, and the row's maximum
-      uint32_t x[2][32];
-      __syncwarp();
-      tc_ld32(s_addr + 64u * half, x[0]);
-      tc_ld32(s_addr + 64u * half + 32u, x[1]);
-      tc_wait_ld();
-      if (Q8) {
-        const float *ks = reinterpret_cast<const float *>(sm + Sh::kScales + (g & 1u) * 512u) + 64u * half;
+      // 1: the row's maximum. The scores are read twice: half of a row's in registers at once leave too few for the rest
+      const int32_t lo_h = lo - 64 * static_cast<int32_t>(half), hi_h = hi - 64 * static_cast<int32_t>(half);
+      const float *ks = reinterpret_cast<const float *>(sm + Sh::kScales + (g & 1u) * 512u) + 64u * half;
+      auto scores = [&](int c, uint32_t (&x)[32]) {
+        __syncwarp();
+        tc_ld32(s_addr + 64u * half + 32u * c, x);
+        tc_wait_ld();
+        if (Q8) {
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          const float4 k4 = *reinterpret_cast<const float4 *>(ks + i);
-          uint32_t *y = &x[i >> 5][i & 31];
-          y[0] = __float_as_uint(__uint_as_float(y[0]) * k4.x); y[1] = __float_as_uint(__uint_as_float(y[1]) * k4.y);
-          y[2] = __float_as_uint(__uint_as_float(y[2]) * k4.z); y[3] = __float_as_uint(__uint_as_float(y[3]) * k4.w);
+          for (int i = 0; i < 32; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + i);
+            x[i] = __float_as_uint(__uint_as_float(x[i]) * k4.x); x[i + 1] = __float_as_uint(__uint_as_float(x[i + 1]) * k4.y);
+            x[i + 2] = __float_as_uint(__uint_as_float(x[i + 2]) * k4.z); x[i + 3] = __float_as_uint(__uint_as_float(x[i + 3]) * k4.w);
+          }
         }
-      }
-      if (!whole) {
-        const int32_t lo_h = lo - 64 * static_cast<int32_t>(half), hi_h = hi - 64 * static_cast<int32_t>(half);
+        if (!whole) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (i < lo_h || i >= hi_h) x[i >> 5][i & 31] = 0xff800000u;
-      }
+          for (int i = 0; i < 32; ++i)
+            if (i + 32 * c < lo_h || i + 32 * c >= hi_h) x[i] = 0xff800000u;
+        }
+      };
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 32; ++i) m4[i & 3] = max3_nan(m4[i & 3], __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
+      for (int c = 0; c < 2; ++c) {
+        uint32_t x[32];
+        scores(c, x);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m4[i & 3] = max3_nan(m4[i & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 16]));
+      }
       const uint32_t own = rounded_up(max3_nan(m4[0], m4[1], max3_nan(m4[2], m4[3], m4[2])));
       top_s[half * 128u] = static_cast<uint16_t>(own);
-      bar_sync(pair, 64);                                 // (both have the scores in registers, too: P may go over them)
+      bar_sync(pair, 64);
       const float mx = max3_nan(__uint_as_float(own << 16), __uint_as_float(static_cast<uint32_t>(top_s[(half ^ 1u) * 128u]) << 16), -INFINITY) * sl2;
       bool grow = mx > m_used + kGrow;
       float alpha = 1.0f;
@@ -597,17 +622,22 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
         l *= alpha;
         m_used = mx;
       }
-      float v_mul[2] = {1.0f, 1.0f};
+      float v_mul[4] = {1.0f, 1.0f, 1.0f, 1.0f};          // of 16 columns each
       if (Q8) {
-        const float4 v4 = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u]);
-        const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+        const float4 va = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u]), vb = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u] + 4);
+        const float vv[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
         float top = v_ref;
+        if (whole) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool seen = hi > 32 * k && lo < 32 * k + 32;
-          top = seen ? fmaxf(top, fabsf(vv[k])) : top;
-          // scales far apart, and some of the keys not seen by the row: they may have set the power
-          redo = redo || (seen && vv[k] < 0.0f && (lo > 32 * k || hi < 32 * k + 32));
+          for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(vv[k]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const bool seen = hi > 16 * k && lo < 16 * k + 16;
+            top = seen ? fmaxf(top, fabsf(vv[k])) : top;
+            // scales far apart, and some of the keys not seen by the row: they may have set the power
+            redo = redo || (seen && vv[k] < 0.0f && (lo > 16 * k || hi < 16 * k + 16));
+          }
         }
         if (top > v_ref) {
           alpha *= v_ref / top;                           // (a power of two, or 0 at first)
@@ -615,7 +645,10 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
           grow = true;
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) v_mul[k] = v_ref > 0.0f ? fminf(fabsf(half ? vv[2 + k] : vv[k]) / v_ref, 1.0f) * kCkPScale : 0.0f;
+        for (int k = 0; k < 4; ++k) {                     // (columns that the row does not see may have a larger power)
+          const float own = fabsf(half ? vv[4 + k] : vv[k]);
+          v_mul[k] = v_ref > 0.0f ? fminf(own * __uint_as_float((254u << 23) - __float_as_uint(v_ref)), 1.0f) * kCkPScale : 0.0f;
+        }
       }
       if (j > b0 && __any_sync(0xffffffffu, grow)) {      // (these scores came after the products before them: O is at rest)
 #pragma unroll 1
@@ -635,22 +668,23 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
       u64 sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
+        uint32_t x[32], pk[16];
+        scores(c, x);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float e0, e1;
-          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), sl2_2, neg_2), e0, e1);
+          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sl2_2, neg_2), e0, e1);
           e0 = fast_ex2(e0);
           e1 = fast_ex2(e1);
           sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
           if (Q8) {
-            e0 *= v_mul[c];
-            e1 *= v_mul[c];
+            e0 *= v_mul[2 * c + (i >> 3)];
+            e1 *= v_mul[2 * c + (i >> 3)];
           }
           pk[i] = BF && !Q8 ? cvt_bf16x2(e1, e0) : cvt_f16x2(e1, e0);
         }
         __syncwarp();
-        tc_st16(s_addr + 32u * half + 16u * c, pk);
+        tc_st16(s_addr + 64u * half + 16u * c, pk);         // (over scores that were read)
       }
       tc_wait_st();
       tc_fence_before_sync();
@@ -751,8 +785,9 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
 }
 
 template <bool BF, bool Q8, int HD>
-__global__ void __launch_bounds__(kCkThreads, 1) b2_attend_chunk(const __grid_constant__ AttendArgs a) {
-  using Sh = ChunkShape<HD>;
+__global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(const __grid_constant__ AttendArgs a) {
+  using Sh = ChunkShape<Q8, HD>;
+  constexpr uint32_t kLoadWarps = ChunkWarps<Q8>::kLoad, kCkThreads = ChunkWarps<Q8>::kThreads;
   extern __shared__ __align__(1024) uint8_t sm[];
   ChunkShared *S = reinterpret_cast<ChunkShared *>(sm + Sh::kShared);
   const uint32_t tid = threadIdx.x, w = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -796,17 +831,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) b2_attend_chunk(const __grid_co
   __syncthreads();
   tc_fence_after_sync();
   if (w < kSoftWarps) {
-    more_registers<Q8 ? kSoftRegs8 : kSoftRegs>();
+    more_registers<ChunkWarps<Q8>::kSoft>();
     chunk_rows<BF, Q8, HD>(a, sm, S);
   } else if (w < kSoftWarps + kLoadWarps) {
-    if constexpr (Q8) more_registers<kLoadRegs8>();       // (a count above the launch's is raised, one below it lowered: the other way round is no instruction)
-    else fewer_registers<kLoadRegs>();
+    if constexpr (!Q8) fewer_registers<ChunkWarps<Q8>::kFill>();
     Walk wk;
     wk.seek(a, cap, seq, before, x0);
     chunk_load<BF, Q8, HD>(a, wk, x0, x1, sm, S);
   } else {
-    fewer_registers<kIssueRegs>();
-    if (w == kSoftWarps + kLoadWarps) chunk_products<Q8 || !BF, HD>(sm, S);
+    fewer_registers<ChunkWarps<Q8>::kIssue>();
+    if (w == kSoftWarps + kLoadWarps) chunk_products<Q8 || !BF, Q8, HD>(sm, S);
   }
   __syncwarp();
   tc_fence_before_sync();
@@ -956,13 +990,13 @@ __global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_cons
 template <bool BF, bool Q8, int HD>
 int Launch(const AttendArgs &a, uint32_t sms, cudaStream_t stream) {
   if (sms > kMostRuns) sms = kMostRuns;
-  b2_attend_chunk<BF, Q8, HD><<<sms, kCkThreads, ChunkSmem<HD>(), stream>>>(a);
+  b2_attend_chunk<BF, Q8, HD><<<sms, ChunkWarps<Q8>::kThreads, ChunkSmem<Q8, HD>(), stream>>>(a);
   if (sms > 1u) b2_attend_join<HD><<<(sms - 1u) * (kChunkRows / kJoinRows), kJoinThreads, 0, stream>>>(a, sms);
   return static_cast<int>(cudaGetLastError());
 }
 template <bool BF, bool Q8, int HD>
 cudaError_t Attr() {
-  return cudaFuncSetAttribute(b2_attend_chunk<BF, Q8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ChunkSmem<HD>()));
+  return cudaFuncSetAttribute(b2_attend_chunk<BF, Q8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ChunkSmem<Q8, HD>()));
 }
 
 }  // namespace
