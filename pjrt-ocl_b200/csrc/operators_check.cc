@@ -83,11 +83,12 @@ std::string CheckAttend(const b2_cache_desc &d, const b2_batch *b, const b2_rows
   std::string m = CheckBatch(b);
   if (!m.empty()) return m;
   if (d.row_dtype == B2_F32) return "attention of f32 rows (f16 or bf16)";
-  if (!(scale > 0.0f && isfinite(scale))) return "scale must be positive and finite";
+  if (!(scale > 0.0f && scale <= 1e38f)) return "scale must be positive and at most 1e38";
   if (window && !causal) return "a window needs causal";
   if (window > 0x7fffffffu) return "window " + N(window) + " (below 2^31)";
   if (reinterpret_cast<uintptr_t>(lse) % 4) return "lse must be 4-byte aligned";
   if ((m = CheckRows("q", q, b->n_rows, d.q_heads, d.row_dtype)).empty()) m = CheckRows("out", o, b->n_rows, d.q_heads, d.row_dtype);
+  if (m.empty() && b->n_rows && q->data == o->data) m = "out lies over q (a row of q may be read after its result is there)";
   return m;
 }
 
