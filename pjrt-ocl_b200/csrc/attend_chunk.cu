@@ -14,10 +14,11 @@
 // The ring holds blocks in the 128-byte-swizzled layout that the tensor cores read, filled page by page: pages have any size, so a row
 // of the cache is found by itself (one page number a row, looked up a block ahead).
 // 8-bit pages: codes become f16 on their way into the ring. K's exactly, its scales go onto the scores, in f32; q is scaled by a power of two
-// for each row to fit f16. V's times their key's scale relative to a power of two above the scales of 16 keys side by side (rounded to 2^-12
-// of themselves, as the weights are); the power goes onto the weights. (V exact, too, with its scales on the weights: 1015 us instead of
-// 793 for 2048 rows behind 14336 of 32 heads of 128 values. A warp that reads 64 scales waits for 8 KB of them.) The codes of a block
-// ahead wait in shared memory as they are, copied asynchronously (in registers: 1045 us).
+// for each row to fit f16. V's, for bf16 rows, times their key's scale relative to a power of two above the scales of 16 keys side by side
+// (rounded to 2^-12 of themselves, as the weights are), the power goes onto the weights; f16 rows' results are rounded no coarser than that
+// themselves, so for them V is exact, too, and its scales go onto the weights before those are rounded. (A warp that reads 64 scales waits
+// for 8 KB of them: 897 us instead of 791 for 2048 rows behind 14336 of 32 heads of 128 values.) The codes of a block ahead wait in
+// shared memory as they are, copied asynchronously (in registers: 1045 us).
 //
 // Work: one CTA to an SM. The tiles of the batch in a row, sequence by sequence and head by head, each weighed by the keys it sees and something for its
 // beginning and end, are dealt to the CTAs in equal runs, whatever their number and lengths; a run that ends inside a tile ends between
@@ -47,12 +48,15 @@ constexpr float kGrow = 8.0f;                             // log2 of the growth 
 constexpr float kCkPScale = 64.0f;                        // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
 constexpr unsigned long long kBudget = 2000000000ull;     // ns that a wait may take
 
-template <bool Q8, int HD>
+template <bool BF, bool Q8, int HD>
 struct ChunkShape {
   static constexpr uint32_t kHalf = 128u * 128u;          // 128 rows of 64 values
   static constexpr uint32_t kBlock = kHalf * (HD / 64);   // Q of a slot, K or V of a block
-  static constexpr uint32_t kStages = HD == 64 ? 8 : Q8 ? 4 : 5;
-  static constexpr uint32_t kQ = 0, kRing = 2 * kBlock, kCodes = kRing + kStages * kBlock, kScales = kCodes + (Q8 ? kBlock : 0u), kTops = kScales + (Q8 ? 1024u : 0u), kShared = kTops + 1024u;      // codes of K and V of a block; K's scales of two; what the softmax warps tell each other
+  static constexpr bool kExactV = Q8 && !BF;              // V's scales go onto the weights
+  static constexpr uint32_t kStages = HD == 64 ? 8 : kExactV ? 3 : Q8 ? 4 : 5;
+  // Q, the ring, codes of K and V of a block, scales of two blocks, what the softmax warps tell each other
+  static constexpr uint32_t kQ = 0, kRing = 2 * kBlock, kCodes = kRing + kStages * kBlock, kScales = kCodes + (Q8 ? kBlock : 0u);
+  static constexpr uint32_t kTops = kScales + (kExactV ? 2048u : Q8 ? 1024u : 0u), kShared = kTops + 1024u;
 };
 // A tile's part that a CTA works on: packed rows [r0, r0 + rows) of a sequence (row x group + head), blocks [b0, b1) of the `blocks` of keys from
 // keys.lo that any of them sees.
@@ -71,9 +75,11 @@ struct ChunkShared {
     int8_t q_exp[256];                                    // 8-bit pages: each row of q was scaled by 2^e
   };
 };
-template <bool Q8, int HD>
-constexpr uint32_t ChunkSmem() { return ChunkShape<Q8, HD>::kShared + ((sizeof(ChunkShared) + 15u) & ~15u); }
-static_assert(ChunkSmem<false, 128>() <= 227u * 1024u && ChunkSmem<true, 128>() <= 227u * 1024u && ChunkSmem<true, 64>() <= 227u * 1024u, "shared memory of an SM");
+template <bool BF, bool Q8, int HD>
+constexpr uint32_t ChunkSmem() { return ChunkShape<BF, Q8, HD>::kShared + ((sizeof(ChunkShared) + 15u) & ~15u); }
+constexpr bool ChunkFits(uint32_t bytes) { return bytes <= 227u * 1024u; }
+static_assert(ChunkFits(ChunkSmem<true, false, 128>()) && ChunkFits(ChunkSmem<true, true, 128>()) && ChunkFits(ChunkSmem<false, true, 128>()) &&
+                  ChunkFits(ChunkSmem<false, true, 64>()), "shared memory of an SM");
 
 // ---- how the work is dealt ----
 typedef unsigned long long u64;
@@ -192,7 +198,7 @@ __device__ __forceinline__ void clear_rows(const AttendArgs &a, const Tile &t, u
 // Rows of q into shared memory, a 16-byte chunk to a thread. As they are they come by asynchronous copies (still under way on return).
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void load_q(const AttendArgs &a, const Tile &t, uint32_t tid, uint32_t base, int8_t *q_exp) {
-  using Sh = ChunkShape<Q8, HD>;
+  using Sh = ChunkShape<BF, Q8, HD>;
   constexpr uint32_t QL = HD / 8, AT = ChunkWarps<Q8>::kLoad * 32u / QL;      // threads to a row, rows at once
   const bool vec = ((reinterpret_cast<uintptr_t>(a.q.p) & 15u) | ((a.q.row | a.q.head) & 7)) == 0;
   const uint32_t c = tid % QL, r0 = tid / QL, rows = t.rows > kCkRows ? 256u : 128u;
@@ -252,7 +258,7 @@ static __device__ __forceinline__ void load_q(const AttendArgs &a, const Tile &t
 
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk, u64 x0, u64 x1, uint8_t *sm, ChunkShared *S) {
-  using Sh = ChunkShape<Q8, HD>;
+  using Sh = ChunkShape<BF, Q8, HD>;
   constexpr uint32_t NS = Sh::kStages;
   volatile uint32_t *failed = &S->failed;
   const uint64_t cap = capacity_of(a.c, a.b);
@@ -330,7 +336,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
       uint32_t h[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) h[q] = cvt_e4m3x2_f16x2(q & 1 ? c[q >> 1] >> 16 : c[q >> 1] & 0xffffu);
-      if (v) {
+      if (v && !Sh::kExactV) {
         const float m = __shfl_sync(0xffffffffu, mul, r0);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
@@ -424,7 +430,11 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         }
         ok = __all_sync(0xffffffffu, free);
         if (!ok) break;
-        if (lane < RW) *reinterpret_cast<float *>(sm + Sh::kScales + buf * 512u + (RW * w + lane) * 4u) = ksc;
+        if (lane < RW) {
+          float *const s = reinterpret_cast<float *>(sm + Sh::kScales + buf * 512u) + RW * w + lane;
+          *s = ksc;
+          if (Sh::kExactV) s[256] = vsc;
+        }
         // V's power of two: above the scales of the warp's keys that are finite
         const uint32_t vb = lane < RW && (__float_as_uint(vsc) & 0x7fffffffu) < 0x7f800000u ? __float_as_uint(vsc) & 0x7fffffffu : 0u;
         const uint32_t most = __reduce_max_sync(0xffffffffu, vb), least = __reduce_min_sync(0xffffffffu, vb ? vb : 0x7f7fffffu);
@@ -459,13 +469,13 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
 }
 
 // ---- the issuing warp -----------------------------------------------------------------------
-template <bool F16, bool Q8, int HD>
+template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_products(uint8_t *sm, ChunkShared *S) {
-  using Sh = ChunkShape<Q8, HD>;
+  using Sh = ChunkShape<BF, Q8, HD>;
   constexpr uint32_t NS = Sh::kStages;
   volatile uint32_t *failed = &S->failed;
   const uint32_t base = smem_addr(sm), tmem = S->tmem;
-  const uint32_t fmt = F16 ? 0u : 1u;
+  const uint32_t fmt = Q8 || !BF ? 0u : 1u;
   const uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kCkKeys >> 3) << 17) | ((kCkRows >> 4) << 24);
   const uint32_t idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) | ((static_cast<uint32_t>(HD) >> 3) << 17) | ((kCkRows >> 4) << 24);
   const uint64_t dq = tc_desc(base + Sh::kQ, 16u, 1024u), dk = tc_desc(base + Sh::kRing, 16u, 1024u), dv = tc_desc(base + Sh::kRing, Sh::kHalf, 1024u);
@@ -544,7 +554,7 @@ __device__ __forceinline__ uint32_t rounded_up(float x) {
 }
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *sm, ChunkShared *S) {
-  using Sh = ChunkShape<Q8, HD>;
+  using Sh = ChunkShape<BF, Q8, HD>;
   volatile uint32_t *failed = &S->failed;
   const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u, s = w >> 3, half = (w >> 2) & 1u, q4 = w & 3u;
   const uint32_t r = s * kCkRows + 32u * q4 + lane;       // the thread's row, of whose keys it has columns 64 half .. + 63
@@ -622,7 +632,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
         l *= alpha;
         m_used = mx;
       }
-      float v_mul[4] = {1.0f, 1.0f, 1.0f, 1.0f};          // of 16 columns each
+      float v_mul[4] = {1.0f, 1.0f, 1.0f, 1.0f};          // of 16 columns each (exact V: the same for all, beside each one's scale)
       if (Q8) {
         const float4 va = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u]), vb = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u] + 4);
         const float vv[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
@@ -646,8 +656,9 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {                     // (columns that the row does not see may have a larger power)
-          const float own = fabsf(half ? vv[4 + k] : vv[k]);
-          v_mul[k] = v_ref > 0.0f ? fminf(own * __uint_as_float((254u << 23) - __float_as_uint(v_ref)), 1.0f) * kCkPScale : 0.0f;
+          const float own = Sh::kExactV ? 1.0f : fabsf(half ? vv[4 + k] : vv[k]);
+          v_mul[k] = v_ref > 0.0f ? own * __uint_as_float((254u << 23) - __float_as_uint(v_ref)) * kCkPScale : 0.0f;
+          if (!Sh::kExactV) v_mul[k] = fminf(v_mul[k], kCkPScale);
         }
       }
       if (j > b0 && __any_sync(0xffffffffu, grow)) {      // (these scores came after the products before them: O is at rest)
@@ -678,8 +689,15 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
           e1 = fast_ex2(e1);
           sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
           if (Q8) {
-            e0 *= v_mul[2 * c + (i >> 3)];
-            e1 *= v_mul[2 * c + (i >> 3)];
+            float f0 = v_mul[2 * c + (i >> 3)], f1 = f0;
+            if (Sh::kExactV) {
+              // (a scale that the row does not see may be anything)
+              const float2 v2 = *reinterpret_cast<const float2 *>(ks + 256 + 32 * c + 2 * i);
+              f0 *= whole || (32 * c + 2 * i >= lo_h && 32 * c + 2 * i < hi_h) ? v2.x : 0.0f;
+              f1 *= whole || (32 * c + 2 * i + 1 >= lo_h && 32 * c + 2 * i + 1 < hi_h) ? v2.y : 0.0f;
+            }
+            e0 *= f0;
+            e1 *= f1;
           }
           pk[i] = BF && !Q8 ? cvt_bf16x2(e1, e0) : cvt_f16x2(e1, e0);
         }
@@ -786,7 +804,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
 
 template <bool BF, bool Q8, int HD>
 __global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(const __grid_constant__ AttendArgs a) {
-  using Sh = ChunkShape<Q8, HD>;
+  using Sh = ChunkShape<BF, Q8, HD>;
   constexpr uint32_t kLoadWarps = ChunkWarps<Q8>::kLoad, kCkThreads = ChunkWarps<Q8>::kThreads;
   extern __shared__ __align__(1024) uint8_t sm[];
   ChunkShared *S = reinterpret_cast<ChunkShared *>(sm + Sh::kShared);
@@ -840,7 +858,7 @@ __global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(c
     chunk_load<BF, Q8, HD>(a, wk, x0, x1, sm, S);
   } else {
     fewer_registers<ChunkWarps<Q8>::kIssue>();
-    if (w == kSoftWarps + kLoadWarps) chunk_products<Q8 || !BF, Q8, HD>(sm, S);
+    if (w == kSoftWarps + kLoadWarps) chunk_products<BF, Q8, HD>(sm, S);
   }
   __syncwarp();
   tc_fence_before_sync();
@@ -990,13 +1008,13 @@ __global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_cons
 template <bool BF, bool Q8, int HD>
 int Launch(const AttendArgs &a, uint32_t sms, cudaStream_t stream) {
   if (sms > kMostRuns) sms = kMostRuns;
-  b2_attend_chunk<BF, Q8, HD><<<sms, ChunkWarps<Q8>::kThreads, ChunkSmem<Q8, HD>(), stream>>>(a);
+  b2_attend_chunk<BF, Q8, HD><<<sms, ChunkWarps<Q8>::kThreads, ChunkSmem<BF, Q8, HD>(), stream>>>(a);
   if (sms > 1u) b2_attend_join<HD><<<(sms - 1u) * (kChunkRows / kJoinRows), kJoinThreads, 0, stream>>>(a, sms);
   return static_cast<int>(cudaGetLastError());
 }
 template <bool BF, bool Q8, int HD>
 cudaError_t Attr() {
-  return cudaFuncSetAttribute(b2_attend_chunk<BF, Q8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ChunkSmem<Q8, HD>()));
+  return cudaFuncSetAttribute(b2_attend_chunk<BF, Q8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ChunkSmem<BF, Q8, HD>()));
 }
 
 }  // namespace
