@@ -65,6 +65,14 @@ struct Tile {
   Seq s;
   Span keys;
 };
+// What a CTA tells the launch that joins: the tile whose first blocks end its run (no rows: none), and its blocks of the tile in which the run
+// begins. Behind the parts in the scratch.
+struct Join {
+  Tile tile;
+  uint32_t b0, b1;
+};
+constexpr size_t kPartFloats = kChunkRows * (128u + 2u);  // (room for a part of 128 values a row)
+__device__ __forceinline__ Join *joins_of(const AttendArgs &a, uint32_t most) { return reinterpret_cast<Join *>(a.part + most * 2u * kPartFloats); }
 struct ChunkShared {
   uint64_t q_full, q_free, full[8], empty[8], s_full[2], p_full[2], pv_done[2], scales_free[2][2];
   uint32_t tmem, failed;
@@ -363,6 +371,11 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
       more = wk.at < x1;
       if (!more) break;
       wk.tile(a, x0, x1, t);
+      if (tid == 0u) {
+        Join *const j = joins_of(a, gridDim.x) + blockIdx.x;
+        if (wk.at < x0) { j->b0 = t.b0; j->b1 = t.b1; }
+        if (t.b0 == 0u && t.b1 != 0u && t.b1 != t.blocks) j->tile = t;
+      }
       // (rows that see no key are cleared by the CTA in whose run the tile begins)
       if (t.blocks == 0u) {
         if (wk.at >= x0) clear_rows(a, t, tid, ChunkWarps<Q8>::kLoad * 32u);
@@ -816,6 +829,11 @@ __global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(c
       if (q.bad) cache_fault(a.c.status, kStBadBatch, i, static_cast<uint32_t>(q.bad), static_cast<uint32_t>(q.value));
     }
   }
+  if (tid == 0u) {                                        // (what is there is of the call before)
+    Join *const j = joins_of(a, gridDim.x) + blockIdx.x;
+    j->tile.rows = 0u;
+    j->b0 = j->b1 = 0u;
+  }
   u64 all = 0ull;
   for (uint32_t i = tid; i < a.b.n_seqs; i += kCkThreads) all += units_of_seq(a, cap, i);
   all = warp_reduce(all, [](u64 x, u64 y) { return x + y; });
@@ -876,47 +894,29 @@ __global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(c
   }
 }
 
-// Tiles that lie in the runs of several CTAs: a warp to a row, the parts in their order. A CTA for each border between two runs (and 32 rows): it has
-// something to do if the border lies between two blocks of a tile, and is the tile's first that does.
+// Tiles that lie in the runs of several CTAs: a warp to a row, the parts in their order. For each CTA whose run ends inside a tile that it began,
+// a CTA of 32 rows at a time. (What to join was written down by the launch before: worked out here again, with 64-bit quotients in every warp, it
+// was 37 us for 2048 rows behind 14336 of 32 heads of 128 values.)
 constexpr uint32_t kJoinThreads = 256, kJoinRows = 32, kMostRuns = 1024;
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_constant__ AttendArgs a, uint32_t most) {
-  __shared__ u64 find[kJoinThreads / 32 + 2];
-  const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint64_t cap = capacity_of(a.c, a.b);
-  u64 all = 0ull;
-  for (uint32_t i = threadIdx.x; i < a.b.n_seqs; i += kJoinThreads) all += units_of_seq(a, cap, i);
-  all = warp_reduce(all, [](u64 x, u64 y) { return x + y; });
-  if (lane == 0u) find[w] = all;
-  __syncthreads();
-  all = 0ull;
-  for (uint32_t i = 0; i < kJoinThreads / 32u; ++i) all += find[i];
-  const uint32_t ctas = ctas_of(a, all, most), border = 1u + blockIdx.x / (kChunkRows / kJoinRows);
-  if (all == 0ull || border >= ctas) return;
-  const Runs runs(all, ctas);
-  const u64 x = runs.begin(border), x_before = runs.begin(border - 1u);
-  uint32_t seq;
-  u64 before;
-  if (!find_unit<kJoinThreads>(a.b.n_seqs, x, find, [&](uint32_t i) { return units_of_seq(a, cap, i); }, seq, before)) return;
-  Walk wk;
-  wk.seek(a, cap, seq, before, x);
-  Tile t;
-  wk.tile(a, x_before, x, t);
-  if (t.b0 != 0u || t.b1 == 0u || t.b1 == t.blocks) return;
-  // the parts: CTAs from `border` - 1 on whose runs have blocks of the tile, the first of them from block 0
+  const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u, begun = blockIdx.x / (kChunkRows / kJoinRows);
+  const Join *const joins = joins_of(a, most);
+  if (joins[begun].tile.rows <= (blockIdx.x % (kChunkRows / kJoinRows)) * kJoinRows) return;
+  const Tile t = joins[begun].tile;
   constexpr uint32_t kPart = kChunkRows * (HD + 2u);
   __shared__ uint32_t part_s[kMostRuns], n_parts;
-  if (threadIdx.x == 0u) n_parts = 0u;
-  __syncthreads();
   if (w == 0u) {
-    uint32_t n = 0u;
-    for (uint32_t c0 = border - 1u; c0 < ctas; c0 += 32u) {
-      const uint32_t c = c0 + lane;
-      const uint32_t lo = c < ctas ? wk.block_at(t.blocks, runs.begin(c)) : t.blocks, hi = c < ctas ? wk.block_at(t.blocks, runs.begin(c + 1u)) : t.blocks;
-      const uint32_t m = __ballot_sync(0xffffffffu, lo < hi);
-      if (lo < hi) part_s[n + __popc(m & ((1u << lane) - 1u))] = c * 2u + (lo == 0u ? 1u : 0u);
+    uint32_t n = 1u;
+    if (lane == 0u) part_s[0] = begun * 2u + 1u;
+    for (uint32_t c0 = begun + 1u; c0 < most; c0 += 32u) {
+      const uint32_t c = c0 + lane, lo = c < most ? joins[c].b0 : 0u, hi = c < most ? joins[c].b1 : 0u;
+      const uint32_t end = __ballot_sync(0xffffffffu, hi == t.blocks), upto = end ? 2u << (__ffs(end) - 1u) : 0u;      // (lanes up to the one with the last block)
+      const bool has = lo < hi && (upto == 0u || ((upto - 1u) >> lane) & 1u);
+      const uint32_t m = __ballot_sync(0xffffffffu, has);
+      if (has) part_s[n + __popc(m & ((1u << lane) - 1u))] = c * 2u;
       n += __popc(m);
-      if (__any_sync(0xffffffffu, hi == t.blocks)) break;
+      if (end) break;
     }
     if (lane == 0u) n_parts = n;
   }
@@ -1025,7 +1025,7 @@ int PrepareAttendChunk() {
     if (e != cudaSuccess) return static_cast<int>(e);
   return 0;
 }
-size_t AttendChunkPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * 2u * kChunkRows * (128u + 2u) * sizeof(float); }
+size_t AttendChunkPartialBytes(uint32_t sms) { return static_cast<size_t>(sms) * (2u * kPartFloats * sizeof(float) + sizeof(Join)); }
 
 int LaunchAttendChunk(const AttendArgs &a, uint32_t sms, CUstream_st *stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -24,8 +24,6 @@ template <> __device__ __forceinline__ __nv_bfloat16 FromF<__nv_bfloat16>(float 
 // V values next to each other, moved as one access.
 template <typename T, int V> struct __align__(sizeof(T) * V) Vec { T v[V]; };
 
-__device__ __forceinline__ uint32_t warp_sum_u32(uint32_t v) { return warp_reduce(v, [](uint32_t a, uint32_t b) { return a + b; }); }
-
 // The first fault a cache's calls meet stays in its status words.
 __device__ __forceinline__ void cache_fault(uint32_t *status, uint32_t code, uint32_t seq, uint32_t where, uint32_t detail) {
   if (atomicCAS(status, 0u, code) == 0u) {
