@@ -311,7 +311,8 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
   const bool in_hd = sub * 16u < a.c.hd * (Q8 ? 1u : 2u);
   auto copy = [&](const uint8_t *pages, uint32_t i, int64_t off, uint32_t mask) {
     const uint32_t dst = base + Sh::kRing + (i % NS) * Sh::kBlock;
-#pragma unroll
+    // (all 16 in a row are more code to fetch: 477 us instead of 464; two at a time 479)
+#pragma unroll 4
     for (uint32_t k = 0; k < N; ++k) {
       const uint32_t r = k * AT + r1;
       const int64_t o = __shfl_sync(0xffffffffu, off, r);
