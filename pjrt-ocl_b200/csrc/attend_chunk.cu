@@ -17,13 +17,16 @@
 // for each row to fit f16. V's, for bf16 rows, times their key's scale relative to a power of two above the scales of 16 keys side by side
 // (rounded to 2^-12 of themselves, as the weights are), the power goes onto the weights; f16 rows' results are rounded no coarser than that
 // themselves, so for them V is exact, too, and its scales go onto the weights before those are rounded. (A warp that reads 64 scales waits
-// for 8 KB of them: 897 us instead of 791 for 2048 rows behind 14336 of 32 heads of 128 values.) The codes of a block ahead wait in
+// for 8 KB of them: 876 us instead of 785 for 2048 rows behind 14336 of 32 heads of 128 values.) The codes of a block ahead wait in
 // shared memory as they are, copied asynchronously (in registers: 1045 us).
 //
 // Work: one CTA to an SM. The tiles of the batch in a row, sequence by sequence and head by head, each weighed by the keys it sees and something for its
 // beginning and end, are dealt to the CTAs in equal runs, whatever their number and lengths; a run that ends inside a tile ends between
 // two blocks of its keys, and a second launch joins the parts. The filling warps walk the run; the others read what they need of a tile
 // from shared memory. The ring runs on from tile to tile.
+//
+// Bound: the tensor cores, under the power cap. 2048 rows behind 14336 of 32 heads of 128 values, bf16: 464 us, 80 % of the rate that a large
+// product sustains; without exponentials and copies it would be 356.
 #include <type_traits>
 
 #include "attend_common.cuh"

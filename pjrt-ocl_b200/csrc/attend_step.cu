@@ -6,7 +6,7 @@
 //
 // Bound: HBM, K and V of every visible key read once.
 // Work: a cache head of a sequence is an item, cut into tiles of 16 or 32 keys. The tiles of the whole batch in a row, with some for
-// what an item costs beside its tiles, are dealt to the CTAs in equal runs (one CTA to an SM), whatever the lengths. A CTA's warps take
+// what an item costs beside its tiles, are dealt to the CTAs in equal runs, whatever the lengths. A CTA's warps take
 // its tiles in turn, each through two stages of its own (K and V of a tile, 8 KB, by 16-byte asynchronous copies, page by page): no barrier
 // stands between tiles. At an item's end the warps' (m, l, o) are joined through the stage each has free; an item that is split between
 // CTAs leaves partial results, and the CTA that comes last joins them in the CTAs' order.
@@ -691,7 +691,8 @@ template <bool BF, bool Q8, int HD, int NR, int NW>
 cudaError_t Attr() {
   return cudaFuncSetAttribute(b2_attend_step<BF, Q8, HD, NR, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, StepShape<Q8, HD, NR, NW>::kSmem);
 }
-// 9 to 16 rows: CTAs of eight warps, whose threads may have 255 registers (with twelve warps and 168, 500 bytes of them were spilled: 32 sequences of 4000 to 8000 tokens, 16 heads to each of 4 cache heads, 8-bit pages: 81 us, 111 so).
+// 9 to 16 rows: CTAs of eight warps, whose threads may have 255 registers (with twelve warps and 168, 500 bytes of them were spilled: 32 sequences
+// of 4000 to 8000 tokens, 16 heads to each of 4 cache heads, 8-bit pages: 81 us, 111 so).
 // Up to 8 rows: items (sequences x cache heads) for no more than the SMs go to CTAs of twelve warps, of which few share an item (8 heads of 131000 keys,
 // bf16: 90 us, 137 with CTAs of three); more items to CTAs of three, which lose less at an item's end (64 sequences of 200 to 16000 tokens, 8 heads, 8-bit
 // pages: 110 us, 120 with CTAs of six).

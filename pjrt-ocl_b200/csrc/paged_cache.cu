@@ -7,6 +7,8 @@
 // Bound: HBM, each row read and written once. A warp takes a token (few tokens: a part of its rows): it looks up the token's sequence, 32 starts
 // at a time, and where its position lies, while the rows of the token before are on the way, and moves the 2 x heads rows, 8 values
 // each of both halves of a row to a thread, a row of K and one of V in flight to each group of threads. No barrier anywhere.
+// Measured, bf16 rows and e4m3 pages of 128 values: written 27 us (53 % of the copy rate; 2.8 instructions of 4 a cycle go to maxima, quotients and
+// conversions), read back 39 us (80 %).
 #include <type_traits>
 
 #include "operators_dev.cuh"
