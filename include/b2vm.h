@@ -315,7 +315,8 @@ b2_status b2_cache_read(b2_cache *cache, const b2_batch *batch, const b2_rows *k
  * own position, of these the last `window` (0 = all); else every position of its sequence (window must be 0). Values
  * that a row does not see never reach it, whatever they are. A row that sees nothing gives zeros. lse (may be NULL):
  * f32 [n_rows][q_heads], the logarithm of the softmax's sum (-inf for a row that sees nothing). Rows are B2_F16 or
- * B2_BF16. 0 < scale <= 1e38. out must not lie over q. e4m3 scales count in full from 2^-80 to 2^103. */
+ * B2_BF16. 0 < scale <= 1e38; max_rows x query heads to a cache head below 2^31. out must not lie over q. e4m3 scales
+ * count in full from 2^-80 to 2^103. */
 b2_status b2_cache_attend(b2_cache *cache, b2_scratch *scratch, const b2_batch *batch, const b2_rows *q, float scale,
                           int causal, uint32_t window, const b2_rows *out, void *lse, void *cuda_stream, char *err,
                           size_t err_cap);

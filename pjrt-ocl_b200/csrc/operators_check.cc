@@ -88,6 +88,9 @@ std::string CheckAttend(const b2_cache_desc &d, const b2_batch *b, const b2_rows
   if (window > 0x7fffffffu) return "window " + N(window) + " (below 2^31)";
   if (reinterpret_cast<uintptr_t>(lse) % 4) return "lse must be 4-byte aligned";
   if ((m = CheckRows("q", q, b->n_rows, d.q_heads, d.row_dtype)).empty()) m = CheckRows("out", o, b->n_rows, d.q_heads, d.row_dtype);
+  // (a sequence's rows x group are numbered in 31 bits)
+  const uint64_t most = b->max_rows && b->max_rows < b->n_rows ? b->max_rows : b->n_rows;
+  if (m.empty() && most * (d.q_heads / d.heads) > 0x7fffffffu) m = "rows of a sequence x q_heads / heads: " + N(most) + " x " + N(d.q_heads / d.heads) + " (below 2^31)";
   if (m.empty() && b->n_rows && q->data == o->data) m = "out lies over q (a row of q may be read after its result is there)";
   return m;
 }

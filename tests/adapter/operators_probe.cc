@@ -148,6 +148,11 @@ static void Refusals() {
   Refused("window", attend(&q, &o, 0.125f, 0, 5, nullptr), "needs causal");
   Refused("window", attend(&q, &o, 0.125f, 1, 0x80000000u, nullptr), "window");
   Refused("lse", attend(&q, &o, 0.125f, 1, 0, mem + 2), "lse");
+  b2_batch many = b;
+  many.n_rows = 0x40000000u;                              // (two heads to a cache head)
+  Refused("2^31 rows x heads", b2::CheckAttend(c, &many, &q, &o, 0.125f, 1, 0, nullptr), "below 2^31");
+  many.max_rows = 1000;
+  Fine("of which a sequence has few", b2::CheckAttend(c, &many, &q, &o, 0.125f, 1, 0, nullptr));
   b2_cache_desc f32 = c;
   f32.row_dtype = B2_F32;
   Refused("f32 rows", b2::CheckAttend(f32, &b, &q, &o, 0.125f, 1, 0, nullptr), "f32 rows");
