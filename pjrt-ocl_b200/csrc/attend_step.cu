@@ -17,8 +17,9 @@
 // 8-bit pages: codes are exact in f16, so the products are f16 x f16 whatever the rows' type. q of type bf16 is scaled by a power of
 // two for each row so that its largest value is near 2^14 (f16 then holds what bf16 held to 2^-38 of that); a key's scale goes onto its
 // scores, a value's onto p, relative to a power of two not below any scale that the row has seen (p v's factor stays in f16's normal range).
-// bf16 pages: p is split into two bf16 values (p and what rounding left), since the second product costs nothing here; the result is
-// then only rounded once, as it is stored.
+// p is split into two 16-bit values (p and what rounding left), since the second product costs little here (64 sequences of 200 to 16000 tokens, f16 rows,
+// 8-bit pages: 116 us, 113 without it; 16-bit pages: no difference); the result is then only
+// rounded once, as it is stored. Only bf16 rows over 8-bit pages do without: p in f16 is eight times finer than their results.
 #include "attend_common.cuh"
 
 namespace b2 {
@@ -503,7 +504,12 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
               pb[g][t][i] = transposed(r);
               pl[g][t][i] = transposed(cvt_bf16x2(hi - __uint_as_float(r & 0xffff0000u), lo - __uint_as_float(r << 16)));
             } else {
-              pb[g][t][i] = transposed(cvt_f16x2(hi, lo));
+              const uint32_t r = cvt_f16x2(hi, lo);
+              pb[g][t][i] = transposed(r);
+              if (!BF) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
+                pl[g][t][i] = transposed(cvt_f16x2(hi - f.y, lo - f.x));
+              }
             }
           }
         }
@@ -522,6 +528,7 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
                 mma_bf16_16816(o[g][n], x, pl[g][t][0], pl[g][t][1]);
               } else {
                 mma_f16_16816(o[g][n], x, pb[g][t][0], pb[g][t][1]);
+                mma_f16_16816(o[g][n], x, pl[g][t][0], pl[g][t][1]);
               }
             }
           }
@@ -535,7 +542,10 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
             const uint32_t c0 = __byte_perm(b[2 * t], 0u, 0x3120), c1 = __byte_perm(b[2 * t + 1], 0u, 0x3120);
             const uint32_t x[4] = {cvt_e4m3x2_f16x2(c0 & 0xffffu), cvt_e4m3x2_f16x2(c0 >> 16), cvt_e4m3x2_f16x2(c1 & 0xffffu), cvt_e4m3x2_f16x2(c1 >> 16)};
 #pragma unroll
-            for (int g = 0; g < NR; ++g) mma_f16_16816(o[g][n], x, pb[g][t][0], pb[g][t][1]);
+            for (int g = 0; g < NR; ++g) {
+              mma_f16_16816(o[g][n], x, pb[g][t][0], pb[g][t][1]);
+              if (!BF) mma_f16_16816(o[g][n], x, pl[g][t][0], pl[g][t][1]);
+            }
           }
         }
       }
