@@ -17,9 +17,9 @@
 // 8-bit pages: codes are exact in f16, so the products are f16 x f16 whatever the rows' type. q of type bf16 is scaled by a power of
 // two for each row so that its largest value is near 2^14 (f16 then holds what bf16 held to 2^-38 of that); a key's scale goes onto its
 // scores, a value's onto p, relative to a power of two not below any scale that the row has seen (p v's factor stays in f16's normal range).
-// p is split into two 16-bit values (p and what rounding left), since the second product costs little here (64 sequences of 200 to 16000 tokens, f16 rows,
-// 8-bit pages: 116 us, 113 without it; 16-bit pages: no difference); the result is then only
-// rounded once, as it is stored. Only bf16 rows over 8-bit pages do without: p in f16 is eight times finer than their results.
+// p is split into two 16-bit values (p and what rounding left), since the second product costs little here (64 sequences of 200 to 16000
+// tokens, f16 rows, 8-bit pages: 116 us, 113 without it; 16-bit pages: no difference); the result is then only rounded once, as it is
+// stored. Only bf16 rows over 8-bit pages do without: p in f16 is eight times finer than their results.
 #include "attend_common.cuh"
 
 namespace b2 {
