@@ -73,7 +73,7 @@ static __device__ __noinline__ void attend_row_alone(const AttendArgs &a, uint32
       float x[4];
       four(a.c.k + o + h * a.c.head_bytes, a.e4m3 ? a.c.ks[so + h * a.c.s_head] : 1.0f, x);
       const float sum = warp_reduce(q[0] * x[0] + q[1] * x[1] + q[2] * x[2] + q[3] * x[3], [](float u, float v) { return u + v; });
-      const float m2 = fmaxf(m, sum), c = m == -INFINITY ? 0.0f : exp2f(m - m2), p = m2 == -INFINITY ? 0.0f : exp2f(sum - m2);
+      const float m2 = fmaxf(m, sum), c = m == -INFINITY ? 0.0f : exp2f(m - m2), p = sum == -INFINITY ? 0.0f : exp2f(sum - m2);     // (a NaN loses in the maximum and stays in p)
       four(a.c.v + o + h * a.c.head_bytes, a.e4m3 ? a.c.vs[so + h * a.c.s_head] : 1.0f, x);
       l = l * c + p;
 #pragma unroll

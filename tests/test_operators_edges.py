@@ -1,0 +1,89 @@
+"""Attention over the paged cache where single values decide: scales far apart, NaN in one place, large scores, keys without a page.
+
+Tolerances count as those of the other operator tests; rows of bf16 over 8-bit pages round their values to 16 bits beside the
+weights, so there they are twice as wide (`_tol`)."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from conftest import package  # noqa: E402
+from operator_refs import Paged, half_step, normal  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.fixture(scope="module")
+def rt():
+    r = package().Runtime.Create(0)
+    yield r
+    r.close()
+
+
+@pytest.fixture(scope="module")
+def scratch(rt):
+    s = package().Scratch.Create(rt)
+    yield s
+    s.close()
+
+
+def _call(p, scratch, q, scale=None, **kw):
+    o, lse = torch.full_like(q, 9.0), torch.full(q.shape[:2], 9.0, device="cuda")
+    p.cache.Attend(p.batch, package().Rows.Of(q), package().Rows.Of(o), scratch, scale=scale, lse=lse.data_ptr(), stream=torch.cuda.current_stream().cuda_stream, **kw)
+    return o, lse
+
+
+def _tol(p, want, tol):
+    return tol * (2 if p.dtype == "e4m3" and p.row_dtype == "bf16" else 1) + half_step(p.row_dtype) * want.abs()
+
+
+def _near(got, want, tol):
+    return bool(((got.double() - want).abs() <= tol).all())
+
+
+def _place(p, b, pos):
+    return int(p.table[b, pos // p.page]), pos % p.page
+
+
+@pytest.mark.parametrize("dtype, row_dtype", [("bf16", "bf16"), ("f16", "f16"), ("e4m3", "bf16"), ("e4m3", "f16")])
+@pytest.mark.parametrize("rows, past, q_heads, window", [(2, 0, 2, 0), (5, 40, 6, 7), (60, 0, 8, 0), (130, 300, 4, 50), (40, 3000, 8, 0)])
+def test_a_nan_alone(rt, scratch, dtype, row_dtype, rows, past, q_heads, window):
+    """One NaN in K, in V, in a scale of either, or in q, at the first key that a row sees: it shows wherever it is seen."""
+    p = Paged(rt, [rows, 1], [past, 20], dtype=dtype, row_dtype=row_dtype, heads=2, q_heads=q_heads, dim=64, page=16, seed=5)
+    clean_q = normal((p.n_rows, q_heads, 64), row_dtype, 8)
+    want, want_lse, tol = p.attend(clean_q, 0.125, True, window)
+    tol, lse_tol = _tol(p, want, tol), 2.0 ** -19 * (1 + want_lse.abs())
+    clean = [x.clone() for x in p.pages], [None if s is None else s.clone() for s in p.scales]
+    row = torch.arange(past, past + rows, device="cuda")
+    head, group = 1, q_heads // 2
+    mine = torch.zeros(p.n_rows, q_heads, dtype=torch.bool, device="cuda")
+    for c in sorted({0, max(0, past - window + 1) if window else 0, past, past + 1}):
+        sees = (c <= row) & ((c > row - window) if window else True)
+        for what in ("k", "v", "q") + (("k scale", "v scale") if dtype == "e4m3" else ()):
+            q = clean_q.clone()
+            for i in range(2):
+                p.pages[i].copy_(clean[0][i])
+                if dtype == "e4m3":
+                    p.scales[i].copy_(clean[1][i])
+            mine[:] = False
+            mine[:rows, head * group:(head + 1) * group] = sees[:, None]
+            if what == "q":
+                mine[:] = False
+                mine[rows - 1, 1] = True
+                q[rows - 1, 1, 63] = NAN
+            elif what.endswith("scale"):
+                p.scales["kv".index(what[0])][(*_place(p, 0, c), head)] = NAN
+            elif dtype == "e4m3":
+                p.pages["kv".index(what)].view(torch.uint8)[(*_place(p, 0, c), head, 17)] = 0x7F
+            else:
+                p.pages["kv".index(what)][(*_place(p, 0, c), head, 17)] = NAN
+            o, lse = _call(p, scratch, q, window=window)
+            assert p.cache.Status()["code"] == 0
+            bad = mine[..., None].expand_as(o).clone()
+            if what == "v":
+                bad[..., :17] = bad[..., 18:] = False
+            assert bool((torch.isnan(o) == bad).all()), (c, what)
+            assert _near(o[~bad], want[~bad], tol[~bad]), (c, what)
+            lse_bad = mine if what in ("k", "q", "k scale") else torch.zeros_like(mine)
+            assert bool((torch.isnan(lse) == lse_bad).all()), (c, what)
+            assert _near(lse[~lse_bad], want_lse[~lse_bad], lse_tol[~lse_bad]), (c, what)
