@@ -49,6 +49,9 @@ struct ChunkWarps {
 constexpr uint32_t kCkCols = 512;                         // tensor memory: S0, S1 (128 columns each), O0, O1
 constexpr float kGrow = 8.0f;                             // log2 of the growth of a row maximum that forces a rescale
 constexpr float kCkPScale = 64.0f;                        // 8-bit pages: p (below 2^8) on the largest scale stays below 2^14
+// V's codes (at most 448) times their scale over a power above it are as large as f16 holds; with scales down to 2^-15 of the power, normal codes stay
+// normal. What a power is above 16 keys for loses no bits as long as their scales are within that: no more than 2^14 (by their exponents) apart.
+constexpr uint32_t kCkVLog = 7, kCkApart = 14;
 constexpr unsigned long long kBudget = 2000000000ull;     // ns that a wait may take
 
 template <bool BF, bool Q8, int HD>
@@ -456,7 +459,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         const uint32_t vb = lane < RW && (__float_as_uint(vsc) & 0x7fffffffu) < 0x7f800000u ? __float_as_uint(vsc) & 0x7fffffffu : 0u;
         const uint32_t most = __reduce_max_sync(0xffffffffu, vb), least = __reduce_min_sync(0xffffffffu, vb ? vb : 0x7f7fffffu);
         const float v_ref = power_above(__uint_as_float(most));
-        if (lane == 0u) S->v_ref[buf][w] = most && (most >> 23) > (least >> 23) + 8u ? -v_ref : v_ref;
+        if (lane == 0u) S->v_ref[buf][w] = most && (most >> 23) > (least >> 23) + kCkApart ? -v_ref : v_ref;
         cp_async_wait<1>();                               // (K's codes)
         put(it, 0u, 1.0f);
         done(it++);
@@ -468,7 +471,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         ok = __all_sync(0xffffffffu, room(it));
         if (!ok) break;
         cp_async_wait<1>();                               // (V's)
-        put(it, 1u, vsc * __uint_as_float((254u << 23) - __float_as_uint(v_ref)));
+        put(it, 1u, vsc * __uint_as_float(((254u + kCkVLog) << 23) - __float_as_uint(v_ref)));
         done(it++);
         if (j + 1u < t.b1) fetch(a.c.v, 1u, off, mask);
         else cp_async_commit();
@@ -662,8 +665,8 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
           for (int k = 0; k < 8; ++k) {
             const bool seen = hi > 16 * k && lo < 16 * k + 16;
             top = seen ? fmaxf(top, fabsf(vv[k])) : top;
-            // scales far apart, and some of the keys not seen by the row: they may have set the power
-            redo = redo || (seen && vv[k] < 0.0f && (lo > 16 * k || hi < 16 * k + 16));
+            // scales far apart, and some of the tile's keys not seen by the row: they may have set the power
+            redo = redo || (seen && vv[k] < 0.0f && (lo > 16 * k || hi < min(16 * k + 16, keys_hi - j0)));
           }
         }
         if (top > v_ref) {
@@ -750,7 +753,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
     float *part = a.part + static_cast<size_t>(split ? part_at - 1u : 0u) * (kChunkRows * (HD + 2u));
     const bool none = m_used == -INFINITY && l == 0.0f;
     float mul = split ? 1.0f : none ? 0.0f : 1.0f / l;
-    if (Q8) mul *= v_ref * (1.0f / kCkPScale);
+    if (Q8) mul *= v_ref * (Sh::kExactV ? 1.0f / kCkPScale : 1.0f / (kCkPScale * (1u << kCkVLog)));
     if (redo && split) mul = __int_as_float(0x7fc00000);  // (for the launch that joins)
     const uint32_t d0 = half * (HD / 2);
     uint8_t *out = has ? row_at(a.o, ts.first + static_cast<int32_t>(tok), head) + 2u * d0 : a.o.p;

@@ -38,7 +38,8 @@ def _tol(p, want, tol):
 
 
 def _near(got, want, tol):
-    return bool(((got.double() - want).abs() <= tol).all())
+    # (what is above a type's largest value, 65504 for f16, is an infinity in it)
+    return bool((((got.double() - want).abs() <= tol) | (got == want.to(got.dtype)) & torch.isinf(got)).all())
 
 
 def _place(p, b, pos):
@@ -87,3 +88,26 @@ def test_a_nan_alone(rt, scratch, dtype, row_dtype, rows, past, q_heads, window)
             lse_bad = mine if what in ("k", "q", "k scale") else torch.zeros_like(mine)
             assert bool((torch.isnan(lse) == lse_bad).all()), (c, what)
             assert _near(lse[~lse_bad], want_lse[~lse_bad], lse_tol[~lse_bad]), (c, what)
+
+
+# rows, past, heads, q heads, row type: parts of a tile's keys by several CTAs, whole tiles, single tokens
+FAR = [(20, 6000, 1, 8, "bf16"), (20, 6000, 1, 8, "f16"), (130, 3, 2, 4, "bf16"), (130, 3, 2, 4, "f16"), (300, 2001, 16, 16, "bf16"), (2, 701, 2, 8, "bf16"), (2, 701, 2, 8, "f16")]
+
+
+@pytest.mark.parametrize("far", [2.0 ** 9, 2.0 ** 13, 2.0 ** 20])
+@pytest.mark.parametrize("causal, window", [(True, 0), (False, 0), (True, 37)])
+@pytest.mark.parametrize("rows, past, heads, q_heads, row_dtype", FAR)
+def test_scales_far_apart(rt, scratch, rows, past, heads, q_heads, row_dtype, causal, window, far):
+    """Neighbours whose V scales are `far` apart, at the end of a sequence that ends inside a block, and where rows begin and end to see."""
+    p = Paged(rt, [rows, 3], [past, 50], dtype="e4m3", row_dtype=row_dtype, heads=heads, q_heads=q_heads, dim=64, seed=3)
+    length = rows + past
+    for pos in range(length - 9, length, 2):
+        p.scales[1][_place(p, 0, pos)] /= far
+    for pos in (past, past + 1, max(0, past - 30)):
+        p.scales[1][_place(p, 0, pos)] *= far
+    q = normal((p.n_rows, q_heads, 64), row_dtype, 8, 2.0)
+    want, want_lse, tol = p.attend(q, 0.125, causal, window)
+    o, lse = _call(p, scratch, q, causal=causal, window=window)
+    assert p.cache.Status()["code"] == 0
+    assert _near(o, want, _tol(p, want, tol))
+    assert _near(lse, want_lse, 2.0 ** -19 * (1 + want_lse.abs()))
