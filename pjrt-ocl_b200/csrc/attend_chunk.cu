@@ -52,7 +52,7 @@ constexpr float kCkPScale = 64.0f;                        // 8-bit pages: p (bel
 // V's codes (at most 448) times their scale over a power above it are as large as f16 holds; with scales down to 2^-15 of the power, normal codes stay
 // normal. What a power is above 16 keys for loses no bits as long as their scales are within that: no more than 2^14 (by their exponents) apart.
 constexpr uint32_t kCkVLog = 7, kCkApart = 14;
-constexpr unsigned long long kBudget = 2000000000ull;     // ns that a wait may take
+constexpr unsigned long long kBudget = 2000000000ull;     // ns that a wait may take without a sign of life
 
 template <bool BF, bool Q8, int HD>
 struct ChunkShape {
@@ -82,6 +82,7 @@ __device__ __forceinline__ Join *joins_of(const AttendArgs &a, uint32_t most) { 
 struct ChunkShared {
   uint64_t q_full, q_free, full[8], empty[8], s_full[2], p_full[2], pv_done[2], scales_free[2][2];
   uint32_t tmem, failed;
+  unsigned long long alive;                               // when a warp last said that it is working rows out again
   alignas(16) float v_ref[2][8];                          // 8-bit pages: powers of two above V's scales of two blocks, 16 keys each; negative: scales far apart
   Tile tile;                                              // no rows: the end
   union {
@@ -94,6 +95,38 @@ constexpr uint32_t ChunkSmem() { return ChunkShape<BF, Q8, HD>::kShared + ((size
 constexpr bool ChunkFits(uint32_t bytes) { return bytes <= 227u * 1024u; }
 static_assert(ChunkFits(ChunkSmem<true, false, 128>()) && ChunkFits(ChunkSmem<true, true, 128>()) && ChunkFits(ChunkSmem<false, true, 128>()) &&
                   ChunkFits(ChunkSmem<false, true, 64>()), "shared memory of an SM");
+
+// Waits of limited time (as in tc_common.cuh): they end without success when another role has, or when kBudget has gone by both since they began and
+// since a warp last said that it works rows out again, which may take long.
+__device__ __forceinline__ bool stuck(ChunkShared *S, unsigned long long t0) {
+  const unsigned long long seen = *const_cast<volatile unsigned long long *>(&S->alive), now = globaltimer_ns();
+  return now > max(t0, seen) + kBudget;
+}
+__device__ __forceinline__ bool wait_for(ChunkShared *S, uint64_t *bar, uint32_t parity) {
+  if (mbar_try_wait_parity(bar, parity)) return true;
+  volatile uint32_t *failed = &S->failed;
+  const unsigned long long t0 = globaltimer_ns();
+  for (;;) {
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait_parity(bar, parity)) return true;
+    if (*failed) return false;
+    if (stuck(S, t0)) { *failed = 1u; return false; }
+  }
+}
+// (a whole warp, in step)
+__device__ __forceinline__ bool wait_together(ChunkShared *S, uint64_t *bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait_parity(bar, parity))) return true;
+  volatile uint32_t *failed = &S->failed;
+  const unsigned long long t0 = globaltimer_ns();
+  for (;;) {
+    for (int i = 0; i < 32; ++i)
+      if (__all_sync(0xffffffffu, mbar_try_wait_parity(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *failed != 0u || stuck(S, t0))) {
+      *failed = 1u;
+      return false;
+    }
+  }
+}
 
 // ---- how the work is dealt ----
 typedef unsigned long long u64;
@@ -274,7 +307,6 @@ template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk, u64 x0, u64 x1, uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<BF, Q8, HD>;
   constexpr uint32_t NS = Sh::kStages;
-  volatile uint32_t *failed = &S->failed;
   const uint64_t cap = capacity_of(a.c, a.b);
   const uint32_t tid = threadIdx.x - kSoftWarps * 32u, lane = tid & 31u, w = tid >> 5;
   const uint32_t base = smem_addr(sm);
@@ -306,7 +338,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
     soff = ok && Q8 ? page * a.c.s_page + slot * a.c.s_slot + t.head * a.c.s_head : 0;
     return __ballot_sync(0xffffffffu, ok);
   };
-  auto room = [&](uint32_t i) { return tc_wait(&S->empty[i % NS], ((i / NS) & 1u) ^ 1u, failed, kBudget); };
+  auto room = [&](uint32_t i) { return wait_for(S, &S->empty[i % NS], ((i / NS) & 1u) ^ 1u); };
   auto done = [&](uint32_t i) {
     fence_proxy_async_smem();
     mbar_arrive(&S->full[i % NS]);
@@ -397,7 +429,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
     bool q_there = false;
     auto q_to_all = [&]() {                               // Q and the tile, when the scores of the tile before are done
       q_there = true;
-      ok = ok && __all_sync(0xffffffffu, tc_wait(&S->q_free, (turn & 1u) ^ 1u, failed, kBudget));
+      ok = ok && __all_sync(0xffffffffu, wait_for(S, &S->q_free, (turn & 1u) ^ 1u));
       if (!ok) return;
       if (tid == 0u) S->tile = t;
       if (found) load_q<BF, Q8, HD>(a, t, tid, base, S->q_exp);
@@ -445,7 +477,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         bool free = room(it);
         for (uint32_t s = 0; s < 2u; ++s) {
           uint32_t &n = used[s][buf];
-          if (n) free = free && tc_wait(&S->scales_free[s][buf], (n - 1u) & 1u, failed, kBudget);
+          if (n) free = free && wait_for(S, &S->scales_free[s][buf], (n - 1u) & 1u);
           if (s < slots) ++n;
         }
         ok = __all_sync(0xffffffffu, free);
@@ -483,8 +515,9 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
   cp_async_wait_all();
   // the products have read what was filled last, and their arrivals on the ring's barriers are in
   if (ok && tid == 0u) {
-    tc_drain(S->empty, NS, it, failed, kBudget);
-    tc_wait(&S->q_free, (turn & 1u) ^ 1u, failed, kBudget);
+    bool read = true;
+    for (uint32_t k = 0; k < NS && read; ++k) read = wait_for(S, &S->empty[(it + k) % NS], (((it + k) / NS) & 1u) ^ 1u);
+    wait_for(S, &S->q_free, (turn & 1u) ^ 1u);
   }
 }
 
@@ -493,7 +526,6 @@ template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_products(uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<BF, Q8, HD>;
   constexpr uint32_t NS = Sh::kStages;
-  volatile uint32_t *failed = &S->failed;
   const uint32_t base = smem_addr(sm), tmem = S->tmem;
   const uint32_t fmt = Q8 || !BF ? 0u : 1u;
   const uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((kCkKeys >> 3) << 17) | ((kCkRows >> 4) << 24);
@@ -523,10 +555,10 @@ static __device__ __forceinline__ void chunk_products(uint8_t *sm, ChunkShared *
     if (leader) tc_commit(&S->empty[st]);
     __syncwarp();
   };
-  auto full = [&](uint32_t i) { return tc_wait_uniform(&S->full[i % NS], (i / NS) & 1u, failed, kBudget); };
+  auto full = [&](uint32_t i) { return wait_together(S, &S->full[i % NS], (i / NS) & 1u); };
   uint32_t it = 0, n[2] = {0u, 0u};                       // the ring's blocks; each slot's blocks
   for (uint32_t turn = 0;; ++turn) {
-    if (!tc_wait_uniform(&S->q_full, turn & 1u, failed, kBudget)) return;
+    if (!wait_together(S, &S->q_full, turn & 1u)) return;
     const uint32_t rows = *const_cast<volatile uint32_t *>(&S->tile.rows);
     const uint32_t blocks = *const_cast<volatile uint32_t *>(&S->tile.b1) - *const_cast<volatile uint32_t *>(&S->tile.b0);
     if (rows == 0u) return;
@@ -541,7 +573,7 @@ static __device__ __forceinline__ void chunk_products(uint8_t *sm, ChunkShared *
       __syncwarp();
       if (!full(it + 1u)) return;
       for (uint32_t s = 0; s < slots; ++s) {
-        if (!tc_wait_uniform(&S->p_full[s], n[s] & 1u, failed, kBudget)) return;
+        if (!wait_together(S, &S->p_full[s], n[s] & 1u)) return;
         ++n[s];
         tc_fence_after_sync();
         values(s, (it + 1u) % NS, j == 0u);
@@ -575,7 +607,6 @@ __device__ __forceinline__ uint32_t rounded_up(float x) {
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<BF, Q8, HD>;
-  volatile uint32_t *failed = &S->failed;
   const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u, s = w >> 3, half = (w >> 2) & 1u, q4 = w & 3u;
   const uint32_t r = s * kCkRows + 32u * q4 + lane;       // the thread's row, of whose keys it has columns 64 half .. + 63
   const uint32_t row_addr = S->tmem + ((32u * q4) << 16), s_addr = row_addr + s * 128u, o_addr = row_addr + 256u + s * HD + half * (HD / 2);
@@ -585,7 +616,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
   uint32_t g = 0, n = 0, mine = 0;                        // blocks of all tiles; the slot's blocks and tiles
 #pragma unroll 1
   for (uint32_t turn = 0;; ++turn) {
-    if (!tc_wait_uniform(&S->q_full, turn & 1u, failed, kBudget)) return;
+    if (!wait_together(S, &S->q_full, turn & 1u)) return;
     const Tile &t = S->tile;
     const uint32_t rows = t.rows, seq = t.seq, part_at = t.part, r0 = t.r0, t_head = t.head;
     const int32_t keys_lo = t.keys.lo, keys_hi = t.keys.hi;
@@ -607,7 +638,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
     bool redo = false;
 #pragma unroll 1
     for (uint32_t j = b0; j < b1; ++j, ++g, ++n) {
-      if (!tc_wait_uniform(&S->s_full[s], n & 1u, failed, kBudget)) return;
+      if (!wait_together(S, &S->s_full[s], n & 1u)) return;
       tc_fence_after_sync();
       const int32_t j0 = keys_lo + static_cast<int32_t>(j * kCkKeys);
       const int32_t lo = sp.lo - j0, hi = sp.hi - j0;     // columns [lo, hi) of the block are seen
@@ -746,7 +777,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
     bar_sync(pair, 64);
     if (half) l = *sum_s;
     bar_sync(pair, 64);                                   // (and the sum)
-    if (!tc_wait_uniform(&S->pv_done[s], mine & 1u, failed, kBudget)) return;
+    if (!wait_together(S, &S->pv_done[s], mine & 1u)) return;
     ++mine;
     tc_fence_after_sync();
     const bool split = part_at != 0u;
@@ -813,11 +844,11 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
     } else if (has && !split && !half && a.lse) {
       a.lse[static_cast<int64_t>(ts.first + static_cast<int32_t>(tok)) * a.q_heads + head] = (m_used + log2f(l)) * 0.69314718055994531f;
     }
-    redo = has && !split && (redo || (!fine && (sp.lo > keys_lo || sp.hi < keys_hi)));
+    redo = has && !split && (redo || (!fine && isfinite(l) && (sp.lo > keys_lo || sp.hi < keys_hi)));      // (a sum that is not finite has met such a score: the result is right)
     for (uint32_t again = __ballot_sync(0xffffffffu, redo); again; again &= again - 1u) {      // (rows of this warp, one after another, its half of the values)
       const uint32_t k = __ffs(again) - 1u, q = r0 + s * kCkRows + 32u * q4 + k;
       __syncwarp();
-      attend_row_alone(a, seq, ts, static_cast<int32_t>(q / a.group), t_head * a.group + q % a.group, d0, HD / 2);
+      attend_row_alone(a, seq, ts, static_cast<int32_t>(q / a.group), t_head * a.group + q % a.group, d0, HD / 2, &S->alive);
     }
   }
 }
@@ -864,6 +895,7 @@ __global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(c
       for (uint32_t i = 0; i < 2u; ++i) mbar_init(&S->scales_free[s][i], 8u);
     }
     S->failed = 0u;
+    S->alive = 0ull;
     fence_mbar_init();
   }
   if (w == kSoftWarps + kLoadWarps) {
@@ -906,7 +938,7 @@ __global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(c
 // was 37 us for 2048 rows behind 14336 of 32 heads of 128 values.)
 constexpr uint32_t kJoinThreads = 256, kJoinRows = 32, kMostRuns = 1024;
 template <int HD>
-__global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_constant__ AttendArgs a, uint32_t most) {
+__global__ void __launch_bounds__(kJoinThreads, 2) b2_attend_join(const __grid_constant__ AttendArgs a, uint32_t most) {
   const uint32_t w = threadIdx.x >> 5, lane = threadIdx.x & 31u, begun = blockIdx.x / (kChunkRows / kJoinRows);
   const Join *const joins = joins_of(a, most);
   if (joins[begun].tile.rows <= (blockIdx.x % (kChunkRows / kJoinRows)) * kJoinRows) return;
@@ -1005,9 +1037,9 @@ __global__ void __launch_bounds__(kJoinThreads) b2_attend_join(const __grid_cons
     }
     if (lane == 0u && a.lse) a.lse[static_cast<int64_t>(row) * a.q_heads + head] = (m + log2f(sum)) * 0.69314718055994531f;
     const Span sp = SeenBy(t.s, static_cast<int32_t>(tok), a.causal, a.window);
-    if (__any_sync(0xffffffffu, !fine) && (sp.lo > t.keys.lo || sp.hi < t.keys.hi)) {
+    if (__any_sync(0xffffffffu, !fine) && isfinite(sum) && (sp.lo > t.keys.lo || sp.hi < t.keys.hi)) {
       __syncwarp();
-      attend_row_alone(a, t.seq, t.s, static_cast<int32_t>(tok), head, 0u, HD);
+      attend_row_alone(a, t.seq, t.s, static_cast<int32_t>(tok), head, 0u, HD, nullptr);
     }
   }
 }

@@ -39,9 +39,12 @@ __device__ __forceinline__ uint8_t *row_at(const RowsRef &r, int32_t row, uint32
 
 // One row of the result by itself, over the keys that it sees and no others, by one warp. A product over a tile of keys gives a
 // key that a row does not see the weight 0, and 0 times a NaN or an infinity is a NaN: where a tile's result is not finite, the
-// rows that do not see all of its keys are worked out here again. Slow, and only reached by caches that hold such values.
-// (of its values [v0, v0 + nv), and lse with the first)
-static __device__ __noinline__ void attend_row_alone(const AttendArgs &a, uint32_t seq, const Seq s, int32_t i, uint32_t head, uint32_t v0, uint32_t nv) {
+// rows that do not see all of its keys are worked out here again. Slow, and only reached by caches whose V holds such values, or
+// 8-bit pages whose scales are further apart than a tile's product holds. (Keys one after another: four at once would take registers from the chunk
+// kernel's loops, whose 8-bit chunk went from 784 to 797 us.)
+// (of its values [v0, v0 + nv), and lse with the first; `alive`: where others see that it goes on, or null)
+static __device__ __noinline__ void attend_row_alone(const AttendArgs &a, uint32_t seq, const Seq s, int32_t i, uint32_t head, uint32_t v0, uint32_t nv,
+                                                     volatile unsigned long long *alive) {
   const uint32_t lane = threadIdx.x & 31u, h = head / a.group, d0 = lane * 4u;
   const bool has = d0 < a.c.hd, bf = a.bf16 != 0u;
   const Span sp = SeenBy(s, i, a.causal, a.window);
@@ -67,18 +70,32 @@ static __device__ __noinline__ void attend_row_alone(const AttendArgs &a, uint32
     int64_t at = -1, sc = 0;
     if (j0 + static_cast<int32_t>(lane) < sp.hi) at = page_offset(a.c, a.b, seq, static_cast<uint32_t>(j0) + lane, &sc);
     const int32_t n = min(32, sp.hi - j0);
+    if (alive && lane == 0u) *alive = globaltimer_ns();
+    float mine = -INFINITY;                               // the score of the lane's key
+#pragma unroll 1
     for (int32_t j = 0; j < n; ++j) {
       const int64_t o = __shfl_sync(0xffffffffu, at, j), so = __shfl_sync(0xffffffffu, sc, j);
       if (o < 0) continue;
       float x[4];
       four(a.c.k + o + h * a.c.head_bytes, a.e4m3 ? a.c.ks[so + h * a.c.s_head] : 1.0f, x);
       const float sum = warp_reduce(q[0] * x[0] + q[1] * x[1] + q[2] * x[2] + q[3] * x[3], [](float u, float v) { return u + v; });
-      const float m2 = fmaxf(m, sum), c = m == -INFINITY ? 0.0f : exp2f(m - m2), p = sum == -INFINITY ? 0.0f : exp2f(sum - m2);     // (a NaN loses in the maximum and stays in p)
-      four(a.c.v + o + h * a.c.head_bytes, a.e4m3 ? a.c.vs[so + h * a.c.s_head] : 1.0f, x);
-      l = l * c + p;
+      if (static_cast<int32_t>(lane) == j) mine = sum;
+    }
+    const float m2 = fmaxf(m, warp_reduce(mine, [](float u, float v) { return fmaxf(u, v); }));
+    const float c = m == -INFINITY ? 0.0f : exp2f(m - m2), p = mine == -INFINITY ? 0.0f : exp2f(mine - m2);     // (a NaN loses in the maximum and stays in p)
+    l = l * c + warp_reduce(p, [](float u, float v) { return u + v; });
+    m = m2;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] = acc[k] * c + p * x[k];
-      m = m2;
+    for (int k = 0; k < 4; ++k) acc[k] *= c;
+#pragma unroll 1
+    for (int32_t j = 0; j < n; ++j) {
+      const int64_t o = __shfl_sync(0xffffffffu, at, j), so = __shfl_sync(0xffffffffu, sc, j);
+      const float pj = __shfl_sync(0xffffffffu, p, j);
+      if (o < 0) continue;
+      float x[4];
+      four(a.c.v + o + h * a.c.head_bytes, a.e4m3 ? a.c.vs[so + h * a.c.s_head] : 1.0f, x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += pj * x[k];
     }
   }
   const bool none = m == -INFINITY && l == 0.0f;

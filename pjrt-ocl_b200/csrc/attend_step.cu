@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
         } else {
           store_row_value(p, x.x, BF); store_row_value(p + 2, x.y, BF); store_row_value(p + 4, x.z, BF); store_row_value(p + 6, x.w, BF);
         }
-        if (cw.s.n > 1 && !(isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w))) atomicOr(&S.redo[turn & 1u], 1u << r);
+        if (cw.s.n > 1 && isfinite(ll) && !(isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w))) atomicOr(&S.redo[turn & 1u], 1u << r);
       }
       if (d == 0u && a.lse) a.lse[static_cast<int64_t>(row) * a.q_heads + head] = (mm + log2f(ll)) * 0.69314718055994531f;
     };
@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
     if (redo) {
       const bool all = whole || together;                 // (else one warp is here)
       for (uint32_t r = all ? w : 0u; r < rows; r += all ? kStepWarps : 1u)
-        if ((redo >> r) & 1u) attend_row_alone(a, cw.b, cw.s, static_cast<int32_t>(r / a.group), cw.h * a.group + r % a.group, 0u, HD);
+        if ((redo >> r) & 1u) attend_row_alone(a, cw.b, cw.s, static_cast<int32_t>(r / a.group), cw.h * a.group + r % a.group, 0u, HD, nullptr);
     }
     if (!more) break;
     w_tile -= t_end;                                      // (the warps take the CTA's tiles in turn, across items)

@@ -111,3 +111,45 @@ def test_scales_far_apart(rt, scratch, rows, past, heads, q_heads, row_dtype, ca
     assert p.cache.Status()["code"] == 0
     assert _near(o, want, _tol(p, want, tol))
     assert _near(lse, want_lse, 2.0 ** -19 * (1 + want_lse.abs()))
+
+
+@pytest.mark.parametrize("dtype, row_dtype", [("bf16", "bf16"), ("f16", "f16"), ("e4m3", "bf16"), ("e4m3", "f16")])
+def test_rows_worked_out_again_behind_the_products(rt, scratch, dtype, row_dtype):
+    """Whole tiles and parts of them, all of whose rows see a V that is not finite: the batch's other tiles are done as ever, captured too, and
+    the call after finds nothing of it."""
+    rows, past = [70] * 40 + [300], list(range(0, 800, 20)) + [9000]
+    p = Paged(rt, rows, past, dtype=dtype, row_dtype=row_dtype, heads=4, q_heads=16, dim=64, page=48, seed=5)
+    q = normal((p.n_rows, 16, 64), row_dtype, 8)
+    want, want_lse, tol = p.attend(q, 0.125)
+    tol = _tol(p, want, tol)
+    clean, _ = _call(p, scratch, q)
+    assert _near(clean, want, tol)
+    keep = p.pages[1].clone()
+    bad = torch.zeros_like(q, dtype=torch.bool)
+    for b in (0, 3, 17, 40):                                     # a NaN at the first key, value 9 of cache head 2; another at the last
+        for pos, d in ((0, 9), (p.lengths[b] - 1, 11)):
+            at = (*_place(p, b, pos), 2, d)
+            if dtype == "e4m3":
+                p.pages[1].view(torch.uint8)[at] = 0x7F
+            else:
+                p.pages[1][at] = NAN
+        first = sum(rows[:b])
+        bad[first:first + rows[b], 8:12, 9] = True
+        bad[first + rows[b] - 1, 8:12, 11] = True
+    o, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    r = package().Rows.Of
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=side):
+        p.cache.Attend(p.batch, r(q), r(o), scratch, lse=lse.data_ptr(), stream=side.cuda_stream)
+    for turn in range(2):
+        o.fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert p.cache.Status()["code"] == 0
+        assert bool((torch.isnan(o) == bad).all()) and _near(o[~bad], want[~bad], tol[~bad])
+        assert _near(lse, want_lse, 2.0 ** -19 * (1 + want_lse.abs()))
+    p.pages[1].copy_(keep)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, clean)
