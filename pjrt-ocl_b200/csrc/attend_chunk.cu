@@ -4,7 +4,9 @@
 // each a tensor-core tile, so that a block of 128 keys is fetched once for all of them. Per slot and block, with the scores in
 // tensor memory:  S = Q K^T (128 x 128 x hd),  p = 2^(s scale log2 e - m) over the running maximum m,  O += P V (128 x hd x 128).
 // O stays in tensor memory; it is rescaled in place only when a row's maximum grew by more than 2^8 since the one in use was set
-// (p then stays below 256 and the result is mathematically the same). P overwrites the scores it came from.
+// (p then stays below 256 and the result is mathematically the same). P overwrites the scores it came from. Two threads that have a row's maximum
+// between them tell each other 16 bits that are not below theirs, and all of them only when a row of their warps may move: a maximum of thousands is off by
+// dozens in 16 bits, and weights of f16 that are 2^-24 of what they should be are gone.
 //
 // Roles of a CTA: a warp to issue the products, four warps (8-bit pages: eight) that fill the ring of K and V blocks (and Q), eight softmax
 // warps for each slot, two threads to a row with half of the keys each (one thread to a row: as fast with 128 values a head, 5 % slower
@@ -604,6 +606,10 @@ __device__ __forceinline__ uint32_t rounded_up(float x) {
   const uint32_t u = __float_as_uint(x);
   return (x > 0.0f ? u + 0xffffu : u) >> 16;              // (NaN and what is below 0: cut off)
 }
+// and x again, from that and its lower half.
+__device__ __forceinline__ float from_halves(uint32_t up, uint32_t low) {
+  return __uint_as_float((up << 16 | low) - (low != 0u && !(up & 0x8000u) ? 0x10000u : 0u));
+}
 template <bool BF, bool Q8, int HD>
 static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *sm, ChunkShared *S) {
   using Sh = ChunkShape<BF, Q8, HD>;
@@ -672,22 +678,17 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
 #pragma unroll
         for (int i = 0; i < 16; ++i) m4[i & 3] = max3_nan(m4[i & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 16]));
       }
-      const uint32_t own = rounded_up(max3_nan(m4[0], m4[1], max3_nan(m4[2], m4[3], m4[2])));
-      top_s[half * 128u] = static_cast<uint16_t>(own);
+      const float own = max3_nan(m4[0], m4[1], max3_nan(m4[2], m4[3], m4[2]));
+      const uint32_t own_up = rounded_up(own);
+      top_s[half * 128u] = static_cast<uint16_t>(own_up);
       bar_sync(pair, 64);
-      const float mx = max3_nan(__uint_as_float(own << 16), __uint_as_float(static_cast<uint32_t>(top_s[(half ^ 1u) * 128u]) << 16), -INFINITY) * sl2;
+      const uint32_t other_up = top_s[(half ^ 1u) * 128u];
+      float mx = max3_nan(__uint_as_float(own_up << 16), __uint_as_float(other_up << 16), -INFINITY) * sl2;
       bool grow = mx > m_used + kGrow;
-      float alpha = 1.0f;
-      if (grow) {
-        alpha = m_used == -INFINITY ? 0.0f : fast_ex2(m_used - mx);
-        l *= alpha;
-        m_used = mx;
-      }
-      float v_mul[4] = {1.0f, 1.0f, 1.0f, 1.0f};          // of 16 columns each (exact V: the same for all, beside each one's scale)
+      float top = v_ref, vv[8];
       if (Q8) {
         const float4 va = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u]), vb = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u] + 4);
-        const float vv[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
-        float top = v_ref;
+        vv[0] = va.x; vv[1] = va.y; vv[2] = va.z; vv[3] = va.w; vv[4] = vb.x; vv[5] = vb.y; vv[6] = vb.z; vv[7] = vb.w;
         if (whole) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(vv[k]));
@@ -700,11 +701,28 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
             redo = redo || (seen && vv[k] < 0.0f && (lo > 16 * k || hi < min(16 * k + 16, keys_hi - j0)));
           }
         }
-        if (top > v_ref) {
+        grow = grow || top > v_ref;
+      }
+      // (the two warps agree: they have the same rows, and the same of all this)
+      const bool move = __any_sync(0xffffffffu, grow);
+      float alpha = 1.0f;
+      if (move) {
+        bar_sync(pair, 64);
+        top_s[half * 128u] = static_cast<uint16_t>(__float_as_uint(own));
+        bar_sync(pair, 64);
+        mx = max3_nan(own, from_halves(other_up, top_s[(half ^ 1u) * 128u]), -INFINITY) * sl2;
+        if (mx > m_used + kGrow) {
+          alpha = m_used == -INFINITY ? 0.0f : fast_ex2(m_used - mx);
+          l *= alpha;
+          m_used = mx;
+        }
+        if (Q8 && top > v_ref) {
           alpha *= v_ref / top;                           // (a power of two, or 0 at first)
           v_ref = top;
-          grow = true;
         }
+      }
+      float v_mul[4] = {1.0f, 1.0f, 1.0f, 1.0f};          // of 16 columns each (exact V: the same for all, beside each one's scale)
+      if (Q8) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {                     // (columns that the row does not see may have a larger power)
           const float own = Sh::kExactV ? 1.0f : fabsf(half ? vv[4 + k] : vv[k]);
@@ -712,7 +730,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
           if (!Sh::kExactV) v_mul[k] = fminf(v_mul[k], kCkPScale);
         }
       }
-      if (j > b0 && __any_sync(0xffffffffu, grow)) {      // (these scores came after the products before them: O is at rest)
+      if (j > b0 && move) {                               // (these scores came after the products before them: O is at rest)
 #pragma unroll 1
         for (uint32_t c0 = 0; c0 < HD / 2; c0 += 16u) {
           uint32_t y[16];

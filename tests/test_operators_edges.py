@@ -153,3 +153,25 @@ def test_rows_worked_out_again_behind_the_products(rt, scratch, dtype, row_dtype
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(o, clean)
+
+
+@pytest.mark.parametrize("dtype, row_dtype", [("f16", "f16"), ("bf16", "bf16"), ("e4m3", "bf16"), ("e4m3", "f16")])
+@pytest.mark.parametrize("rows, past, q_heads", [(1, 300, 4), (3, 40, 8), (40, 100, 4), (300, 0, 2), (33, 5000, 2)])
+@pytest.mark.parametrize("base", [1250.0, -1250.0, 2048.0, 3000.0, -3000.0, 4096.0, -4160.0])
+def test_large_scores(rt, scratch, dtype, row_dtype, rows, past, q_heads, base):
+    """Scores around `base` that differ by a few: what is common to a row's scores cancels, however large it is."""
+    p = Paged(rt, [rows], [past], dtype=dtype, row_dtype=row_dtype, heads=1, q_heads=q_heads, dim=64, page=16, seed=6)
+    if dtype == "e4m3":                                          # (codes 256 and a scale of 2^-3: 32 exactly)
+        p.pages[0].view(torch.uint8)[..., 0] = 0x78
+        p.scales[0].fill_(2.0 ** -3)
+        p.pages[0].view(torch.uint8)[..., 1:] = torch.randint(0x28, 0x38, p.pages[0][..., 1:].shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda", dtype=torch.uint8)
+    else:
+        p.pages[0][..., 0] = 32.0
+    q = normal((rows, q_heads, 64), row_dtype, 8, 0.25)
+    q[..., 0] = base / 32.0                                      # (at most 7 bits: exact)
+    want, want_lse, tol = p.attend(q, 1.0)
+    o, lse = _call(p, scratch, q, scale=1.0)
+    assert p.cache.Status()["code"] == 0
+    assert _near(o, want, _tol(p, want, tol))
+    # a score and its sum in f32: 64 terms, all but a few of them small beside the first
+    assert _near(lse, want_lse, 16 * 2.0 ** -24 * want_lse.abs() + 2.0 ** -17)
