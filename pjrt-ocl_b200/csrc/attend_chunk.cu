@@ -86,6 +86,8 @@ struct ChunkShared {
   uint32_t tmem, failed;
   unsigned long long alive;                               // when a warp last said that it is working rows out again
   alignas(16) float v_ref[2][8];                          // 8-bit pages: powers of two above V's scales of two blocks, 16 keys each; negative: scales far apart
+  // Keys of a block whose pages do not exist, a bit each; a block is filled at most four ahead of the one that the softmax warps are at.
+  alignas(16) uint32_t absent[8][kCkKeys / 32u];
   Tile tile;                                              // no rows: the end
   union {
     unsigned long long find[30];                          // (before any row is looked at)
@@ -330,15 +332,21 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
     }
   };
   // ---- K and V ----
-  auto place = [&](int64_t &off, int64_t &soff) -> uint32_t {       // the lane's key; which lanes of the warp have one
-    bool ok = live;
-    if (ok && static_cast<uint32_t>(page) >= a.c.n_pages) {
-      cache_fault(a.c.status, kStBadPage, t.seq, entry, static_cast<uint32_t>(page));
-      ok = false;
-    }
+  uint32_t absent = 0u;
+  auto place = [&](int64_t &off, int64_t &soff) -> uint32_t {       // the lane's key; which lanes of the warp have one, and which have one without a page
+    const bool lost = live && static_cast<uint32_t>(page) >= a.c.n_pages, ok = live && !lost;
+    if (lost) cache_fault(a.c.status, kStBadPage, t.seq, entry, static_cast<uint32_t>(page));
+    absent = __ballot_sync(0xffffffffu, lost);
     off = ok ? page * a.c.page_bytes + slot * a.c.slot_bytes + t.head * a.c.head_bytes : 0;
     soff = ok && Q8 ? page * a.c.s_page + slot * a.c.s_slot + t.head * a.c.s_head : 0;
     return __ballot_sync(0xffffffffu, ok);
+  };
+  auto say_absent = [&](uint32_t i) {                     // (with K of a block, item i of the ring)
+    uint32_t *const to = S->absent[(i >> 1) & 7u];
+    if (lane == 0u) {
+      if (Q8) reinterpret_cast<uint16_t *>(to)[w] = static_cast<uint16_t>(absent);
+      else to[w] = absent;
+    }
   };
   auto room = [&](uint32_t i) { return wait_for(S, &S->empty[i % NS], ((i / NS) & 1u) ^ 1u); };
   auto done = [&](uint32_t i) {
@@ -458,6 +466,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
           // (a lane that gave up takes its warp with it)
           ok = __all_sync(0xffffffffu, ok && room(it));
           if (!ok) break;
+          if (v == 0u) say_absent(it);
           copy(v ? a.c.v : a.c.k, it, off, mask);
           ++it;
           if (it > settled + 2u) { cp_async_wait<2>(); settle(it - 2u); }
@@ -484,6 +493,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         }
         ok = __all_sync(0xffffffffu, free);
         if (!ok) break;
+        say_absent(it);
         if (lane < RW) {
           float *const s = reinterpret_cast<float *>(sm + Sh::kScales + buf * 512u) + RW * w + lane;
           *s = ksc;
@@ -601,6 +611,8 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// The bits below bit n (none below 0, all from 32 on).
+__device__ __forceinline__ uint32_t below(int32_t n) { return static_cast<uint32_t>((1ull << max(0, min(32, n))) - 1ull); }
 // x as the next bf16 that is not below it (its bits).
 __device__ __forceinline__ uint32_t rounded_up(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -648,7 +660,8 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
       tc_fence_after_sync();
       const int32_t j0 = keys_lo + static_cast<int32_t>(j * kCkKeys);
       const int32_t lo = sp.lo - j0, hi = sp.hi - j0;     // columns [lo, hi) of the block are seen
-      const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= static_cast<int32_t>(kCkKeys));
+      const uint4 gone = *reinterpret_cast<const uint4 *>(S->absent[g & 7u]);
+      const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= static_cast<int32_t>(kCkKeys) && (gone.x | gone.y | gone.z | gone.w) == 0u);
       // 1: the row's maximum. The scores are read twice: half of a row's in registers at once leave too few for the rest
       const int32_t lo_h = lo - 64 * static_cast<int32_t>(half), hi_h = hi - 64 * static_cast<int32_t>(half);
       const float *ks = reinterpret_cast<const float *>(sm + Sh::kScales + (g & 1u) * 512u) + 64u * half;
@@ -665,9 +678,10 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
           }
         }
         if (!whole) {
+          const uint32_t hide = S->absent[g & 7u][2u * half + c] | below(lo_h - 32 * c) | ~below(hi_h - 32 * c);
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (i + 32 * c < lo_h || i + 32 * c >= hi_h) x[i] = 0xff800000u;
+            if ((hide >> i) & 1u) x[i] = 0xff800000u;
         }
       };
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};

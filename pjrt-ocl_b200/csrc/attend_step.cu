@@ -194,6 +194,8 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
   int32_t page = -1;                                      // page number of the lane's key in that tile
   uint32_t key_slot = 0, key_entry = 0;
   bool key_live = false;
+  uint32_t keys_next = 0u;                                // which keys of the tile fetched last are there, a bit each
+  constexpr uint32_t kAllKeys = KT == 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u;
   auto look_ahead = [&]() {                               // the next tile's place, and its keys' pages on the way
     while (p_more && p_tile >= p_end) {
       p_tile -= p_end;
@@ -219,13 +221,13 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
         live = false;
       }
       const uint32_t mask = __ballot_sync(0xffffffffu, live);
+      keys_next = mask;
       constexpr int kAtOnce = 32 / CH;
       const uint32_t sub = lane % CH, r0 = lane / CH;
       const bool in_hd = sub * 16u < a.c.hd * (Q8 ? 1u : 2u);
       const int64_t head_at = pw.h * a.c.head_bytes + sub * 16u;
       const uint32_t entry0 = __shfl_sync(0xffffffffu, key_entry, 0);
-      constexpr uint32_t kAll = KT == 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u;
-      if (mask == kAll && __all_sync(0xffffffffu, lane >= KT || key_entry == entry0)) {     // a whole tile in one page
+      if (mask == kAllKeys && __all_sync(0xffffffffu, lane >= KT || key_entry == entry0)) {     // a whole tile in one page
         int64_t o = __shfl_sync(0xffffffffu, page, 0) * a.c.page_bytes + (__shfl_sync(0xffffffffu, key_slot, 0) + r0) * a.c.slot_bytes + head_at;
         if (!in_hd) o = 0;
         const int64_t step = in_hd ? kAtOnce * a.c.slot_bytes : 0;
@@ -362,6 +364,7 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
     for (; w_tile < t_end; w_tile += kStepWarps, ++taken) {
       cp_async_wait_all();
       __syncwarp();
+      const uint32_t there = keys_next;
       issue();                                            // into the other stage
       const uint32_t st = ring_s + (taken % kStages) * Sh::kStage;
       const int32_t j0 = cw.keys.lo + static_cast<int32_t>(w_tile) * KT;
@@ -402,8 +405,8 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
             }
           }
       }
-      // keys that the row does not see at -inf; the thread's keys: 16 t + quad, + 8
-      const bool whole = j0 >= full_lo && j0 + KT <= full_hi;
+      // keys that the row does not see, or that have no page, at -inf; the thread's keys: 16 t + quad, + 8
+      const bool whole = j0 >= full_lo && j0 + KT <= full_hi && there == kAllKeys;
       float vs[MT][2], top[NR][2], v_top[NR][2];
 #pragma unroll
       for (int g = 0; g < NR; ++g) { top[g][0] = top[g][1] = -INFINITY; v_top[g][0] = v_top[g][1] = 0.0f; }
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
             for (int c = 0; c < 4; ++c) {
               const int32_t j = j0 + t * 16 + static_cast<int32_t>(quad) + 8 * (c >> 1);
               const int e = c & 1;
-              const bool seen = j >= sp[g][e].lo && j < sp[g][e].hi;
+              const bool seen = j >= sp[g][e].lo && j < sp[g][e].hi && ((there >> (t * 16 + quad + 8 * (c >> 1))) & 1u);
               s[g][t][c] = seen ? s[g][t][c] : -INFINITY;
               if (Q8) v_top[g][e] = fmaxf(v_top[g][e], seen ? vs[t][c >> 1] : 0.0f);
             }

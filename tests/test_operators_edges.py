@@ -175,3 +175,54 @@ def test_large_scores(rt, scratch, dtype, row_dtype, rows, past, q_heads, base):
     assert _near(o, want, _tol(p, want, tol))
     # a score and its sum in f32: 64 terms, all but a few of them small beside the first
     assert _near(lse, want_lse, 16 * 2.0 ** -24 * want_lse.abs() + 2.0 ** -17)
+
+
+def _without(p, b, q, scale, absent, window=0):
+    """Sequence b's rows in 64 bits, keys of `absent` left out: out, lse, sum w |v|, the largest sum |q k|."""
+    n, length, g = p.rows[b], p.lengths[b], p.q_heads // p.heads
+    first = sum(p.rows[:b])
+    k, v = (p.values(b, i).repeat_interleave(g, 1).transpose(0, 1) for i in (0, 1))
+    x = q[first:first + n].double().transpose(0, 1)
+    row, key = torch.arange(length - n, length, device="cuda")[:, None], torch.arange(length, device="cuda")[None]
+    seen = (key <= row) & ~absent[None]
+    if window:
+        seen = seen & (key > row - window)
+    s = (x @ k.transpose(1, 2) * scale).masked_fill(~seen, -INF)
+    lse = torch.logsumexp(s, -1)
+    w = torch.where(seen, torch.exp(s - lse[..., None]), torch.zeros_like(s))
+    reach = (x.abs() @ k.abs().transpose(1, 2) * scale).amax(-1)
+    return [t.transpose(0, 1) for t in (w @ v, lse, w @ v.abs(), reach)]
+
+
+@pytest.mark.parametrize("dtype, row_dtype", [("bf16", "bf16"), ("f16", "f16"), ("e4m3", "bf16"), ("e4m3", "f16")])
+@pytest.mark.parametrize("rows, past, q_heads, page, window", [(1, 200, 4, 16, 0), (3, 60, 8, 7, 0), (2, 500, 2, 64, 90), (40, 100, 4, 16, 0), (150, 4000, 4, 24, 0), (300, 37, 2, 5, 60)])
+def test_keys_without_a_page_are_absent(rt, scratch, dtype, row_dtype, rows, past, q_heads, page, window):
+    """The sequence that names pages outside the cache: its rows over the keys that there are."""
+    p = Paged(rt, [2, rows], [9, past], dtype=dtype, row_dtype=row_dtype, heads=2, q_heads=q_heads, dim=64, page=page, seed=7)
+    q = (normal((p.n_rows, q_heads, 64), row_dtype, 8).abs() + 0.25).to(normal((1,), row_dtype, 0).dtype)
+    if dtype == "e4m3":
+        p.pages[0].view(torch.uint8).bitwise_or_(0x80)           # scores below 0: a key of zeros would outweigh all others
+    else:
+        p.pages[0].copy_(-p.pages[0].abs())
+    length = rows + past
+    last = (length - 1) // page
+    for entries in ((0,), (last,), (last // 2, last // 2 + 1), tuple(range(0, last + 1, 2)), tuple(range(last + 1))):
+        absent = torch.zeros(length, dtype=torch.bool, device="cuda")
+        for e in entries:
+            absent[e * page:(e + 1) * page] = True
+        want, want_lse, size, reach = _without(p, 1, q, 0.125, absent, window)
+        keep = p.table.clone()
+        for i, e in enumerate(entries):
+            p.table[1, e] = -1 if i % 2 else p.n_pages
+        o, lse = _call(p, scratch, q, window=window)
+        if bool(absent[max(0, past + 1 - window) if window else 0:].any()):       # (what nobody sees is not looked up)
+            with pytest.raises(package().InvalidArgument, match="sequence 1 names page"):
+                p.cache.Status()
+        assert p.cache.Status()["code"] == 0
+        p.table.copy_(keep)
+        got, got_lse = o[2:], lse[2:]
+        none = want_lse == -INF
+        assert bool((got_lse[none] == -INF).all()) and not bool(got[none].any())
+        off = (2 * (68 * 2.0 ** -24 * reach + 2.0 ** -22 + (length / 8 + 16) * 2.0 ** -24) + 2 * half_step("f16" if dtype == "e4m3" else row_dtype))[..., None]
+        assert _near(got[~none], want[~none], (off * size + half_step(row_dtype) * want.abs())[~none]), entries
+        assert _near(got_lse[~none], want_lse[~none], (2 * 68 * 2.0 ** -24 * reach + 2.0 ** -19 * (1 + want_lse.abs()))[~none]), entries
