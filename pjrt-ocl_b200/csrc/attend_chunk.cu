@@ -288,7 +288,7 @@ static __device__ __forceinline__ void load_q(const AttendArgs &a, const Tile &t
 #pragma unroll
         for (uint32_t o = QL / 2u; o > 0u; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const int ex = static_cast<int>(__float_as_uint(top) >> 23);
-        const int e = ex == 0 || ex == 255 ? 0 : max(-100, min(100, 127 + 14 - ex));
+        const int e = ex == 0 || ex == 255 ? 0 : min(100, 127 + 14 - ex);      // (-113 and more)
         const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
         if (c == 0u) q_exp[r + k * AT] = static_cast<int8_t>(e);
         auto h2 = [&](uint32_t x) { return cvt_f16x2(__uint_as_float(x & 0xffff0000u) * up, __uint_as_float(x << 16) * up); };

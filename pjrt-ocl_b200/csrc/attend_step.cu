@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // 2^e brings the largest to [2^14, 2^15); rows of zeros, and of what is not finite, stay as they are
             const int ex = static_cast<int>(__float_as_uint(top) >> 23);
-            const int e = ex == 0 || ex == 255 ? 0 : max(-100, min(100, 127 + 14 - ex));
+            const int e = ex == 0 || ex == 255 ? 0 : min(100, 127 + 14 - ex);      // (-113 and more)
             const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks)

@@ -226,3 +226,18 @@ def test_keys_without_a_page_are_absent(rt, scratch, dtype, row_dtype, rows, pas
         off = (2 * (68 * 2.0 ** -24 * reach + 2.0 ** -22 + (length / 8 + 16) * 2.0 ** -24) + 2 * half_step("f16" if dtype == "e4m3" else row_dtype))[..., None]
         assert _near(got[~none], want[~none], (off * size + half_step(row_dtype) * want.abs())[~none]), entries
         assert _near(got_lse[~none], want_lse[~none], (2 * 68 * 2.0 ** -24 * reach + 2.0 ** -19 * (1 + want_lse.abs()))[~none]), entries
+
+
+@pytest.mark.parametrize("rows", [1, 4, 50])
+def test_queries_of_any_size_over_8_bit_pages(rt, scratch, rows):
+    """Rows of bf16 between 2^-60 and 2^126, K's scales the other way round."""
+    p = Paged(rt, [rows], [70], dtype="e4m3", heads=2, q_heads=4, dim=64, page=16, seed=4)
+    scales, base = p.scales[0].clone(), normal((rows, 4, 64), "bf16", 8)
+    for e in (-60, 0, 90, 113, 115, 120, 123):
+        q = (base.double() * 2.0 ** e).bfloat16()
+        p.scales[0].copy_(scales * 2.0 ** -e)
+        want, want_lse, tol = p.attend(q, 0.125)
+        o, lse = _call(p, scratch, q)
+        assert p.cache.Status()["code"] == 0
+        assert _near(o, want, _tol(p, want, tol)), e
+        assert _near(lse, want_lse, 2.0 ** -19 * (1 + want_lse.abs())), e
