@@ -303,6 +303,8 @@ typedef struct {
 } b2_batch;
 b2_status b2_cache_create(b2_runtime *rt, const b2_cache_desc *desc, b2_cache **out, char *err, size_t err_cap);
 void b2_cache_destroy(b2_cache *cache);
+/* Budget of each of attention's waits on the tensor cores, in nanoseconds (default 2e9), for the calls that follow. */
+void b2_cache_set_wait_budget_ns(b2_cache *cache, uint64_t ns);
 /* The batch's rows of K and V into the pages. e4m3: scale = max|x| / 448 of the row, code = x / scale to the nearest
  * (ties to even); a row of zeros has scale 0; one that holds a NaN or an infinity reads back as NaN throughout.
  * Two rows of one call that name the same slot leave a mixture there. */

@@ -54,7 +54,6 @@ constexpr float kCkPScale = 64.0f;                        // 8-bit pages: p (bel
 // V's codes (at most 448) times their scale over a power above it are as large as f16 holds; with scales down to 2^-15 of the power, normal codes stay
 // normal. What a power is above 16 keys for loses no bits as long as their scales are within that: no more than 2^14 (by their exponents) apart.
 constexpr uint32_t kCkVLog = 7, kCkApart = 14;
-constexpr unsigned long long kBudget = 2000000000ull;     // ns that a wait may take without a sign of life
 
 template <bool BF, bool Q8, int HD>
 struct ChunkShape {
@@ -84,6 +83,7 @@ __device__ __forceinline__ Join *joins_of(const AttendArgs &a, uint32_t most) { 
 struct ChunkShared {
   uint64_t q_full, q_free, full[8], empty[8], s_full[2], p_full[2], pv_done[2], scales_free[2][2];
   uint32_t tmem, failed;
+  unsigned long long budget;                              // ns that a wait may take without a sign of life
   unsigned long long alive;                               // when a warp last said that it is working rows out again
   alignas(16) float v_ref[2][8];                          // 8-bit pages: powers of two above V's scales of two blocks, 16 keys each; negative: scales far apart
   // Keys of a block whose pages do not exist, a bit each; a block is filled at most four ahead of the one that the softmax warps are at.
@@ -100,11 +100,11 @@ constexpr bool ChunkFits(uint32_t bytes) { return bytes <= 227u * 1024u; }
 static_assert(ChunkFits(ChunkSmem<true, false, 128>()) && ChunkFits(ChunkSmem<true, true, 128>()) && ChunkFits(ChunkSmem<false, true, 128>()) &&
                   ChunkFits(ChunkSmem<false, true, 64>()), "shared memory of an SM");
 
-// Waits of limited time (as in tc_common.cuh): they end without success when another role has, or when kBudget has gone by both since they began and
+// Waits of limited time (as in tc_common.cuh): they end without success when another role has, or when the budget has gone by both since they began and
 // since a warp last said that it works rows out again, which may take long.
 __device__ __forceinline__ bool stuck(ChunkShared *S, unsigned long long t0) {
   const unsigned long long seen = *const_cast<volatile unsigned long long *>(&S->alive), now = globaltimer_ns();
-  return now > max(t0, seen) + kBudget;
+  return now - max(t0, min(seen, now)) > S->budget;
 }
 __device__ __forceinline__ bool wait_for(ChunkShared *S, uint64_t *bar, uint32_t parity) {
   if (mbar_try_wait_parity(bar, parity)) return true;
@@ -613,6 +613,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 }
 // The bits below bit n (none below 0, all from 32 on).
 __device__ __forceinline__ uint32_t below(int32_t n) { return static_cast<uint32_t>((1ull << max(0, min(32, n))) - 1ull); }
+constexpr uint16_t kLeft = 0xffffu;
 // x as the next bf16 that is not below it (its bits).
 __device__ __forceinline__ uint32_t rounded_up(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -632,9 +633,15 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
   uint16_t *top_s = reinterpret_cast<uint16_t *>(sm + Sh::kTops) + s * 256u + 32u * q4 + lane;      // [slot][half][row]
   float *sum_s = reinterpret_cast<float *>(sm + Sh::kTops + s * 512u + (lane >> 4) * 256u + 64u * q4) + (lane & 15u);      // (in the same two warps' bytes)
   uint32_t g = 0, n = 0, mine = 0;                        // blocks of all tiles; the slot's blocks and tiles
+  // A warp whose wait ran out meets the other of its pair once more, which may have got through: at the exchange of the maxima, where kLeft (no NaN that a
+  // maximum gives) tells it to leave as well, or at its own end.
+  auto leave = [&]() {
+    top_s[half * 128u] = kLeft;
+    bar_sync(pair, 64);
+  };
 #pragma unroll 1
   for (uint32_t turn = 0;; ++turn) {
-    if (!wait_together(S, &S->q_full, turn & 1u)) return;
+    if (!wait_together(S, &S->q_full, turn & 1u)) return leave();
     const Tile &t = S->tile;
     const uint32_t rows = t.rows, seq = t.seq, part_at = t.part, r0 = t.r0, t_head = t.head;
     const int32_t keys_lo = t.keys.lo, keys_hi = t.keys.hi;
@@ -643,7 +650,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
     const int32_t e = Q8 && BF ? S->q_exp[r] : 0;
     __syncwarp();
     if (lane == 0u) mbar_arrive(&S->q_free);
-    if (rows == 0u) return;
+    if (rows == 0u) return leave();
     if (s * kCkRows >= rows) {                            // the other slot's alone
       g += b1 - b0;
       continue;
@@ -656,7 +663,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
     bool redo = false;
 #pragma unroll 1
     for (uint32_t j = b0; j < b1; ++j, ++g, ++n) {
-      if (!wait_together(S, &S->s_full[s], n & 1u)) return;
+      if (!wait_together(S, &S->s_full[s], n & 1u)) return leave();
       tc_fence_after_sync();
       const int32_t j0 = keys_lo + static_cast<int32_t>(j * kCkKeys);
       const int32_t lo = sp.lo - j0, hi = sp.hi - j0;     // columns [lo, hi) of the block are seen
@@ -697,6 +704,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
       top_s[half * 128u] = static_cast<uint16_t>(own_up);
       bar_sync(pair, 64);
       const uint32_t other_up = top_s[(half ^ 1u) * 128u];
+      if (other_up == kLeft) return;                      // (all lanes)
       float mx = max3_nan(__uint_as_float(own_up << 16), __uint_as_float(other_up << 16), -INFINITY) * sl2;
       bool grow = mx > m_used + kGrow;
       float top = v_ref, vv[8];
@@ -809,7 +817,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
     bar_sync(pair, 64);
     if (half) l = *sum_s;
     bar_sync(pair, 64);                                   // (and the sum)
-    if (!wait_together(S, &S->pv_done[s], mine & 1u)) return;
+    if (!wait_together(S, &S->pv_done[s], mine & 1u)) return leave();
     ++mine;
     tc_fence_after_sync();
     const bool split = part_at != 0u;
@@ -927,6 +935,7 @@ __global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(c
       for (uint32_t i = 0; i < 2u; ++i) mbar_init(&S->scales_free[s][i], 8u);
     }
     S->failed = 0u;
+    S->budget = a.wait_budget_ns;
     S->alive = 0ull;
     fence_mbar_init();
   }

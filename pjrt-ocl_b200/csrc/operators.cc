@@ -29,6 +29,7 @@ struct b2_cache {
   uint32_t sms = 0;
   b2_cache_desc desc{};
   b2::CacheView view{};
+  uint64_t wait_budget_ns = 2000000000ull;      // (set while other threads' calls read it)
 };
 
 namespace {
@@ -329,6 +330,10 @@ void b2_cache_destroy(b2_cache *c) {
   delete c;
 }
 
+void b2_cache_set_wait_budget_ns(b2_cache *cache, uint64_t ns) {
+  if (cache) __atomic_store_n(&cache->wait_budget_ns, ns, __ATOMIC_RELAXED);
+}
+
 b2_status b2_cache_write(b2_cache *cache, const b2_batch *batch, const b2_rows *k, const b2_rows *v, void *cuda_stream, char *err, size_t err_cap) {
   return Entry("b2_cache_write", err, err_cap, [&]() -> b2_status { return Move("b2_cache_write", cache, batch, k, v, cuda_stream, true, err, err_cap); });
 }
@@ -365,6 +370,7 @@ b2_status b2_cache_attend(b2_cache *cache, b2_scratch *scratch, const b2_batch *
     a.window = window;
     a.bf16 = d.row_dtype == B2_BF16 ? 1u : 0u;
     a.e4m3 = d.dtype == B2_E4M3 ? 1u : 0u;
+    a.wait_budget_ns = __atomic_load_n(&cache->wait_budget_ns, __ATOMIC_RELAXED);
     OnDevice on(cache->device);
     cudaError_t e = on.error();
     if (e == cudaSuccess) {

@@ -97,6 +97,7 @@ struct AttendArgs {
   FastDiv by_group;
   uint32_t bf16;                   // type of the rows
   uint32_t e4m3;
+  uint64_t wait_budget_ns;         // of each wait on the tensor cores
 };
 
 // Keys that row i of a sequence sees: [lo, hi).

@@ -247,6 +247,10 @@ class PagedCache:
         if st:
             _check(st, err)
 
+    def set_wait_budget_ns(self, ns: int) -> None:
+        """Of each of attention's waits on the tensor cores, for the calls that follow (default 2e9)."""
+        lib().b2_cache_set_wait_budget_ns(self._h, ns)
+
     def Status(self) -> dict:
         """Waits for the device; raises what this cache's calls met since the last report."""
         st, err = _ExecStatus(), _errbuf()

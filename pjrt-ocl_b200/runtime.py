@@ -100,7 +100,7 @@ EXPORTS = [
     "b2_loaded_lane_timing", "b2_loaded_lane_times", "b2_loaded_in_out_result",
     "b2_loaded_preset_arrivals", "b2_scratch_create", "b2_scratch_destroy", "b2_rope_frequencies", "b2_rope_create",
     "b2_rope_destroy", "b2_rope_apply", "b2_rope_apply_backward", "b2_cache_create", "b2_cache_destroy", "b2_cache_write",
-    "b2_cache_read", "b2_cache_attend", "b2_cache_status",
+    "b2_cache_read", "b2_cache_attend", "b2_cache_status", "b2_cache_set_wait_budget_ns",
 ]
 
 
@@ -165,6 +165,7 @@ def lib():
         "b2_cache_write": (ctypes.c_int, [vp] * 5 + [cp, sz]),
         "b2_cache_read": (ctypes.c_int, [vp] * 5 + [cp, sz]),
         "b2_cache_attend": (ctypes.c_int, [vp] * 4 + [ctypes.c_float, ctypes.c_int, u32] + [vp] * 3 + [cp, sz]),
+        "b2_cache_set_wait_budget_ns": (None, [vp, ctypes.c_uint64]),
         "b2_cache_status": (ctypes.c_int, [vp, ctypes.POINTER(_ExecStatus), cp, sz]),
     }
     for name, (res, args) in sig.items():

@@ -241,3 +241,28 @@ def test_queries_of_any_size_over_8_bit_pages(rt, scratch, rows):
         assert p.cache.Status()["code"] == 0
         assert _near(o, want, _tol(p, want, tol)), e
         assert _near(lse, want_lse, 2.0 ** -19 * (1 + want_lse.abs())), e
+
+
+@pytest.mark.parametrize("dtype, row_dtype, dim", [("bf16", "bf16", 128), ("f16", "f16", 64), ("e4m3", "bf16", 128), ("e4m3", "f16", 64)])
+def test_waits_that_run_out_are_reported(rt, scratch, dtype, row_dtype, dim):
+    """With no time for any wait the roles of a CTA give up one after another, wherever they are: each call ends, and says so; those after it are
+    as ever."""
+    vm = package()
+    p = Paged(rt, [300, 40], [2000, 100], dtype=dtype, row_dtype=row_dtype, heads=4, q_heads=8, dim=dim, page=16, seed=2)
+    q = normal((p.n_rows, 8, dim), row_dtype, 8)
+    clean, _ = _call(p, scratch, q)
+    want, _, tol = p.attend(q, dim ** -0.5)
+    assert _near(clean, want, _tol(p, want, tol)) and p.cache.Status()["code"] == 0
+    reported = 0
+    for turn in range(12):
+        p.cache.set_wait_budget_ns(turn * 1000)
+        o, _ = _call(p, scratch, q)
+        try:
+            assert p.cache.Status()["code"] == 0 and torch.equal(o, clean)
+        except vm.DeadlineExceeded as e:
+            assert "tensor cores" in str(e)
+            reported += 1
+    assert reported > 0
+    p.cache.set_wait_budget_ns(2_000_000_000)
+    for _ in range(2):
+        assert torch.equal(_call(p, scratch, q)[0], clean) and p.cache.Status()["code"] == 0
