@@ -87,7 +87,7 @@ struct ChunkShared {
   unsigned long long alive;                               // when a warp last said that it is working rows out again
   alignas(16) float v_ref[2][8];                          // 8-bit pages: powers of two above V's scales of two blocks, 16 keys each; negative: scales far apart
   // Keys of a block whose pages do not exist, a bit each; a block is filled at most four ahead of the one that the softmax warps are at.
-  alignas(16) uint32_t absent[8][kCkKeys / 32u];
+  uint32_t absent[8][kCkKeys / 32u];
   Tile tile;                                              // no rows: the end
   union {
     unsigned long long find[30];                          // (before any row is looked at)
@@ -667,8 +667,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
       tc_fence_after_sync();
       const int32_t j0 = keys_lo + static_cast<int32_t>(j * kCkKeys);
       const int32_t lo = sp.lo - j0, hi = sp.hi - j0;     // columns [lo, hi) of the block are seen
-      const uint4 gone = *reinterpret_cast<const uint4 *>(S->absent[g & 7u]);
-      const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= static_cast<int32_t>(kCkKeys) && (gone.x | gone.y | gone.z | gone.w) == 0u);
+      const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= static_cast<int32_t>(kCkKeys) && S->absent[g & 7u][lane & 3u] == 0u);
       // 1: the row's maximum. The scores are read twice: half of a row's in registers at once leave too few for the rest
       const int32_t lo_h = lo - 64 * static_cast<int32_t>(half), hi_h = hi - 64 * static_cast<int32_t>(half);
       const float *ks = reinterpret_cast<const float *>(sm + Sh::kScales + (g & 1u) * 512u) + 64u * half;
@@ -704,9 +703,8 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
       top_s[half * 128u] = static_cast<uint16_t>(own_up);
       bar_sync(pair, 64);
       const uint32_t other_up = top_s[(half ^ 1u) * 128u];
-      if (other_up == kLeft) return;                      // (all lanes)
       float mx = max3_nan(__uint_as_float(own_up << 16), __uint_as_float(other_up << 16), -INFINITY) * sl2;
-      bool grow = mx > m_used + kGrow;
+      bool grow = !(mx <= m_used + kGrow);                // (a NaN as well)
       float top = v_ref, vv[8];
       if (Q8) {
         const float4 va = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u]), vb = *reinterpret_cast<const float4 *>(S->v_ref[g & 1u] + 4);
@@ -729,6 +727,7 @@ static __device__ __forceinline__ void chunk_rows(const AttendArgs &a, uint8_t *
       const bool move = __any_sync(0xffffffffu, grow);
       float alpha = 1.0f;
       if (move) {
+        if (other_up == kLeft) return;                    // (all lanes)
         bar_sync(pair, 64);
         top_s[half * 128u] = static_cast<uint16_t>(__float_as_uint(own));
         bar_sync(pair, 64);
