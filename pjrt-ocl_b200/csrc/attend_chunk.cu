@@ -104,31 +104,32 @@ static_assert(ChunkFits(ChunkSmem<true, false, 128>()) && ChunkFits(ChunkSmem<tr
 // since a warp last said that it works rows out again, which may take long.
 __device__ __forceinline__ bool stuck(ChunkShared *S, unsigned long long t0) {
   const unsigned long long seen = *const_cast<volatile unsigned long long *>(&S->alive), now = globaltimer_ns();
-  return now - max(t0, min(seen, now)) > S->budget;
+  return now - max(t0, min(seen, now)) >= S->budget;
 }
 __device__ __forceinline__ bool wait_for(ChunkShared *S, uint64_t *bar, uint32_t parity) {
   if (mbar_try_wait_parity(bar, parity)) return true;
   volatile uint32_t *failed = &S->failed;
   const unsigned long long t0 = globaltimer_ns();
   for (;;) {
-    for (int i = 0; i < 32; ++i)
-      if (mbar_try_wait_parity(bar, parity)) return true;
     if (*failed) return false;
     if (stuck(S, t0)) { *failed = 1u; return false; }
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait_parity(bar, parity)) return true;
   }
 }
+static __device__ __noinline__ bool wait_for_away(ChunkShared *S, uint64_t *bar, uint32_t parity) { return wait_for(S, bar, parity); }
 // (a whole warp, in step)
 __device__ __forceinline__ bool wait_together(ChunkShared *S, uint64_t *bar, uint32_t parity) {
   if (__all_sync(0xffffffffu, mbar_try_wait_parity(bar, parity))) return true;
   volatile uint32_t *failed = &S->failed;
   const unsigned long long t0 = globaltimer_ns();
   for (;;) {
-    for (int i = 0; i < 32; ++i)
-      if (__all_sync(0xffffffffu, mbar_try_wait_parity(bar, parity))) return true;
     if (__any_sync(0xffffffffu, *failed != 0u || stuck(S, t0))) {
       *failed = 1u;
       return false;
     }
+    for (int i = 0; i < 32; ++i)
+      if (__all_sync(0xffffffffu, mbar_try_wait_parity(bar, parity))) return true;
   }
 }
 
@@ -331,6 +332,12 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
       page = __ldg(a.b.pages + static_cast<int64_t>(t.seq) * a.b.pages_stride + entry);
     }
   };
+  // (the wait itself: 8-bit pages out of line, where the loop has the registers and not the code: 782 and 870 us for 796 and 908; 16-bit pages in line: 479 us
+  // for 596)
+  auto ready = [&](uint64_t *bar, uint32_t parity) {
+    if constexpr (Q8) return mbar_try_wait_parity(bar, parity) || wait_for_away(S, bar, parity);
+    else return wait_for(S, bar, parity);
+  };
   // ---- K and V ----
   uint32_t absent = 0u;
   auto place = [&](int64_t &off, int64_t &soff) -> uint32_t {       // the lane's key; which lanes of the warp have one, and which have one without a page
@@ -348,7 +355,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
       else to[w] = absent;
     }
   };
-  auto room = [&](uint32_t i) { return wait_for(S, &S->empty[i % NS], ((i / NS) & 1u) ^ 1u); };
+  auto room = [&](uint32_t i) { return ready(&S->empty[i % NS], ((i / NS) & 1u) ^ 1u); };
   auto done = [&](uint32_t i) {
     fence_proxy_async_smem();
     mbar_arrive(&S->full[i % NS]);
@@ -439,7 +446,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
     bool q_there = false;
     auto q_to_all = [&]() {                               // Q and the tile, when the scores of the tile before are done
       q_there = true;
-      ok = ok && __all_sync(0xffffffffu, wait_for(S, &S->q_free, (turn & 1u) ^ 1u));
+      ok = ok && __all_sync(0xffffffffu, ready(&S->q_free, (turn & 1u) ^ 1u));
       if (!ok) return;
       if (tid == 0u) S->tile = t;
       if (found) load_q<BF, Q8, HD>(a, t, tid, base, S->q_exp);
@@ -488,7 +495,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
         bool free = room(it);
         for (uint32_t s = 0; s < 2u; ++s) {
           uint32_t &n = used[s][buf];
-          if (n) free = free && wait_for(S, &S->scales_free[s][buf], (n - 1u) & 1u);
+          if (n) free = free && ready(&S->scales_free[s][buf], (n - 1u) & 1u);
           if (s < slots) ++n;
         }
         ok = __all_sync(0xffffffffu, free);
@@ -528,8 +535,8 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
   // the products have read what was filled last, and their arrivals on the ring's barriers are in
   if (ok && tid == 0u) {
     bool read = true;
-    for (uint32_t k = 0; k < NS && read; ++k) read = wait_for(S, &S->empty[(it + k) % NS], (((it + k) / NS) & 1u) ^ 1u);
-    wait_for(S, &S->q_free, (turn & 1u) ^ 1u);
+    for (uint32_t k = 0; k < NS && read; ++k) read = ready(&S->empty[(it + k) % NS], (((it + k) / NS) & 1u) ^ 1u);
+    ready(&S->q_free, (turn & 1u) ^ 1u);
   }
 }
 

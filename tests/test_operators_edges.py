@@ -255,7 +255,7 @@ def test_waits_that_run_out_are_reported(rt, scratch, dtype, row_dtype, dim):
     assert _near(clean, want, _tol(p, want, tol)) and p.cache.Status()["code"] == 0
     reported = 0
     for turn in range(12):
-        p.cache.set_wait_budget_ns(turn * 1000)
+        p.cache.set_wait_budget_ns(turn // 4 * 1000)             # (0: the first look has to do)
         o, _ = _call(p, scratch, q)
         try:
             assert p.cache.Status()["code"] == 0 and torch.equal(o, clean)
