@@ -7,6 +7,7 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <mutex>
 #include <new>
 #include <string>
 
@@ -94,6 +95,24 @@ b2::BatchView View(const b2_batch *b) {
   return v;
 }
 
+// What the handles of a device have in common, made with the first of them and kept: the kernels' attributes, and a stream on which the contents of
+// a new handle are settled without waiting for anything else on the device. The device is current.
+cudaError_t OfDevice(int device, cudaStream_t *stream) {
+  static std::mutex lock;
+  static cudaStream_t streams[64] = {};
+  if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> held(lock);
+  if (!streams[device]) {
+    for (int e : {b2::PrepareRope(), b2::PrepareAttendStep(), b2::PrepareAttendChunk()})
+      if (e) return static_cast<cudaError_t>(e);
+    const cudaError_t e = cudaStreamCreateWithFlags(&streams[device], cudaStreamNonBlocking);
+    if (e != cudaSuccess) return e;
+  }
+  *stream = streams[device];
+  return cudaSuccess;
+}
+b2_status Kind(cudaError_t e) { return e == cudaErrorMemoryAllocation ? B2_RESOURCE_EXHAUSTED : B2_INTERNAL; }
+
 // What every create call needs of a runtime.
 template <typename H>
 b2_status OfRuntime(const char *name, b2_runtime *rt, H *h, char *err, size_t cap) {
@@ -135,11 +154,13 @@ b2_status b2_scratch_create(b2_runtime *rt, b2_scratch **out, char *err, size_t 
     OnDevice on(s.device);
     const size_t uses[3] = {sizeof(float) * 2 * 256 * b2::RopeBackwardCtas(s.sms), b2::AttendStepPartialBytes(s.sms), b2::AttendChunkPartialBytes(s.sms)};
     s.bytes = kCounterBytes + std::max(uses[0], std::max(uses[1], uses[2]));
+    cudaStream_t own = nullptr;
     cudaError_t e = on.error();
+    if (e == cudaSuccess) e = OfDevice(s.device, &own);
     if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&s.mem), s.bytes);
-    if (e != cudaSuccess) return CudaFail(err, err_cap, "b2_scratch_create", e, B2_RESOURCE_EXHAUSTED);
-    e = cudaMemset(s.mem, 0, kCounterBytes);
-    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) return CudaFail(err, err_cap, "b2_scratch_create", e, Kind(e));
+    e = cudaMemsetAsync(s.mem, 0, kCounterBytes, own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(own);
     b2_scratch *h = e == cudaSuccess ? new (std::nothrow) b2_scratch(s) : nullptr;
     if (!h) {
       cudaFree(s.mem);
@@ -198,12 +219,13 @@ b2_status b2_rope_create(b2_runtime *rt, const b2_rope_desc *desc, b2_rope **out
     double turns[128];
     for (uint32_t i = 0; i < desc->rot_dim / 2; ++i) turns[i] = desc->frequencies[i] / (2.0 * 3.14159265358979323846);
     OnDevice on(r.device);
+    cudaStream_t own = nullptr;
     cudaError_t e = on.error();
-    if (e == cudaSuccess) e = static_cast<cudaError_t>(b2::PrepareRope());
+    if (e == cudaSuccess) e = OfDevice(r.device, &own);
     if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void **>(&r.turns), sizeof turns);
-    if (e != cudaSuccess) return CudaFail(err, err_cap, name, e, B2_RESOURCE_EXHAUSTED);
-    e = cudaMemcpy(r.turns, turns, sizeof(double) * (desc->rot_dim / 2), cudaMemcpyHostToDevice);
-    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) return CudaFail(err, err_cap, name, e, Kind(e));
+    e = cudaMemcpyAsync(r.turns, turns, sizeof(double) * (desc->rot_dim / 2), cudaMemcpyHostToDevice, own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(own);
     b2_rope *h = e == cudaSuccess ? new (std::nothrow) b2_rope(r) : nullptr;
     if (!h) {
       cudaFree(r.turns);
@@ -307,13 +329,13 @@ b2_status b2_cache_create(b2_runtime *rt, const b2_cache_desc *desc, b2_cache **
     v.n_pages = desc->n_pages; v.page_size = desc->page_size; v.heads = desc->heads; v.hd = desc->head_dim;
     v.by_page = b2::FastDiv(desc->page_size);
     OnDevice on(c.device);
+    cudaStream_t own = nullptr;
     cudaError_t ce = on.error();
-    if (ce == cudaSuccess) ce = static_cast<cudaError_t>(b2::PrepareAttendStep());
-    if (ce == cudaSuccess) ce = static_cast<cudaError_t>(b2::PrepareAttendChunk());
+    if (ce == cudaSuccess) ce = OfDevice(c.device, &own);
     if (ce == cudaSuccess) ce = cudaMalloc(reinterpret_cast<void **>(&v.status), 4 * sizeof(uint32_t));
-    if (ce != cudaSuccess) return CudaFail(err, err_cap, name, ce, ce == cudaErrorMemoryAllocation ? B2_RESOURCE_EXHAUSTED : B2_INTERNAL);
-    ce = cudaMemset(v.status, 0, 4 * sizeof(uint32_t));
-    if (ce == cudaSuccess) ce = cudaDeviceSynchronize();
+    if (ce != cudaSuccess) return CudaFail(err, err_cap, name, ce, Kind(ce));
+    ce = cudaMemsetAsync(v.status, 0, 4 * sizeof(uint32_t), own);
+    if (ce == cudaSuccess) ce = cudaStreamSynchronize(own);
     b2_cache *h = ce == cudaSuccess ? new (std::nothrow) b2_cache(c) : nullptr;
     if (!h) {
       cudaFree(v.status);

@@ -266,3 +266,31 @@ def test_waits_that_run_out_are_reported(rt, scratch, dtype, row_dtype, dim):
     p.cache.set_wait_budget_ns(2_000_000_000)
     for _ in range(2):
         assert torch.equal(_call(p, scratch, q)[0], clean) and p.cache.Status()["code"] == 0
+
+
+def test_handles_are_made_while_the_device_is_busy(rt, scratch):
+    """A server makes and captures for a new batch while its last one runs: nothing of that is waited for."""
+    vm = package()
+    p = Paged(rt, [3], [20], heads=2, dim=64)
+    vm.Rope.Create(rt, 64, 2, 2, "bf16")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ends = []
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(2_000_000_000)                     # about a second
+            ends.append(torch.cuda.Event())
+            ends[-1].record()
+    first = p.cache                                              # (a handle that goes waits: its memory may be in use)
+    p.bind()
+    rope, other = vm.Rope.Create(rt, 64, 2, 2, "bf16"), vm.Scratch.Create(rt)
+    assert not any(e.query() for e in ends)
+    torch.cuda.synchronize()
+    q = normal((3, 2, 64), "bf16", 1)
+    want, _, tol = p.attend(q, 0.125)
+    assert _near(_call(p, other, q)[0], want, _tol(p, want, tol)) and p.cache.Status()["code"] == 0
+    out, pos = torch.empty_like(q), torch.zeros(3, dtype=torch.int32, device="cuda")
+    r = vm.Rows.Of
+    rope.Apply(3, pos.data_ptr(), r(q), r(q), r(out), r(out))
+    assert torch.equal(out, q)                                   # (position 0)
+    first.close()
