@@ -113,6 +113,15 @@ cudaError_t OfDevice(int device, cudaStream_t *stream) {
 }
 b2_status Kind(cudaError_t e) { return e == cudaErrorMemoryAllocation ? B2_RESOURCE_EXHAUSTED : B2_INTERNAL; }
 
+// Memory of a handle that goes. Waits for what uses it; a capture that is under way on some stream stays as it is.
+void Release(void *p) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  cudaFree(p);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  cudaGetLastError();
+}
+
 // What every create call needs of a runtime.
 template <typename H>
 b2_status OfRuntime(const char *name, b2_runtime *rt, H *h, char *err, size_t cap) {
@@ -173,7 +182,7 @@ b2_status b2_scratch_create(b2_runtime *rt, b2_scratch **out, char *err, size_t 
 void b2_scratch_destroy(b2_scratch *s) {
   if (!s) return;
   OnDevice on(s->device);
-  cudaFree(s->mem);
+  Release(s->mem);
   delete s;
 }
 
@@ -238,7 +247,7 @@ b2_status b2_rope_create(b2_runtime *rt, const b2_rope_desc *desc, b2_rope **out
 void b2_rope_destroy(b2_rope *r) {
   if (!r) return;
   OnDevice on(r->device);
-  cudaFree(r->turns);
+  Release(r->turns);
   delete r;
 }
 
@@ -348,7 +357,7 @@ b2_status b2_cache_create(b2_runtime *rt, const b2_cache_desc *desc, b2_cache **
 void b2_cache_destroy(b2_cache *c) {
   if (!c) return;
   OnDevice on(c->device);
-  cudaFree(c->view.status);
+  Release(c->view.status);
   delete c;
 }
 

@@ -294,3 +294,23 @@ def test_handles_are_made_while_the_device_is_busy(rt, scratch):
     rope.Apply(3, pos.data_ptr(), r(q), r(q), r(out), r(out))
     assert torch.equal(out, q)                                   # (position 0)
     first.close()
+
+
+def test_handles_that_go_during_a_capture(rt, scratch):
+    """As a collector does it: the capture is not ended by it, and its graph runs."""
+    vm = package()
+    p = Paged(rt, [3], [20], heads=2, dim=64)
+    gone = [vm.Rope.Create(rt, 64, 2, 2, "bf16"), vm.Scratch.Create(rt), p.cache]
+    p.bind()
+    q = normal((3, 2, 64), "bf16", 1)
+    want, _ = _call(p, scratch, q)
+    o, r = torch.zeros_like(q), vm.Rows.Of
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=side):
+        for handle in gone:
+            handle.close()
+        p.cache.Attend(p.batch, r(q), r(o), scratch, stream=side.cuda_stream)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, want) and p.cache.Status()["code"] == 0
