@@ -257,7 +257,7 @@ b2_status b2_rope_frequencies(uint32_t rot_dim, double base, int scaling, double
 b2_status b2_rope_create(b2_runtime *rt, const b2_rope_desc *desc, b2_rope **out, char *err, size_t err_cap);
 void b2_rope_destroy(b2_rope *rope);
 /* positions: device, n_rows int32. Weights: device, head_dim values each; NULL = ones. The results may be written over
- * the inputs (same data and strides). */
+ * the inputs (same data and strides); else results and inputs lie apart, and so do the two results and the rows of each. */
 b2_status b2_rope_apply(const b2_rope *rope, uint32_t n_rows, const void *positions, const b2_rows *q, const b2_rows *k,
                         const void *q_weight, const void *k_weight, const b2_rows *q_out, const b2_rows *k_out,
                         void *cuda_stream, char *err, size_t err_cap);
@@ -317,7 +317,8 @@ b2_status b2_cache_read(b2_cache *cache, const b2_batch *batch, const b2_rows *k
  * own position, of these the last `window` (0 = all); else every position of its sequence (window must be 0). Values
  * that a row does not see never reach it, whatever they are. A row that sees nothing gives zeros. lse (may be NULL):
  * f32 [n_rows][q_heads], the logarithm of the softmax's sum (-inf for a row that sees nothing). Rows are B2_F16 or
- * B2_BF16. 0 < scale <= 1e38; max_rows x query heads to a cache head below 2^31. out must not lie over q. e4m3 scales
+ * B2_BF16. 0 < scale <= 1e38; max_rows x query heads to a cache head below 2^31. out must not lie over q, nor its rows
+ * or heads over each other. e4m3 scales
  * count in full from 2^-80 to 2^103. */
 b2_status b2_cache_attend(b2_cache *cache, b2_scratch *scratch, const b2_batch *batch, const b2_rows *q, float scale,
                           int causal, uint32_t window, const b2_rows *out, void *lse, void *cuda_stream, char *err,

@@ -139,6 +139,10 @@ b2_status Move(const char *name, b2_cache *c, const b2_batch *batch, const b2_ro
   std::string m = b2::CheckBatch(batch);
   if (m.empty()) m = b2::CheckRows("k", k, batch->n_rows, c->desc.heads, c->desc.row_dtype);
   if (m.empty()) m = b2::CheckRows("v", v, batch->n_rows, c->desc.heads, c->desc.row_dtype);
+  if (m.empty() && !write) {
+    const b2_cache_desc &d = c->desc;
+    if ((m = b2::CheckResult("k", k, batch->n_rows, d.heads, d.head_dim, d.row_dtype)).empty()) m = b2::CheckResult("v", v, batch->n_rows, d.heads, d.head_dim, d.row_dtype);
+  }
   if (!m.empty()) return Refuse(name, err, cap, m);
   if (!batch->n_seqs || !batch->n_rows) return B2_OK;
   OnDevice on(c->device);
@@ -283,6 +287,16 @@ static b2_status RopeCall(const char *name, const b2_rope *r, b2_scratch *scratc
     a.heads[t] = heads[t];
     any_dw = any_dw || a.dw[t];
   }
+  for (int t = 0; t < 2; ++t) {
+    const char *const result = backward ? "gradient of an input" : "result";
+    std::string m = b2::CheckResult(result, y[t], n_rows, heads[t], d.head_dim, d.dtype);
+    for (int u = 0; u < 2 && m.empty(); ++u) {
+      if (need_x) m = b2::CheckApart(result, y[t], heads[t], of[u], x[u], heads[u], n_rows, d.head_dim, d.dtype, t == u);
+      if (m.empty() && backward) m = b2::CheckApart(result, y[t], heads[t], "gradient of a result", g[u], heads[u], n_rows, d.head_dim, d.dtype, t == u);
+    }
+    if (m.empty() && t) m = b2::CheckApart(result, y[1], heads[1], "the other result", y[0], heads[0], n_rows, d.head_dim, d.dtype, false);
+    if (!m.empty()) return Refuse(name, err, cap, m);
+  }
   if (any_dw) {
     if (!scratch) return Refuse(name, err, cap, "gradients of weights need a scratch");
     if (scratch->device != r->device) return Refuse(name, err, cap, "the scratch is another device's");
@@ -378,7 +392,9 @@ b2_status b2_cache_attend(b2_cache *cache, b2_scratch *scratch, const b2_batch *
     const char *name = "b2_cache_attend";
     if (!cache) return Refuse(name, err, err_cap, "null cache");
     const b2_cache_desc &d = cache->desc;
-    const std::string m = b2::CheckAttend(d, batch, q, out, scale, causal, window, lse);
+    std::string m = b2::CheckAttend(d, batch, q, out, scale, causal, window, lse);
+    if (m.empty()) m = b2::CheckResult("out", out, batch->n_rows, d.q_heads, d.head_dim, d.row_dtype);
+    if (m.empty()) m = b2::CheckApart("out", out, d.q_heads, "q (a row of q may be read after its result is there)", q, d.q_heads, batch->n_rows, d.head_dim, d.row_dtype, false);
     if (!m.empty()) return Refuse(name, err, err_cap, m, d.row_dtype == B2_F32 && b2::CheckBatch(batch).empty() ? B2_UNIMPLEMENTED : B2_INVALID_ARGUMENT);
     if (!scratch) return Refuse(name, err, err_cap, "null scratch");
     if (scratch->device != cache->device) return Refuse(name, err, err_cap, "the scratch is another device's");

@@ -131,6 +131,10 @@ std::string CheckRopeDesc(const b2_rope_desc *d);
 std::string CheckCacheDesc(const b2_cache_desc *d);
 std::string CheckBatch(const b2_batch *b);
 std::string CheckRows(const char *what, const b2_rows *r, uint32_t n_rows, uint32_t heads, uint32_t dtype);
+// Results: their own rows and heads apart from each other, and apart from other rows (`same`: but for the very same ones). Both sets have been checked as rows.
+std::string CheckResult(const char *what, const b2_rows *r, uint32_t n_rows, uint32_t heads, uint32_t head_dim, uint32_t dtype);
+std::string CheckApart(const char *result, const b2_rows *y, uint32_t y_heads, const char *other, const b2_rows *x, uint32_t x_heads, uint32_t n_rows, uint32_t head_dim, uint32_t dtype,
+                       bool same);
 std::string CheckAttend(const b2_cache_desc &d, const b2_batch *b, const b2_rows *q, const b2_rows *o, float scale, int causal, uint32_t window, const void *lse);
 
 // ---- launches; each returns a cudaError_t's value ----

@@ -1,6 +1,8 @@
 // What the operators' entry points refuse before anything reaches the device. Host only: no CUDA here.
 #include <math.h>
 
+#include <algorithm>
+
 #include "operators.h"
 
 namespace b2 {
@@ -10,7 +12,55 @@ std::string N(uint64_t v) { return std::to_string(v); }
 bool Float(uint32_t t) { return t == B2_F32 || t == B2_F16 || t == B2_BF16; }
 bool Half(uint32_t t) { return t == B2_F16 || t == B2_BF16; }
 
+// Rows by bytes: head h of row r is `width` bytes from at + r row + h head.
+typedef __int128 Wide;               // (2^31 rows of strides up to 2^40)
+struct Place {
+  Wide at, row, head, lo, hi;        // [lo, hi): all of it
+  int64_t n, heads, width;
+  Place(const b2_rows &r, uint32_t rows, uint32_t h, uint32_t head_dim, uint32_t dtype) : n(rows), heads(h) {
+    const int64_t e = TypeBytes(dtype);
+    at = static_cast<Wide>(reinterpret_cast<uintptr_t>(r.data));
+    row = rows > 1 ? static_cast<Wide>(r.row_stride) * e : 0;
+    head = h > 1 ? static_cast<Wide>(r.head_stride) * e : 0;
+    width = head_dim * e;
+    const Wide far_row = row * (n - 1), far_head = head * (heads - 1);
+    lo = at + std::min<Wide>(far_row, 0) + std::min<Wide>(far_head, 0);
+    hi = at + std::max<Wide>(far_row, 0) + std::max<Wide>(far_head, 0) + width;
+  }
+};
+Wide Abs(Wide x) { return x < 0 ? -x : x; }
+// Whether |d - r row - h head| < width for some r in (-n, n) and h in [h0, h1]; `itself`: but for r = h = 0.
+bool Meets(Wide d, Wide row, Wide head, int64_t n, int64_t h0, int64_t h1, int64_t width, bool itself) {
+  for (int64_t h = h0; h <= h1; ++h) {
+    const Wide rest = d - h * head, near = row ? std::max<Wide>(1 - n, std::min<Wide>(rest / row, n - 1)) : 0;
+    for (Wide r = near - 1; r <= near + 1; ++r)
+      if (Abs(r) < n && Abs(rest - r * row) < width && !(itself && r == 0 && h == 0)) return true;
+  }
+  return false;
+}
+
 }  // namespace
+
+std::string CheckResult(const char *what, const b2_rows *r, uint32_t n_rows, uint32_t heads, uint32_t head_dim, uint32_t dtype) {
+  if (n_rows == 0 || heads == 0) return "";
+  const Place p(*r, n_rows, heads, head_dim, dtype);
+  const bool by_rows = (heads == 1 || Abs(p.head) >= p.width) && (n_rows == 1 || Abs(p.row) >= Abs(p.head) * (p.heads - 1) + p.width);
+  const bool by_heads = (n_rows == 1 || Abs(p.row) >= p.width) && (heads == 1 || Abs(p.head) >= Abs(p.row) * (p.n - 1) + p.width);
+  if (by_rows || by_heads || !Meets(0, p.row, p.head, p.n, 0, p.heads - 1, p.width, true)) return "";
+  return std::string(what) + ": rows or heads lie over each other";
+}
+
+std::string CheckApart(const char *result, const b2_rows *y, uint32_t y_heads, const char *other, const b2_rows *x, uint32_t x_heads, uint32_t n_rows, uint32_t head_dim,
+                       uint32_t dtype, bool same) {
+  if (n_rows == 0 || y_heads == 0 || x_heads == 0) return "";
+  const Place p(*y, n_rows, y_heads, head_dim, dtype), q(*x, n_rows, x_heads, head_dim, dtype);
+  if (p.hi <= q.lo || q.hi <= p.lo) return "";
+  const bool rows_alike = p.row == q.row, heads_alike = p.head == q.head || y_heads == 1 || x_heads == 1;
+  if (same && p.at == q.at && rows_alike && p.head == q.head) return "";
+  // (rows of different strides in the same memory: taken to meet)
+  if (rows_alike && heads_alike && !Meets(q.at - p.at, p.row, y_heads > 1 ? p.head : q.head, p.n, 1 - q.heads, p.heads - 1, p.width, false)) return "";
+  return std::string(result) + " lies over " + other;
+}
 
 std::string CheckRopeDesc(const b2_rope_desc *d) {
   if (!d) return "null description";

@@ -291,7 +291,7 @@ def test_handles_are_made_while_the_device_is_busy(rt, scratch):
     assert _near(_call(p, other, q)[0], want, _tol(p, want, tol)) and p.cache.Status()["code"] == 0
     out, pos = torch.empty_like(q), torch.zeros(3, dtype=torch.int32, device="cuda")
     r = vm.Rows.Of
-    rope.Apply(3, pos.data_ptr(), r(q), r(q), r(out), r(out))
+    rope.Apply(3, pos.data_ptr(), r(q), r(q), r(out), r(torch.empty_like(q)))
     assert torch.equal(out, q)                                   # (position 0)
     first.close()
 
@@ -314,3 +314,45 @@ def test_handles_that_go_during_a_capture(rt, scratch):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(o, want) and p.cache.Status()["code"] == 0
+
+
+def test_results_over_inputs_or_themselves_are_refused(rt, scratch):
+    vm = package()
+    p = Paged(rt, [2, 3], [20, 5], heads=2, q_heads=4, dim=64)
+    r = vm.Rows.Of
+    flat = normal((6 * 8 * 64,), "bf16", 1)
+    fused = flat[:5 * 8 * 64].view(5, 8, 64)
+    q, beside = fused[:, :4], fused[:, 4:]
+    for out in (q, flat[64:64 + 5 * 512].view(5, 8, 64)[:, :4], flat[512:512 + 5 * 512].view(5, 8, 64)[:, :4], fused[:, 1:5], fused[:, 3:7], flat[1:1 + 5 * 512].view(5, 8, 64)[:, :4],
+                flat[512 - 63:512 - 63 + 5 * 512].view(5, 8, 64)[:, :4], flat[256:256 + 5 * 256].view(5, 4, 64)):
+        with pytest.raises(vm.InvalidArgument, match="over q"):
+            p.cache.Attend(p.batch, r(q), r(out), scratch)
+    for out in (beside, flat.new_empty(5, 4, 64), fused.new_empty(4, 5, 64).transpose(0, 1)):
+        p.cache.Attend(p.batch, r(q), r(out), scratch)
+    for out in (fused.new_empty(1, 4, 64).expand(5, 4, 64), fused.new_empty(5, 1, 64).expand(5, 4, 64), fused.new_empty(2000).as_strided((5, 4, 64), (128, 64, 1)),
+                fused.new_empty(2000).as_strided((5, 4, 64), (63, 400, 1))):
+        with pytest.raises(vm.InvalidArgument, match="over each other"):
+            p.cache.Attend(p.batch, r(q), r(out), scratch)
+    for out in (fused.new_empty(1, 2, 64).expand(5, 2, 64), fused.new_empty(5, 1, 64).expand(5, 2, 64)):
+        with pytest.raises(vm.InvalidArgument, match="over each other"):
+            p.cache.Read(p.batch, r(q[:, :2].clone()), r(out))
+    p.cache.Attend(p.batch, r(q), r(fused.new_empty(2000).as_strided((5, 4, 64), (65, 390, 1))), scratch)      # (heads first, a gap in each row)
+    pos = torch.arange(5, dtype=torch.int32, device="cuda")
+    k, other = fused[:, 4:6], fused.new_empty(5, 4, 64)
+    rope = vm.Rope.Create(rt, 64, 4, 2, "bf16")
+    want = [torch.empty_like(t) for t in (q, k)]
+    rope.Apply(5, pos.data_ptr(), r(q), r(k), r(want[0]), r(want[1]))
+    for q_out, k_out, part in ((fused[:, 1:5], k, "over q"), (q, fused[:, 3:5], "over q"), (k.new_empty(5, 4, 64), fused[:, 5:7], "over k"), (fused[:, 2:6], k.new_empty(5, 2, 64), "over q"),
+                               (other, other[:, :2], "other result"), (other[:1].expand(5, 4, 64), k, "over each other")):
+        with pytest.raises(vm.InvalidArgument, match=part):
+            rope.Apply(5, pos.data_ptr(), r(q), r(k), r(q_out), r(k_out))
+    g = [normal(t.shape, "bf16", 5) for t in (q, k)]
+    with pytest.raises(vm.InvalidArgument, match="over gradient of a result"):
+        rope.ApplyBackward(5, pos.data_ptr(), None, None, r(g[0]), r(g[1]), r(other), r(g[0][:, 2:]))
+    rope.Apply(5, pos.data_ptr(), r(q), r(k), r(q), r(k))        # over its own inputs, in the fused rows
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    one = vm.Rope.Create(rt, 64, 1, 1, "bf16")                   # one row, one head: strides say nothing
+    x = normal((3, 64), "bf16", 1)
+    one.Apply(1, pos.data_ptr(), vm.Rows(x[0].data_ptr(), "bf16", (1, 1, 64), (0, 0)), vm.Rows(x[1].data_ptr(), "bf16", (1, 1, 64), (7, 3)), vm.Rows(x[0].data_ptr(), "bf16", (1, 1, 64), (1, 1)),
+              vm.Rows(x[2].data_ptr(), "bf16", (1, 1, 64)))
+    assert torch.equal(x[2], x[1]) and p.cache.Status()["code"] == 0
