@@ -1,13 +1,14 @@
 """The operators beside the programs (include/b2vm.h): rotary positions with the norms of queries and keys, a paged
 cache of keys and values, and the attention of new rows over it. No counterpart in the reference.
 
-Device buffers are the caller's, as addresses (`data_ptr()` of a torch tensor, or what `Runtime.AllocDevice` gave);
-rows x heads x head_dim tensors as `Rows`. Calls are enqueued on `stream` (0 = the default stream of the runtime's
+Device buffers are the caller's: a torch tensor, whose type, size and device are checked, or an address (`data_ptr()`, or
+what `Runtime.AllocDevice` gave), which is taken as it is; rows x heads x head_dim tensors as `Rows`. Calls are enqueued on `stream` (0 = the default stream of the runtime's
 device) and not waited for; a refusal raises the same errors as the rest of the package.
 """
 from __future__ import annotations
 
 import ctypes
+import operator
 import threading
 
 from .runtime import _ERRCAP, InvalidArgument, Runtime, _check, _errbuf, _ExecStatus, lib
@@ -55,6 +56,26 @@ def _dtype(name: str) -> int:
     if name not in DTYPES:
         raise InvalidArgument(f"unknown type {name!r} (one of {', '.join(DTYPES)})")
     return DTYPES[name]
+
+
+_NAMES = {"i32": "torch.int32", "f32": "torch.float32", "f16": "torch.float16", "bf16": "torch.bfloat16"}
+
+
+def _address(what: str, x, dtype: str, n: int, device) -> int:
+    """The address of `n` values of a type: an address already, None (0), or a tensor that has them without gaps."""
+    if type(x) is int:
+        return x
+    if x is None:
+        return 0
+    if not hasattr(x, "data_ptr"):
+        return operator.index(x)
+    if str(x.dtype) != _NAMES[dtype]:
+        raise InvalidArgument(f"{what}: of type {x.dtype}, want {_NAMES[dtype]}")
+    if not x.is_cuda or (device is not None and x.device.index != device):
+        raise InvalidArgument(f"{what}: on {x.device}, the runtime is on {'a device' if device is None else device}")
+    if not x.is_contiguous() or x.numel() < n:
+        raise InvalidArgument(f"{what}: {list(x.shape)} of strides {list(x.stride())}, want {n} values without gaps")
+    return x.data_ptr()
 
 
 class Rows:
@@ -141,6 +162,7 @@ class Rope:
     def __init__(self, rt: Runtime, handle, desc: dict):
         self._rt, self._h, self.desc = rt, handle, desc
         self._dev = rt.device_ordinal
+        self._dim, self._wt = desc["head_dim"], desc["weight_dtype"]
         self._q, self._k = ((desc["dtype"], desc[heads], desc["head_dim"]) for heads in ("q_heads", "k_heads"))
         self._apply, self._back = lib().b2_rope_apply, lib().b2_rope_apply_backward
 
@@ -155,24 +177,30 @@ class Rope:
         d = _RopeDesc(head_dim, rot_dim, q_heads, k_heads, _dtype(dtype), _dtype(weight_dtype), int(interleaved), int(norm), eps, magnitude, arr)
         h, err = ctypes.c_void_p(), _errbuf()
         _check(lib().b2_rope_create(rt._h if rt is not None else None, ctypes.byref(d), ctypes.byref(h), err, _ERRCAP), err)
-        return Rope(rt, h, {"head_dim": head_dim, "q_heads": q_heads, "k_heads": k_heads, "dtype": dtype, "norm": bool(norm)})
+        return Rope(rt, h, {"head_dim": head_dim, "q_heads": q_heads, "k_heads": k_heads, "dtype": dtype, "norm": bool(norm), "weight_dtype": weight_dtype})
 
-    def Apply(self, n_rows: int, positions: int, q, k, q_out, k_out, q_weight: int = 0, k_weight: int = 0, stream: int = 0) -> None:
+    def Apply(self, n_rows: int, positions, q, k, q_out, k_out, q_weight=0, k_weight=0, stream: int = 0) -> None:
+        """`positions`: int32 [n_rows]; weights: head_dim values each, or 0 (ones)."""
         dev, qk, kk, err = self._dev, self._q, self._k, _local.err
+        if not type(positions) is type(q_weight) is type(k_weight) is int:      # (small calls' time is Python's)
+            positions = _address("positions", positions, "i32", n_rows, dev)
+            q_weight, k_weight = (_address(what, t, self._wt, self._dim, dev) for what, t in (("q_weight", q_weight), ("k_weight", k_weight)))
         st = self._apply(self._h, n_rows, positions, _rows("q", q, dev, n_rows, qk), _rows("k", k, dev, n_rows, kk), q_weight, k_weight,
                          _rows("q_out", q_out, dev, n_rows, qk), _rows("k_out", k_out, dev, n_rows, kk), stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
-    def ApplyBackward(self, n_rows: int, positions: int, q, k, dq_out, dk_out, dq, dk, q_weight: int = 0, k_weight: int = 0, dq_weight: int = 0, dk_weight: int = 0,
+    def ApplyBackward(self, n_rows: int, positions, q, k, dq_out, dk_out, dq, dk, q_weight=0, k_weight=0, dq_weight=0, dk_weight=0,
                       scratch: Scratch = None, stream: int = 0) -> None:
         """Gradients; q and k (the inputs of Apply) are needed with norm only, `scratch` for those of the weights."""
         dev, qk, kk, err = self._dev, self._q, self._k, _local.err
         norm = self.desc["norm"]
         x = [None if r is None and not norm else _rows(what, r, dev, n_rows, kind) for what, r, kind in (("q", q, qk), ("k", k, kk))]
-        st = self._back(self._h, scratch._h if scratch is not None else None, n_rows, positions, x[0], x[1], q_weight, k_weight,
+        w = [_address(what, t, self._wt, self._dim, dev) for what, t in (("q_weight", q_weight), ("k_weight", k_weight))]
+        dw = [_address(what, t, "f32", self._dim, dev) for what, t in (("dq_weight", dq_weight), ("dk_weight", dk_weight))]
+        st = self._back(self._h, scratch._h if scratch is not None else None, n_rows, _address("positions", positions, "i32", n_rows, dev), x[0], x[1], w[0], w[1],
                         _rows("dq_out", dq_out, dev, n_rows, qk), _rows("dk_out", dk_out, dev, n_rows, kk),
-                        _rows("dq", dq, dev, n_rows, qk), _rows("dk", dk, dev, n_rows, kk), dq_weight, dk_weight, stream, err, _ERRCAP)
+                        _rows("dq", dq, dev, n_rows, qk), _rows("dk", dk, dev, n_rows, kk), dw[0], dw[1], stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
@@ -189,16 +217,22 @@ class Rope:
 
 
 class Batch:
-    """Sequences of a batch: device addresses of int32 row_start[n_seqs + 1], length[n_seqs] and pages[n_seqs][pages_stride],
-    and the bounds that the host knows (see b2_batch)."""
+    """Sequences of a batch: int32 row_start[n_seqs + 1], length[n_seqs] and pages[n_seqs][pages_stride] on the device (tensors are
+    kept), and the bounds that the host knows (see b2_batch)."""
 
-    __slots__ = ("_keep", "_ref", "n_rows")
+    __slots__ = ("_keep", "_ref", "n_rows", "_device", "_tensors")
 
-    def __init__(self, n_seqs: int, row_start: int, length: int, pages: int, max_pages: int, n_rows: int, max_rows: int = 0, pages_stride=None):
+    def __init__(self, n_seqs: int, row_start, length, pages, max_pages: int, n_rows: int, max_rows: int = 0, pages_stride=None):
         for what, v in (("n_seqs", n_seqs), ("max_pages", max_pages), ("n_rows", n_rows), ("max_rows", max_rows)):
             if not 0 <= v <= 0xFFFFFFFF:
                 raise InvalidArgument(f"{what} {v} is out of range")
-        self._keep = _BatchC(n_seqs, n_rows, max_rows, max_pages, max_pages if pages_stride is None else pages_stride, row_start, length, pages)
+        self._tensors = [t for t in (row_start, length, pages) if hasattr(t, "data_ptr")]
+        self._device = self._tensors[0].device.index if self._tensors and self._tensors[0].is_cuda else None
+        if pages_stride is None:
+            pages_stride = pages.shape[1] if hasattr(pages, "data_ptr") and pages.dim() == 2 else max_pages
+        row_start, length, pages = (_address(what, t, "i32", n, self._device) for what, t, n in (
+            ("row_start", row_start, n_seqs + 1), ("length", length, n_seqs), ("pages", pages, (n_seqs - 1) * pages_stride + max_pages if n_seqs else 0)))
+        self._keep = _BatchC(n_seqs, n_rows, max_rows, max_pages, pages_stride, row_start, length, pages)
         self._ref = ctypes.byref(self._keep)
         self.n_rows = n_rows
 
@@ -225,25 +259,30 @@ class PagedCache:
         _check(lib().b2_cache_create(rt._h if rt is not None else None, ctypes.byref(d), ctypes.byref(h), err, _ERRCAP), err)
         return PagedCache(rt, h, {"dtype": dtype, "row_dtype": row_dtype, "heads": heads, "q_heads": q_heads, "head_dim": head_dim})
 
+    def _batch(self, batch: Batch):
+        if batch._device not in (None, self._dev):
+            raise InvalidArgument(f"batch: on device {batch._device}, the runtime is on {self._dev}")
+        return batch._ref
+
     def Write(self, batch: Batch, k: Rows, v: Rows, stream: int = 0) -> None:
         n, err = batch.n_rows, _local.err
-        st = self._write(self._h, batch._ref, _rows("k", k, self._dev, n, self._kv), _rows("v", v, self._dev, n, self._kv), stream, err, _ERRCAP)
+        st = self._write(self._h, self._batch(batch), _rows("k", k, self._dev, n, self._kv), _rows("v", v, self._dev, n, self._kv), stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
     def Read(self, batch: Batch, k: Rows, v: Rows, stream: int = 0) -> None:
         n, err = batch.n_rows, _local.err
-        st = self._read(self._h, batch._ref, _rows("k", k, self._dev, n, self._kv), _rows("v", v, self._dev, n, self._kv), stream, err, _ERRCAP)
+        st = self._read(self._h, self._batch(batch), _rows("k", k, self._dev, n, self._kv), _rows("v", v, self._dev, n, self._kv), stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
-    def Attend(self, batch: Batch, q: Rows, out: Rows, scratch: Scratch, scale=None, causal: bool = True, window: int = 0, lse: int = 0, stream: int = 0) -> None:
-        """`scale` defaults to 1 / sqrt(head_dim); `lse`: device f32 [n_rows][q_heads], or 0."""
+    def Attend(self, batch: Batch, q: Rows, out: Rows, scratch: Scratch, scale=None, causal: bool = True, window: int = 0, lse=0, stream: int = 0) -> None:
+        """`scale` defaults to 1 / sqrt(head_dim); `lse`: f32 [n_rows][q_heads], or 0."""
         if not 0 <= window <= 0xFFFFFFFF:
             raise InvalidArgument(f"window {window} is out of range")
         n, err = batch.n_rows, _local.err
-        st = self._attend(self._h, scratch._h if scratch is not None else None, batch._ref, _rows("q", q, self._dev, n, self._q), self._scale if scale is None else scale,
-                          1 if causal else 0, window, _rows("out", out, self._dev, n, self._q), lse, stream, err, _ERRCAP)
+        st = self._attend(self._h, scratch._h if scratch is not None else None, self._batch(batch), _rows("q", q, self._dev, n, self._q), self._scale if scale is None else scale,
+                          1 if causal else 0, window, _rows("out", out, self._dev, n, self._q), _address("lse", lse, "f32", n * self._q[1], self._dev), stream, err, _ERRCAP)
         if st:
             _check(st, err)
 
