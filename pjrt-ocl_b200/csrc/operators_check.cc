@@ -73,7 +73,7 @@ std::string CheckRopeDesc(const b2_rope_desc *d) {
   if (d->rot_dim && !d->frequencies) return "null frequencies";
   for (uint32_t i = 0; i < d->rot_dim / 2; ++i)
     if (!isfinite(d->frequencies[i])) return "frequency " + N(i) + " is not finite";
-  if (d->rot_dim && !isfinite(d->magnitude)) return "magnitude must be finite";
+  if (d->rot_dim && !isfinite(static_cast<float>(d->magnitude))) return "magnitude must be finite in f32";
   return "";
 }
 

@@ -1,8 +1,10 @@
-"""Which rows lie over each other, without a device: the operators' checks against the bytes of all small layouts."""
+"""What the operators refuse, without a device: rows that lie over each other (against the bytes of all small layouts), values that f32 does not hold."""
 import os
 import subprocess
 
-from conftest import ROOT
+import pytest
+
+from conftest import ROOT, package
 
 CSRC = os.path.join(ROOT, "pjrt-ocl_b200", "csrc")
 
@@ -13,3 +15,13 @@ def test_rows_over_each_other(tmp_path):
                     os.path.join(CSRC, "operators_check.cc"), "-o", exe], check=True)
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr
+
+
+def test_a_magnitude_that_f32_does_not_hold():
+    """It is multiplied in f32: an infinity there would make sines of 0 a NaN."""
+    vm = package()
+    for magnitude in (1e39, -1e300, float("nan"), float("inf")):
+        with pytest.raises(vm.InvalidArgument, match="magnitude"):
+            vm.Rope.Create(None, 64, 1, 1, "bf16", magnitude=magnitude)
+    with pytest.raises(vm.InvalidArgument, match="null runtime"):
+        vm.Rope.Create(None, 64, 1, 1, "bf16", magnitude=3e38)
