@@ -236,7 +236,8 @@ void b2_scratch_destroy(b2_scratch *scratch);
  * A head's row x (head_dim values) becomes, with `norm`, y = x * w / sqrt(mean(x^2) + eps), else y = x. Its first
  * rot_dim values are turned by pairs: (a, b) = (y[i], y[i + rot_dim/2]), or (y[2i], y[2i+1]) when `interleaved`,
  * by the angle position * frequencies[i]: a' = m (a cos - b sin), b' = m (a sin + b cos), m = magnitude. The rest
- * passes. In f32, the angle in 64 bits (any int32 position is exact to the last f32 bit of its sine), one rounding. */
+ * passes. In f32, the angle in 64 bits, one rounding. Sine and cosine are off by 2^-22 at most where position *
+ * frequency is below 2^27, by 2^-20 at the last int32 position and a frequency of 1. */
 typedef struct b2_rope b2_rope;
 typedef struct {
   uint32_t head_dim, rot_dim;      /* even; head_dim <= 256, rot_dim <= head_dim, 0 = the norms alone */

@@ -6,7 +6,8 @@
 //
 // Bound: HBM. Every row is read once and written once (backward: x and dy read, dx written).
 // A warp takes a token (few tokens: a part of its heads). It works out the token's angles once, in 64-bit turns (position x turns, less the
-// nearest whole number: exact for every int32 position; sine and cosine of the rest in f32), and keeps those of its pairs in registers for all
+// nearest whole number; sine and cosine of the rest in f32. Quotient and product are off by 2^-53 each: 2^-52 of the angle, 2^-25 at 2^27 and 2^-21 at 2^31;
+// the rest as f32 by 2^-26 turns, 2^-23.3; f32's sine by some 2^-24), and keeps those of its pairs in registers for all
 // heads. A row belongs to up to 32 threads; a thread holds V pairs of it, both halves of each, so that neither layout needs an exchange
 // between threads: the half layout is two V-wide accesses rot/2 apart, the neighbouring one two that touch. What lies behind
 // rot is treated the same with no angle. V is as wide as the addresses, strides and rot allow up to 16 bytes. The next rows are on the

@@ -2,6 +2,8 @@
 
 Tolerances count as those of the other operator tests; rows of bf16 over 8-bit pages round their values to 16 bits beside the
 weights, so there they are twice as wide (`_tol`)."""
+from fractions import Fraction
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -356,3 +358,36 @@ def test_results_over_inputs_or_themselves_are_refused(rt, scratch):
     one.Apply(1, pos.data_ptr(), vm.Rows(x[0].data_ptr(), "bf16", (1, 1, 64), (0, 0)), vm.Rows(x[1].data_ptr(), "bf16", (1, 1, 64), (7, 3)), vm.Rows(x[0].data_ptr(), "bf16", (1, 1, 64), (1, 1)),
               vm.Rows(x[2].data_ptr(), "bf16", (1, 1, 64)))
     assert torch.equal(x[2], x[1]) and p.cache.Status()["code"] == 0
+
+
+def _sine_and_cosine(position, frequency):
+    """To 2^-80 or so: the angle as a fraction, pi to 60 digits, series."""
+    pi = Fraction(3141592653589793238462643383279502884197169399375105820974944, 10 ** 60)
+    angle = (position * Fraction(frequency)) % (2 * pi)
+    angle = Fraction(round(angle * 2 ** 120), 2 ** 120)
+    out = []
+    for term, k in ((angle, 1), (Fraction(1), 0)):
+        total = Fraction(0)
+        while abs(term) > Fraction(1, 2 ** 90):
+            total += term
+            k += 2
+            term = Fraction(round(-term * angle * angle / (k * (k - 1)) * 2 ** 120), 2 ** 120)
+        out.append(float(total))
+    return out
+
+
+def test_sines_of_far_positions(rt):
+    """Rows of pairs (1, 0) in f32 come back as cosine and sine."""
+    vm = package()
+    freq = [1.0, 0.5 ** 0.5, 10000.0 ** -0.25, 1e-2, 1.0 - 2.0 ** -53, 3e-4, 1e-4, 2.0 ** -20]
+    pos = [0, 1, 17, 131071, 999999, 2 ** 24 + 1, 2 ** 27 - 1, -(2 ** 27) + 3, 2 ** 30 + 12345, 2 ** 31 - 1, -(2 ** 31), 1686629713 // 5]
+    rope = vm.Rope.Create(rt, 16, 1, 0, "f32", frequencies=freq)
+    x = torch.zeros(len(pos), 1, 16, device="cuda")
+    x[..., :8] = 1.0
+    out = torch.empty_like(x)
+    rope.Apply(len(pos), torch.tensor(pos, dtype=torch.int32, device="cuda"), vm.Rows.Of(x), None, vm.Rows.Of(out), None, stream=torch.cuda.current_stream().cuda_stream)
+    for i, p in enumerate(pos):
+        for j, f in enumerate(freq):
+            sine, cosine = _sine_and_cosine(p, f)
+            off = max(abs(float(out[i, 0, j]) - cosine), abs(float(out[i, 0, 8 + j]) - sine))
+            assert off <= (2.0 ** -22 if abs(p) * f < 2 ** 27 else 2.0 ** -20), (p, f, off * 2 ** 24)
