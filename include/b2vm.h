@@ -251,7 +251,8 @@ typedef struct {
 } b2_rope_desc;
 /* Frequencies base^(-2i/rot_dim), and their forms for contexts longer than the one trained on (`factor` times):
  * LINEAR divides them by factor; STRETCH takes base * factor^(rot_dim/(rot_dim-2)); PARTS leaves those that make
- * `fast` turns or more over original_length, divides those that make `slow` or fewer, and blends between. */
+ * `fast` turns or more over original_length, divides those that make `slow` or fewer, and blends between, linearly in
+ * turns. (Blended over the pairs' index instead, as some checkpoints have it, the frequencies are others: hand those in.) */
 enum { B2_ROPE_PLAIN = 0, B2_ROPE_LINEAR = 1, B2_ROPE_STRETCH = 2, B2_ROPE_PARTS = 3 };
 b2_status b2_rope_frequencies(uint32_t rot_dim, double base, int scaling, double factor, double original_length,
                               double slow, double fast, double *out, size_t out_cap, char *err, size_t err_cap);
@@ -319,8 +320,16 @@ b2_status b2_cache_read(b2_cache *cache, const b2_batch *batch, const b2_rows *k
  * that a row does not see never reach it, whatever they are. A row that sees nothing gives zeros. lse (may be NULL):
  * f32 [n_rows][q_heads], the logarithm of the softmax's sum (-inf for a row that sees nothing). Rows are B2_F16 or
  * B2_BF16. 0 < scale <= 1e38; max_rows x query heads to a cache head below 2^31. out must not lie over q, nor its rows
- * or heads over each other. e4m3 scales
- * count in full from 2^-80 to 2^103. */
+ * or heads over each other.
+ * Sums, maxima and logarithms are f32. What the products take has 16 bits, each rounding off by half a step at most
+ * (bf16 2^-8, f16 2^-11 of the value):
+ *   single tokens (max_rows x query heads to a cache head <= 16): the weights as two values each, so that nothing is lost
+ *     beside f32; bf16 rows over e4m3 pages: weight x V's scale as one f16;
+ *   chunks, 16-bit pages: the weights as one value of the rows' type; e4m3 pages: f16 rows: weight x V's scale as one f16;
+ *     bf16 rows: the weights as one f16, V x its scale as another.
+ * e4m3 scales: each from 2^-80 to 2^103 by itself. Of the keys that a row sees together, one whose V scale is 2^19 below the
+ * largest still counts in full, one 2^31 below no more, whatever its weight (f16 holds no less); chunks of bf16 rows: in full
+ * down to 2^14 below the largest of its neighbours, 16 keys side by side. */
 b2_status b2_cache_attend(b2_cache *cache, b2_scratch *scratch, const b2_batch *batch, const b2_rows *q, float scale,
                           int causal, uint32_t window, const b2_rows *out, void *lse, void *cuda_stream, char *err,
                           size_t err_cap);

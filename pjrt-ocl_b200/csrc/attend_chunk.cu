@@ -17,7 +17,7 @@
 // of the cache is found by itself (one page number a row, looked up a block ahead).
 // 8-bit pages: codes become f16 on their way into the ring. K's exactly, its scales go onto the scores, in f32; q is scaled by a power of two
 // for each row to fit f16. V's, for bf16 rows, times their key's scale relative to a power of two above the scales of 16 keys side by side
-// (rounded to 2^-12 of themselves, as the weights are), the power goes onto the weights; f16 rows' results are rounded no coarser than that
+// (rounded to 2^-11 of themselves, as the weights are), the power goes onto the weights; f16 rows' results are rounded no coarser than that
 // themselves, so for them V is exact, too, and its scales go onto the weights before those are rounded. (A warp that reads 64 scales waits
 // for 8 KB of them: 876 us instead of 785 for 2048 rows behind 14336 of 32 heads of 128 values.) The codes of a block ahead wait in
 // shared memory as they are, copied asynchronously (in registers: 1045 us).

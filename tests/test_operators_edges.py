@@ -391,3 +391,25 @@ def test_sines_of_far_positions(rt):
             sine, cosine = _sine_and_cosine(p, f)
             off = max(abs(float(out[i, 0, j]) - cosine), abs(float(out[i, 0, 8 + j]) - sine))
             assert off <= (2.0 ** -22 if abs(p) * f < 2 ** 27 else 2.0 ** -20), (p, f, off * 2 ** 24)
+
+
+@pytest.mark.parametrize("row_dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows, q_heads", [(1, 4), (4, 8), (40, 4), (200, 2)])
+@pytest.mark.parametrize("apart, other", [(2.0 ** 19, 32), (2.0 ** 14, 1)])
+def test_a_small_v_scale_under_all_the_weight(rt, scratch, row_dtype, rows, q_heads, apart, other):
+    """A key that has the weight counts in full beside one that has none and a V scale `apart` times larger."""
+    p = Paged(rt, [rows], [100], dtype="e4m3", row_dtype=row_dtype, heads=2, q_heads=q_heads, dim=64, page=16, seed=6)
+    c = 35
+    p.pages[0].view(torch.uint8)[...] = 0x30                     # scores alike, but for key c's
+    p.pages[0].view(torch.uint8)[_place(p, 0, c)] = 0x50
+    p.scales[0].fill_(1.0)
+    p.scales[1].fill_(1.0 / 448)
+    p.scales[1][_place(p, 0, c + other)] *= apart
+    q = torch.full((rows, q_heads, 64), 1.0, device="cuda").to(normal((1,), row_dtype, 0).dtype)
+    want, want_lse, tol = p.attend(q, 0.125)                     # (8 x (16 - 0.5) = 60 and more between them: e^-60 x 2^19 is nothing)
+    assert _near(want, p.values(0, 1)[c].repeat_interleave(q_heads // 2, 0).expand_as(want), 2.0 ** -40)
+    o, lse = _call(p, scratch, q)
+    assert p.cache.Status()["code"] == 0
+    # values below f16's smallest normal one are off by half of its smallest step, 2^-25: of V, which is held 2^7 higher, over a power above its 16 keys' scales
+    low = 2.0 ** -32 * 2 * float(p.scales[1].max()) if other == 1 else 0.0
+    assert _near(o, want, _tol(p, want, tol) + low) and _near(lse, want_lse, 2.0 ** -19 * (1 + want_lse.abs()))
