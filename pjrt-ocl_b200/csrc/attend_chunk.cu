@@ -19,7 +19,7 @@
 // for each row to fit f16. V's, for bf16 rows, times their key's scale relative to a power of two above the scales of 16 keys side by side
 // (rounded to 2^-11 of themselves, as the weights are), the power goes onto the weights; f16 rows' results are rounded no coarser than that
 // themselves, so for them V is exact, too, and its scales go onto the weights before those are rounded. (A warp that reads 64 scales waits
-// for 8 KB of them: 876 us instead of 785 for 2048 rows behind 14336 of 32 heads of 128 values.) The codes of a block ahead wait in
+// for 8 KB of them: 871 us instead of 782 for 2048 rows behind 14336 of 32 heads of 128 values, in a graph.) The codes of a block ahead wait in
 // shared memory as they are, copied asynchronously (in registers: 1045 us).
 //
 // Work: one CTA to an SM. The tiles of the batch in a row, sequence by sequence and head by head, each weighed by the keys it sees and something for its
@@ -27,8 +27,8 @@
 // two blocks of its keys, and a second launch joins the parts. The filling warps walk the run; the others read what they need of a tile
 // from shared memory. The ring runs on from tile to tile.
 //
-// Bound: the tensor cores, under the power cap. 2048 rows behind 14336 of 32 heads of 128 values, bf16: 464 us, 80 % of the rate that a large
-// product sustains; without exponentials and copies it would be 356.
+// Bound: the tensor cores, under the power cap. 2048 rows behind 14336 of 32 heads of 128 values, bf16: 474 us in a graph with L2 warm, 78 % of
+// the rate that a large product sustains (without exponentials and copies it would be 356); 555 us one call after another with L2 cold, 67 %.
 #include <type_traits>
 
 #include "attend_common.cuh"
@@ -366,7 +366,7 @@ static __device__ __forceinline__ void chunk_load(const AttendArgs &a, Walk &wk,
   const bool in_hd = sub * 16u < a.c.hd * (Q8 ? 1u : 2u);
   auto copy = [&](const uint8_t *pages, uint32_t i, int64_t off, uint32_t mask) {
     const uint32_t dst = base + Sh::kRing + (i % NS) * Sh::kBlock;
-    // (all 16 in a row are more code to fetch: 477 us instead of 464; two at a time 479)
+    // (all 16 in a row are more code to fetch: 477 us instead of 464 in a graph; two at a time 479)
 #pragma unroll 4
     for (uint32_t k = 0; k < N; ++k) {
       const uint32_t r = k * AT + r1;
@@ -980,7 +980,8 @@ __global__ void __launch_bounds__(ChunkWarps<Q8>::kThreads, 1) b2_attend_chunk(c
   }
 }
 
-// Tiles that lie in the runs of several CTAs: a warp to a row, the parts in their order. For each CTA whose run ends inside a tile that it began,
+// Tiles that lie in the runs of several CTAs (registers for two CTAs to an SM: with fewer the row's loop spills, 42 us instead of 40 for 128 rows behind
+// 4000 keys): a warp to a row, the parts in their order. For each CTA whose run ends inside a tile that it began,
 // a CTA of 32 rows at a time. (What to join was written down by the launch before: worked out here again, with 64-bit quotients in every warp, it
 // was 37 us for 2048 rows behind 14336 of 32 heads of 128 values.)
 constexpr uint32_t kJoinThreads = 256, kJoinRows = 32, kMostRuns = 1024;

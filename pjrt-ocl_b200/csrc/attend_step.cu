@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(NW * 32, PerSm(NW)) b2_attend_step(const __gri
   uint32_t t_begin = tile_at(u0, x0, cw.nt), t_end = tile_at(u1, x0, cw.nt);
   if (t_begin >= t_end) return;                           // (a run that is shorter than what an item costs beside its tiles)
 
-  // ---- the warp's copies: its tiles are w, w + 12, .. of the CTA's ----
+  // ---- the warp's copies: its tiles are w, w + NW, .. of the CTA's ----
   uint8_t *const ring = sm + w * (kStages * Sh::kStage);
   const uint32_t ring_s = smem_addr(ring);
   Walk<KT> pw = cw;                                       // the item of the next tile to fetch
